@@ -45,6 +45,9 @@ enum tab_status {
   TAB_ERR_TIMEOUT = -6      /* a bounded device-side wait gave up (read back via tab_gmm_status) */
 };
 
+/* activations of the dense operators; GELU by the error function or by its tanh approximation */
+enum tab_act { TAB_ACT_NONE = 0, TAB_ACT_RELU = 1, TAB_ACT_GELU = 2, TAB_ACT_GELU_TANH = 3, TAB_ACT_SILU = 4 };
+
 enum tab_dtype { TAB_I8 = 1, TAB_I32 = 3, TAB_I64 = 4, TAB_F16 = 5, TAB_F32 = 6, TAB_BF16 = 15 };
 
 /* Library version (major*10000 + minor*100 + patch).  Nearest reference analogue: the pybind module
@@ -442,6 +445,63 @@ TAB_API int tab_grouped_matmul_finalize_routing(const int8_t* x, const int8_t* p
                                         size_t workspace_bytes, int64_t expected_rows_per_group, tab_stream_t stream);
 TAB_API int tab_gmm_status(int* status_host, tab_stream_t stream);
 TAB_API int tab_gmm_status_reset(tab_stream_t stream);
+
+/* ---- dense 16-bit products: the shared expert, projections, their gradients ------------------------------------------------
+ * No counterpart on the reference's path (its shared experts are dense modules beside the routed ones); they serve
+ * npu_gated_ffn, npu_linear_act and npu_checkpoint_weight_grad of this package.
+ *
+ * dtype 5 (fp16) or 15 (bf16) for every 16-bit tensor of a call; accumulators and epilogues are fp32.  All pointers 16-byte
+ * aligned, leading dimensions and output features (N, H, I) multiples of 8; rows and the contraction are free.  An operand with `mn` = 0 is contiguous
+ * along the contraction (element (i, k) at i * ld + k), with `mn` = 1 along its own index (k * ld + i).
+ * keep / keep_q + keep_scale (all null: nothing is kept) receive the values before the activation for the backward pass,
+ * 16-bit, or int8 with one fp32 scale per row and 64 values (keep_ld a multiple of 64, scales [M, keep_ld / 64]; see
+ * tab_checkpoint_quant).  A kept row of the gated forms holds the gate, then the up values; with 8 bits either half begins at a multiple
+ * of 64 (the up values at I rounded up).
+ *
+ * tab_dense_matmul:       out[M, N] = act(A B + bias[N]) + residual[M, N], A [M, K], B [K, N] (index n)
+ * tab_gated_matmul:       h[M, I] = act(z[:, :I]) * z[:, I:], z = x weight + bias[2 I], weight [K, 2 I]
+ * tab_gated_matmul_grad:  dh = the product of dy [M, K] with the operand weight (index i of I, contraction over K: the second
+ *                         projection's [I, K] weight has mn = 0 here when its rows are contiguous);
+ *                         from the kept gate g and up u: dz[M, 2 I] = [dh u act'(g) | dh act(g)] and h = act(g) u again
+ * tab_gated_ffn:          y[M, H] = (act(z[:, :I]) * z[:, I:]) w2 + bias2[H] + residual, z = x w1 + bias1; h lives in the workspace */
+TAB_API int tab_dense_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes);
+TAB_API int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M,
+                             int64_t N, int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q,
+                             float* keep_scale, int64_t keep_ld, void* out, void* workspace, size_t workspace_bytes,
+                             tab_stream_t stream);
+TAB_API int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
+                             int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld,
+                             void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream);
+TAB_API int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M,
+                                  int64_t I, int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale,
+                                  int64_t keep_ld, void* dz, void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream);
+TAB_API int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes);
+TAB_API int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ldw1, int w1_mn, const void* w2, int64_t ldw2, int w2_mn,
+                          int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual,
+                          int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* y, void* workspace,
+                          size_t workspace_bytes, tab_stream_t stream);
+TAB_API int tab_dense_status(int* status_host, tab_stream_t stream);
+TAB_API int tab_dense_status_reset(tab_stream_t stream);
+
+/* ---- activations kept in 8 bits, and the elementwise half of the backward pass ----
+ * tab_checkpoint_quant: per row and 64 consecutive values scale = amax / 127, q = rint(x / scale) (IEEE division, ties to even; a block of
+ * zeros: scale 0, q 0; a block with a value that is not finite: scale NaN, q 0, so that it comes back as NaN).
+ * x [rows, cols] of dtype 5, 6 or 15 with ldx elements between rows; q int8 [rows, ldq]; scale fp32 [rows, lds], lds >= ceil(cols / 64).
+ * tab_checkpoint_dequant: y = q * scale, rounded once to dtype 5, 6 or 15; columns [cols, pad_cols) of y become 0.
+ * tab_act_grad: dz[M, N] = dy[M, N] act'(z), z kept in 16 bits (keep) or 8 (keep_q, keep_scale); dz null: nothing is stored (then act
+ *   must be 0).  column_sums null, or fp32 [splits, N]: partial column sums of dz, one row per slice of the rows, summed by
+ *   tab_column_sums into out[N] of `dtype` in slice order; the number of slices is tab_act_grad_splits(M, N).
+ * tab_copy_2d: 16-bit elements; dst(r, c) = src(r, c) inside [src_rows, src_cols), 0 elsewhere in [dst_rows, dst_cols); any strides. */
+TAB_API int tab_checkpoint_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
+                                 int64_t lds, tab_stream_t stream);
+TAB_API int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t lds, int64_t rows, int64_t cols, void* y,
+                                   int dtype, int64_t ldy, int64_t pad_cols, tab_stream_t stream);
+TAB_API int tab_act_grad_splits(int64_t M, int64_t N, size_t* splits);
+TAB_API int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, int64_t N, int act, const void* keep, const int8_t* keep_q,
+                         const float* keep_scale, int64_t keep_ld, void* dz, float* column_sums, tab_stream_t stream);
+TAB_API int tab_column_sums(const float* column_sums, int64_t splits, int64_t N, void* out, int dtype, tab_stream_t stream);
+TAB_API int tab_copy_2d(const void* src, int64_t src_row_stride, int64_t src_col_stride, int64_t src_rows, int64_t src_cols, void* dst,
+                        int64_t dst_row_stride, int64_t dst_col_stride, int64_t dst_rows, int64_t dst_cols, tab_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,395 @@
+// Host side of the dense 16-bit GEMMs: argument checks, tensor maps, the choice between the narrow and the pair kernel, the
+// split of tiles, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
+#include <stdlib.h>
+
+#include "dense_common.cuh"
+#include "dense_narrow.cuh"
+#include "dense_pair.cuh"
+
+namespace tab {
+
+typedef CUresult (*DenseEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static DenseEncodeFn dense_encode_fn() {
+  static DenseEncodeFn fn = []() -> DenseEncodeFn {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<DenseEncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+static int dense_sms() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kNumSMs;
+  if (cached[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) n = kNumSMs;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+static long long dense_wait_cycles() {
+  static const long long cycles = []() {
+    long long ms = 2000;
+    if (const char* f = getenv("TAB_GMM_WAIT_MS")) {
+      const long long v = atoll(f);
+      if (v >= 1 && v <= 600000) ms = v;
+    }
+    return ms * kDnCyclesPerMs;
+  }();
+  return cycles;
+}
+
+// One operand: `rows` indices of the product times `depth` contraction elements, 16-bit, `ld` elements between lines.
+// mn = 0: a line is one index (contiguous along the contraction); mn = 1: a line is one contraction element.
+struct DenseOperand {
+  const void* ptr;
+  int64_t ld, rows, depth;
+  int mn;
+};
+
+static int check_operand(const char* op, const char* name, const DenseOperand& o) {
+  if (!o.ptr) return fail(TAB_ERR_BAD_ARG, "%s: null pointer (%s)", op, name);
+  if (!aligned16(o.ptr) || o.ld % 8 != 0)
+    return fail(TAB_ERR_ALIGNMENT, "%s: %s must be 16-byte aligned with a leading dimension that is a multiple of 8 (got %lld)", op, name, (long long)o.ld);
+  const int64_t line = o.mn ? o.rows : o.depth, lines = o.mn ? o.depth : o.rows;
+  if (o.ld < line && lines > 1) return fail(TAB_ERR_BAD_ARG, "%s: leading dimension %lld of %s is shorter than a line (%lld)", op, (long long)o.ld, name, (long long)line);
+  return TAB_OK;
+}
+
+// box_rows: product indices per box (64, or the token columns of the narrow kernel)
+static int make_map(const char* op, const DenseOperand& o, int box_rows, CUtensorMap* map) {
+  DenseEncodeFn enc = dense_encode_fn();
+  if (!enc) return fail(TAB_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from the driver", op);
+  const int64_t line = o.mn ? o.rows : o.depth, lines = o.mn ? o.depth : o.rows;
+  cuuint64_t dims[2] = {(cuuint64_t)line, (cuuint64_t)lines};
+  cuuint64_t strides[1] = {(cuuint64_t)((o.ld > 0 ? o.ld : 8) * 2)};
+  cuuint32_t box[2] = {64, (cuuint32_t)(o.mn ? kDnBlockK : box_rows)};
+  cuuint32_t es[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TAB_ERR_CUDA, "%s: tensor map rejected (CUresult %d)", op, (int)r);
+  return TAB_OK;
+}
+
+// ---- split of tiles (pair kernel) ----
+struct DensePlan {
+  int row_tiles, col_tiles, num_kb, pairs, sk_tiles;
+  size_t partial_bytes, arrival_bytes;
+};
+
+// Time in blocks of the contraction: whole tiles only take ceil(tiles / pairs) turns of num_kb.  Splitting the last, partly
+// filled turn (or that and one full turn) evenly costs its share plus the joins: about 8 blocks' time to store a part and 4
+// per part that the last CTA adds up.
+static DensePlan dense_plan(int64_t M, int64_t col_tiles, int64_t depth) {
+  DensePlan d = {};
+  d.row_tiles = (int)((M + 255) / 256);
+  d.col_tiles = (int)col_tiles;
+  d.num_kb = (int)((depth + kDnBlockK - 1) / kDnBlockK);
+  const int max_pairs = dense_sms() / 2;
+  const int64_t tiles = static_cast<int64_t>(d.row_tiles) * d.col_tiles;
+  d.pairs = (int)(tiles < max_pairs ? tiles : max_pairs);
+  const int64_t full = tiles / max_pairs, rem = tiles % max_pairs;
+  if (rem == 0) return d;
+  double best = static_cast<double>(full + 1) * d.num_kb;
+  for (int more = 0; more < 2; ++more) {
+    if (more > full) break;
+    const int64_t sk = rem + more * max_pairs;
+    if (sk * d.num_kb < 2 * max_pairs) continue;                   // every pair holds work
+    const double parts = static_cast<double>((max_pairs + sk - 1) / sk) + 1.0;
+    const double cost = static_cast<double>(full - more) * d.num_kb + static_cast<double>(sk) * d.num_kb / max_pairs + 8.0 + 4.0 * parts;
+    if (cost < best) {
+      best = cost;
+      d.sk_tiles = (int)sk;
+    }
+  }
+  if (d.sk_tiles) {
+    d.pairs = max_pairs;
+    d.partial_bytes = static_cast<size_t>(max_pairs) * 2 * 2 * kDpPartFloats * sizeof(float);
+    d.arrival_bytes = (static_cast<size_t>(d.sk_tiles) * 2 * sizeof(int) + 255) / 256 * 256;
+  }
+  return d;
+}
+
+template <typename T, int EPI>
+static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMap& mb, const DenseParams& p, int pairs, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDpSmemBytes);
+  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: shared memory opt-in failed: %s", op, cudaGetErrorString(e));
+  dense_pair_kernel<T, EPI><<<2 * pairs, kDpThreads, kDpSmemBytes, st>>>(ma, mb, p);
+  return check_launch(op);
+}
+
+template <int EPI>
+static int launch_pair_epi(const char* op, int dtype, const DenseOperand& a, const DenseOperand& b, DenseParams& p, const DensePlan& plan, void* ws,
+                           size_t ws_bytes, cudaStream_t st) {
+  p.num_kb = plan.num_kb;
+  p.row_tiles = plan.row_tiles;
+  p.col_tiles = plan.col_tiles;
+  p.sk_tiles = plan.sk_tiles;
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
+  p.idesc = ptx::idesc_f16(256, kDpCols, dtype == TAB_BF16 ? 1 : 0, a.mn, b.mn);
+  p.wait_cycles = dense_wait_cycles();
+  if (plan.sk_tiles) {
+    if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return fail(TAB_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", op);
+    if (ws_bytes < plan.partial_bytes + plan.arrival_bytes)
+      return fail(TAB_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", op, ws_bytes, plan.partial_bytes + plan.arrival_bytes);
+    p.arrivals = static_cast<int*>(ws);
+    p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.arrival_bytes);
+    const cudaError_t e = cudaMemsetAsync(ws, 0, plan.arrival_bytes, st);
+    if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: memset: %s", op, cudaGetErrorString(e));
+  }
+  CUtensorMap ma, mb;
+  int rc = make_map(op, a, 64, &ma);
+  if (rc == TAB_OK) rc = make_map(op, b, 64, &mb);
+  if (rc != TAB_OK) return rc;
+  return dtype == TAB_BF16 ? launch_pair_t<__nv_bfloat16, EPI>(op, ma, mb, p, plan.pairs, st)
+                           : launch_pair_t<__half, EPI>(op, ma, mb, p, plan.pairs, st);
+}
+
+// ---- narrow kernel ----
+// Up to 128 rows the weights are read once either way and the narrow kernel pads nothing to 256 rows.
+static bool use_narrow(int64_t M, const DenseOperand& x) { return M <= kNwMaxTokens && x.mn == 0; }
+
+template <typename T, int EPI>
+static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensorMap& mx, const DenseParams& p, int tiles, cudaStream_t st) {
+  const int smem = 1024 + p.stages * dense_narrow_stage_bytes(p.nt) + kNwCtrlBytes;
+  cudaError_t e = cudaFuncSetAttribute(dense_narrow_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNwSmemTarget);
+  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: shared memory opt-in failed: %s", op, cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.split));
+  cfg.blockDim = dim3(kNwThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.dependent ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, dense_narrow_kernel<T, EPI>, mw, mx, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TAB_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
+  return check_launch(op);
+}
+
+template <int EPI>
+static int launch_narrow_epi(const char* op, int dtype, const DenseOperand& x, const DenseOperand& w, DenseParams& p, cudaStream_t st) {
+  p.num_kb = (int)((x.depth + kDnBlockK - 1) / kDnBlockK);
+  p.nt = 16;
+  while (p.nt < p.M) p.nt *= 2;
+  const int tiles = EPI == kEpiGlu ? (p.N + 63) / 64 : (p.N + 127) / 128;
+  // two CTAs per SM as long as each keeps a few blocks of the contraction
+  p.split = 1;
+  while (p.split < kNwMaxSplit && tiles * p.split * 2 <= 2 * dense_sms() && p.split * 2 * 4 <= p.num_kb) p.split *= 2;
+  p.stages = (kNwSmemTarget - 1024 - kNwCtrlBytes) / dense_narrow_stage_bytes(p.nt);
+  if (p.stages > kNwMaxStages) p.stages = kNwMaxStages;
+  p.a_mn = w.mn;
+  p.b_mn = 0;
+  p.idesc = ptx::idesc_f16(128, p.nt, dtype == TAB_BF16 ? 1 : 0, w.mn, 0);
+  p.wait_cycles = dense_wait_cycles();
+  CUtensorMap mw, mx;
+  int rc = make_map(op, w, 64, &mw);
+  if (rc == TAB_OK) rc = make_map(op, x, p.nt, &mx);
+  if (rc != TAB_OK) return rc;
+  return dtype == TAB_BF16 ? launch_narrow_t<__nv_bfloat16, EPI>(op, mw, mx, p, tiles, st)
+                           : launch_narrow_t<__half, EPI>(op, mw, mx, p, tiles, st);
+}
+static_assert(kNwMaxTokens * 128 * 4 <= 3 * dense_narrow_stage_bytes(kNwMaxTokens), "the parts of a tile overlay the ring");
+static_assert(1024 + 3 * dense_narrow_stage_bytes(kNwMaxTokens) + kNwCtrlBytes <= kNwSmemTarget, "three stages at the widest tile");
+
+// ---- checks ----
+static int check_dense(const char* op, int dtype, int64_t M, int64_t N, int64_t K, int act) {
+  if (M < 0 || N <= 0 || K <= 0) return fail(TAB_ERR_BAD_ARG, "%s: M=%lld N=%lld K=%lld", op, (long long)M, (long long)N, (long long)K);
+  if (dtype != TAB_BF16 && dtype != TAB_F16) return fail(TAB_ERR_UNSUPPORTED, "%s: dtype %d (want 5 or 15)", op, dtype);
+  if (act < TAB_ACT_NONE || act > TAB_ACT_SILU) return fail(TAB_ERR_BAD_ARG, "%s: activation %d", op, act);
+  if (N % 8 != 0) return fail(TAB_ERR_ALIGNMENT, "%s: %lld output features (must be a multiple of 8)", op, (long long)N);
+  if (M > (1LL << 30) || N > (1LL << 24) || K > (1LL << 30)) return fail(TAB_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  if (((M + 255) / 256) * ((N + 127) / 128) > (1LL << 28)) return fail(TAB_ERR_UNSUPPORTED, "%s: too many tiles", op);
+  return TAB_OK;
+}
+
+static int check_keep(const char* op, const void* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld, int64_t width) {
+  if (keep && keep_q) return fail(TAB_ERR_BAD_ARG, "%s: keep either 16-bit or 8-bit values", op);
+  if (keep_q && !keep_scale) return fail(TAB_ERR_BAD_ARG, "%s: 8-bit values need their scales", op);
+  if ((keep || keep_q) && (keep_ld < width || keep_ld > (1LL << 30))) return fail(TAB_ERR_BAD_ARG, "%s: kept rows hold %lld values, %lld are needed", op, (long long)keep_ld, (long long)width);
+  if ((keep && (!aligned16(keep) || keep_ld % 8 != 0)) || (keep_q && (!aligned16(keep_q) || keep_ld % kKeepBlock != 0)))
+    return fail(TAB_ERR_ALIGNMENT, "%s: kept values must be 16-byte aligned with rows of a multiple of 8 (8-bit: 64) values", op);
+  return TAB_OK;
+}
+
+static int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
+
+static int check_epilogue_ptrs(const char* op, const void* bias, const void* residual, const void* out) {
+  if (!out) return fail(TAB_ERR_BAD_ARG, "%s: null output", op);
+  if (!aligned16(out) || !aligned16(bias) || !aligned16(residual)) return fail(TAB_ERR_ALIGNMENT, "%s: bias, residual and output must be 16-byte aligned", op);
+  return TAB_OK;
+}
+
+static size_t plan_bytes(const DensePlan& d) { return d.partial_bytes + d.arrival_bytes; }
+static size_t dense_ws(int64_t M, int64_t col_tiles, int64_t depth) { return M > 0 ? plan_bytes(dense_plan(M, col_tiles, depth)) : 0; }
+
+static int gated_matmul(const char* op, const DenseOperand& x, const DenseOperand& w, int dtype, int64_t M, int64_t I, const void* bias, int act,
+                        void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h, void* ws, size_t ws_bytes, cudaStream_t st) {
+  DenseParams p = {};
+  p.M = (int)M;
+  p.N = (int)I;
+  p.act = act;
+  p.bias = bias;
+  p.out = h;
+  p.keep = keep;
+  p.keep_q = keep_q;
+  p.keep_scale = keep_scale;
+  p.keep_ld = (int)keep_ld;
+  p.keep_up = (int)(keep_q ? up64(I) : I);
+  if (use_narrow(M, x)) return launch_narrow_epi<kEpiGlu>(op, dtype, x, w, p, st);
+  return launch_pair_epi<kEpiGlu>(op, dtype, x, w, p, dense_plan(M, (I + 127) / 128, x.depth), ws, ws_bytes, st);
+}
+
+static int linear_matmul(const char* op, const DenseOperand& a, const DenseOperand& b, int dtype, int64_t M, int64_t N, const void* bias,
+                         const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* out, int dependent,
+                         void* ws, size_t ws_bytes, cudaStream_t st) {
+  DenseParams p = {};
+  p.M = (int)M;
+  p.N = (int)N;
+  p.act = act;
+  p.bias = bias;
+  p.residual = residual;
+  p.out = out;
+  p.keep = keep;
+  p.keep_q = keep_q;
+  p.keep_scale = keep_scale;
+  p.keep_ld = (int)keep_ld;
+  p.dependent = dependent;
+  if (use_narrow(M, a)) return launch_narrow_epi<kEpiLinear>(op, dtype, a, b, p, st);
+  return launch_pair_epi<kEpiLinear>(op, dtype, a, b, p, dense_plan(M, (N + 255) / 256, a.depth), ws, ws_bytes, st);
+}
+
+}  // namespace tab
+
+using namespace tab;
+
+extern "C" int tab_dense_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes) {
+  if (!bytes || M < 0 || N <= 0 || K <= 0) return fail(TAB_ERR_BAD_ARG, "dense_matmul: M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  const size_t linear = dense_ws(M, (N + 255) / 256, K), gated = dense_ws(M, (N + 127) / 128, K);
+  *bytes = linear > gated ? linear : gated;
+  return TAB_OK;
+}
+
+extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M, int64_t N,
+                                int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale,
+                                int64_t keep_ld, void* out, void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+  const char* op = "dense_matmul";
+  int rc = check_dense(op, dtype, M, N, K, act);
+  if (rc != TAB_OK || M == 0) return rc;
+  const DenseOperand oa = {a, lda, M, K, a_mn ? 1 : 0}, ob = {b, ldb, N, K, b_mn ? 1 : 0};
+  if ((rc = check_operand(op, "a", oa)) != TAB_OK || (rc = check_operand(op, "b", ob)) != TAB_OK) return rc;
+  if ((rc = check_epilogue_ptrs(op, bias, residual, out)) != TAB_OK) return rc;
+  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, keep_q ? up64(N) : N)) != TAB_OK) return rc;
+  return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0, workspace, workspace_bytes,
+                       as_stream(stream));
+}
+
+extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
+                                int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h,
+                                void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+  const char* op = "gated_matmul";
+  int rc = check_dense(op, dtype, M, I, K, act);
+  if (rc != TAB_OK || M == 0) return rc;
+  const DenseOperand ox = {x, ldx, M, K, 0}, ow = {weight, ldw, 2 * I, K, w_mn ? 1 : 0};
+  if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
+  if ((rc = check_epilogue_ptrs(op, bias, nullptr, h)) != TAB_OK) return rc;
+  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
+  return gated_matmul(op, ox, ow, dtype, M, I, bias, act, keep, keep_q, keep_scale, keep_ld, h, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
+                                     int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld,
+                                     void* dz, void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+  const char* op = "gated_matmul_grad";
+  int rc = check_dense(op, dtype, M, I, K, act);
+  if (rc != TAB_OK || M == 0) return rc;
+  const DenseOperand oa = {dy, lddy, M, K, 0}, ow = {weight, ldw, I, K, w_mn ? 1 : 0};
+  if ((rc = check_operand(op, "dy", oa)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
+  if ((rc = check_epilogue_ptrs(op, dz, nullptr, h)) != TAB_OK) return rc;
+  if (!dz || (!keep && !keep_q)) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
+  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
+  DenseParams p = {};
+  p.M = (int)M;
+  p.N = (int)I;
+  p.act = act;
+  p.out = h;
+  p.dgate = dz;
+  p.keep = const_cast<void*>(keep);
+  p.keep_q = const_cast<int8_t*>(keep_q);
+  p.keep_scale = const_cast<float*>(keep_scale);
+  p.keep_ld = (int)keep_ld;
+  p.keep_up = (int)(keep_q ? up64(I) : I);
+  return launch_pair_epi<kEpiGluGrad>(op, dtype, oa, ow, p, dense_plan(M, (I + 255) / 256, K), workspace, workspace_bytes, as_stream(stream));
+}
+
+// workspace of tab_gated_ffn: the hidden rows h [M, I], then what the split tiles of either product need
+static size_t ffn_h_bytes(int64_t M, int64_t I) { return (static_cast<size_t>(M) * I * 2 + 255) / 256 * 256; }
+
+extern "C" int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes) {
+  if (!bytes || M < 0 || H <= 0 || I <= 0) return fail(TAB_ERR_BAD_ARG, "gated_ffn: M=%lld H=%lld I=%lld", (long long)M, (long long)H, (long long)I);
+  const size_t up = dense_ws(M, (I + 127) / 128, H), down = dense_ws(M, (H + 255) / 256, I);
+  *bytes = ffn_h_bytes(M, I) + (up > down ? up : down);
+  return TAB_OK;
+}
+
+extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ldw1, int w1_mn, const void* w2, int64_t ldw2, int w2_mn,
+                             int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual, int act,
+                             void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* y, void* workspace,
+                             size_t workspace_bytes, tab_stream_t stream) {
+  const char* op = "gated_ffn";
+  int rc = check_dense(op, dtype, M, I, H, act);
+  if (rc == TAB_OK) rc = check_dense(op, dtype, M, H, I, act);
+  if (rc != TAB_OK || M == 0) return rc;
+  const DenseOperand ox = {x, ldx, M, H, 0}, o1 = {w1, ldw1, 2 * I, H, w1_mn ? 1 : 0}, o2 = {w2, ldw2, H, I, w2_mn ? 1 : 0};
+  if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight1", o1)) != TAB_OK || (rc = check_operand(op, "weight2", o2)) != TAB_OK)
+    return rc;
+  if ((rc = check_epilogue_ptrs(op, bias1, residual, y)) != TAB_OK || (rc = check_epilogue_ptrs(op, bias2, nullptr, y)) != TAB_OK) return rc;
+  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
+  size_t need = 0;
+  tab_gated_ffn_workspace_bytes(M, H, I, &need);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return fail(TAB_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", op);
+  if (workspace_bytes < need) return fail(TAB_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", op, workspace_bytes, need);
+  const size_t h_bytes = ffn_h_bytes(M, I);
+  void* rest = static_cast<uint8_t*>(workspace) + h_bytes;
+  const size_t rest_bytes = workspace_bytes - h_bytes;
+  cudaStream_t st = as_stream(stream);
+  rc = gated_matmul(op, ox, o1, dtype, M, I, bias1, act, keep, keep_q, keep_scale, keep_ld, workspace, rest, rest_bytes, st);
+  if (rc != TAB_OK) return rc;
+  const DenseOperand oh = {workspace, I, M, I, 0};
+  return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, rest, rest_bytes, st);
+}
+
+extern "C" int tab_dense_status_reset(tab_stream_t stream) {
+  cudaError_t e = cudaStreamSynchronize(as_stream(stream));
+  const int zero = 0;
+  if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_dense_status, &zero, sizeof(int));
+  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "dense_status_reset: %s", cudaGetErrorString(e));
+  return TAB_OK;
+}
+
+extern "C" int tab_dense_status(int* status_host, tab_stream_t stream) {
+  if (!status_host) return fail(TAB_ERR_BAD_ARG, "dense_status: null pointer");
+  cudaError_t e = cudaStreamSynchronize(as_stream(stream));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(status_host, g_dense_status, sizeof(int));
+  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "dense_status: %s", cudaGetErrorString(e));
+  if (*status_host != 0) return fail(TAB_ERR_TIMEOUT, "dense matmul: device-side wait %d gave up", *status_host);
+  return TAB_OK;
+}

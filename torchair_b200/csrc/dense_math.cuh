@@ -1,0 +1,108 @@
+// Arithmetic of the dense operators: the activations with their derivatives, the 8-bit form of kept activations, packing.
+#pragma once
+
+#include "tab_common.cuh"
+
+namespace tab {
+
+// ---- activations ---------------------------------------------------------------------------------------------------------
+// fp32 throughout.  silu and the tanh form of GELU are both z * sigmoid(u): 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), which
+// needs no cancelling sum for very negative z.
+
+__device__ __forceinline__ float sigmoid_f(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+
+constexpr float kGeluC = 0.7978845608028654f;      // sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+constexpr float kInvSqrt2 = 0.7071067811865476f;
+constexpr float kInvSqrt2Pi = 0.3989422804014327f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == TAB_ACT_RELU) return z < 0.f ? 0.f : z;     // NaN stays NaN
+  if constexpr (ACT == TAB_ACT_SILU) return z * sigmoid_f(z);
+  if constexpr (ACT == TAB_ACT_GELU) return 0.5f * z * (1.0f + erff(z * kInvSqrt2));
+  if constexpr (ACT == TAB_ACT_GELU_TANH) return z * sigmoid_f(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
+  return z;
+}
+
+// value and derivative
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float& a, float& d) {
+  if constexpr (ACT == TAB_ACT_RELU) {
+    a = z < 0.f ? 0.f : z;
+    d = z > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == TAB_ACT_SILU) {
+    const float s = sigmoid_f(z);
+    a = z * s;
+    d = s * (1.0f + z * (1.0f - s));
+  } else if constexpr (ACT == TAB_ACT_GELU) {
+    const float c = 0.5f * (1.0f + erff(z * kInvSqrt2));
+    a = z * c;
+    d = c + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+  } else if constexpr (ACT == TAB_ACT_GELU_TANH) {
+    const float s = sigmoid_f(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
+    a = z * s;
+    d = s + z * s * (1.0f - s) * (2.0f * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
+  } else {
+    a = z;
+    d = 1.f;
+  }
+}
+
+template <int ACT>
+struct ActTag {
+  static constexpr int value = ACT;
+};
+
+// Calls f(ActTag<act>()): the choice is made once per chunk of values, outside the loops over them.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case TAB_ACT_RELU: f(ActTag<TAB_ACT_RELU>()); break;
+    case TAB_ACT_SILU: f(ActTag<TAB_ACT_SILU>()); break;
+    case TAB_ACT_GELU: f(ActTag<TAB_ACT_GELU>()); break;
+    case TAB_ACT_GELU_TANH: f(ActTag<TAB_ACT_GELU_TANH>()); break;
+    default: f(ActTag<TAB_ACT_NONE>()); break;
+  }
+}
+
+// ---- 8-bit blocks --------------------------------------------------------------------------------------------------------
+// 64 values of a row share a scale: scale = amax / 127, q = rint(v / scale).  A block that holds a value that is not
+// finite is kept as q = 0 with the scale NaN, so that it comes back as NaN and an overflow is not lost on the way.
+constexpr int kKeepBlock = 64;
+
+__device__ __forceinline__ RowQuant make_block_quant(float amax, bool finite) {
+  RowQuant rq = make_row_quant(amax);
+  if (!finite) {
+    rq.scale = __int_as_float(0x7fc00000);
+    rq.inv = 0.f;
+    rq.exact = false;
+  }
+  return rq;                         // quant8 stores zeros where !(scale > 0): NaN included
+}
+
+// ---- packing -------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+}  // namespace tab

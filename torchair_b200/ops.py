@@ -579,6 +579,22 @@ def gmm_status_reset(device=None) -> None:
         _lib.call("tab_gmm_status_reset", ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
 
 
+def dense_status(device=None) -> int:
+    """Like gmm_status for the dense matmuls (npu_gated_ffn, npu_linear_act, npu_checkpoint_weight_grad)."""
+    dev = _device(device)
+    with torch.cuda.device(dev):
+        st = ctypes.c_int(0)
+        _lib.call("tab_dense_status", ctypes.byref(st), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        return int(st.value)
+
+
+def dense_status_reset(device=None) -> None:
+    """Clears the dense matmuls' sticky status word (synchronises the current stream)."""
+    dev = _device(device)
+    with torch.cuda.device(dev):
+        _lib.call("tab_dense_status_reset", ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+
+
 def routing_status(device=None) -> int:
     """Synchronises the current stream, returns and clears the routing kernels' status word: bit 0 = an expert id
     outside the valid range was clamped, bit 1 = a row_idx value outside [0, T*K) was skipped.  Does not raise."""
@@ -606,6 +622,12 @@ def check_status(device=None) -> None:
             if st_.value:
                 gmm_status_reset(dev)
             raise RuntimeError(f"grouped GEMM status {st_.value}: {msg}")
+        rc = _lib.load().tab_dense_status(ctypes.byref(st_), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        if rc != 0:
+            msg = _lib.last_error()
+            if st_.value:
+                dense_status_reset(dev)
+            raise RuntimeError(f"dense matmul status {st_.value}: {msg}")
         _lib.call("tab_quant_status", ctypes.byref(st_), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
     st = ep.peer_status()
     if st:
