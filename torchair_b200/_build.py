@@ -9,6 +9,8 @@ from concurrent.futures import ThreadPoolExecutor
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libtorchair_b200.so")
+TORCH_SOURCE = os.path.join(CSRC, "torch_dense.cpp")
+TORCH_LIB_PATH = os.path.join(PKG_DIR, "libtorchair_b200_torch.so")
 SOURCES = ["api.cu", "quant.cu", "routing.cu", "gmm_i8.cu", "gmm_finalize.cu", "ep_peer.cu", "dense.cu", "checkpoint.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
@@ -28,8 +30,27 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_torch_library(force: bool = False) -> str:
+    """Compiles the PyTorch side of the dense operators against the installed torch and links it to libtorchair_b200.so."""
+    api = os.path.join(PKG_DIR, "..", "include", "tab_api.h")
+    if not force and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, api]):
+        return TORCH_LIB_PATH
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    lib_dir = os.path.join(os.path.dirname(os.path.abspath(torch.__file__)), "lib")
+    cuda_home = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [f"-I{d}" for d in include_paths()] + [f"-I{os.path.join(cuda_home, 'include')}", TORCH_SOURCE, "-o", TORCH_LIB_PATH]
+    cmd += [f"-L{PKG_DIR}", "-ltorchair_b200", f"-L{lib_dir}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TORCH_SOURCE}:\n{r.stdout}\n{r.stderr}")
+    return TORCH_LIB_PATH
+
+
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compiles every .cu under csrc/ and links the shared library; returns its path."""
+    """Compiles every .cu under csrc/ and links the shared library, then its PyTorch side; returns the former's path."""
     nvcc = _nvcc()
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(PKG_DIR, "..", "include", "tab_api.h"))
@@ -55,6 +76,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_torch_library(force)
     return LIB_PATH
 
 

@@ -79,6 +79,8 @@ SIGNATURES = {
 _RESTYPE = {"tab_last_error": c_char_p, "tab_launch_count": ctypes.c_longlong}
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libtorchair_b200.so")
+# PyTorch side of the dense operators (csrc/torch_dense.cpp), linked against the library above; loaded by dense.py
+TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libtorchair_b200_torch.so")
 _lock = threading.Lock()
 _lib = None
 

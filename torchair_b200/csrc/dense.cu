@@ -2,6 +2,8 @@
 // split of tiles, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
 #include <stdlib.h>
 
+#include <atomic>
+
 #include "dense_common.cuh"
 #include "dense_narrow.cuh"
 #include "dense_pair.cuh"
@@ -118,10 +120,22 @@ static DensePlan dense_plan(int64_t M, int64_t col_tiles, int64_t depth) {
   return d;
 }
 
+// Raises a kernel's dynamic shared memory limit once per device.
+template <typename F>
+static int allow_smem(const char* op, F* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return TAB_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: shared memory opt-in failed: %s", op, cudaGetErrorString(e));
+  if (dev >= 0 && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return TAB_OK;
+}
+
 template <typename T, int EPI>
 static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMap& mb, const DenseParams& p, int pairs, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDpSmemBytes);
-  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: shared memory opt-in failed: %s", op, cudaGetErrorString(e));
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(op, dense_pair_kernel<T, EPI>, kDpSmemBytes, done);
+  if (rc != TAB_OK) return rc;
   dense_pair_kernel<T, EPI><<<2 * pairs, kDpThreads, kDpSmemBytes, st>>>(ma, mb, p);
   return check_launch(op);
 }
@@ -161,8 +175,9 @@ static bool use_narrow(int64_t M, const DenseOperand& x) { return M <= kNwMaxTok
 template <typename T, int EPI>
 static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensorMap& mx, const DenseParams& p, int tiles, cudaStream_t st) {
   const int smem = 1024 + p.stages * dense_narrow_stage_bytes(p.nt) + kNwCtrlBytes;
-  cudaError_t e = cudaFuncSetAttribute(dense_narrow_kernel<T, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kNwSmemTarget);
-  if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: shared memory opt-in failed: %s", op, cudaGetErrorString(e));
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(op, dense_narrow_kernel<T, EPI>, kNwSmemTarget, done);
+  if (rc != TAB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.split));
   cfg.blockDim = dim3(kNwThreads);
@@ -177,7 +192,7 @@ static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensor
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.dependent ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, dense_narrow_kernel<T, EPI>, mw, mx, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, dense_narrow_kernel<T, EPI>, mw, mx, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(TAB_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));

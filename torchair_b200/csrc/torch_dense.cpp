@@ -1,0 +1,725 @@
+// PyTorch side of the dense 16-bit operators (schemas and documentation: torchair_b200/dense.py): argument checks, layouts,
+// workspaces and the autograd formulas around the C entry points of include/tab_api.h.
+//
+// Why C++: a decode step of these operators runs 5 to 20 microseconds on the GPU.  The same host path in Python took 43 us per
+// call of npu_linear_act (8 x 2048 -> 7168), five times the kernel; this one takes about as long as the kernel.
+#include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <array>
+#include <string>
+#include <tuple>
+
+#include "../../include/tab_api.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+constexpr int64_t kBlock = 64;      // values of a row that share a scale in an 8-bit checkpoint
+
+int64_t up(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
+
+void ok(int rc, const char* entry) { TORCH_CHECK(rc == TAB_OK, entry, " failed (", rc, "): ", tab_last_error()); }
+
+// ---- checks (the same words as the Meta implementations) ----
+int act_code(const char* op, c10::string_view a) {
+  if (a == "none") return TAB_ACT_NONE;
+  if (a == "relu") return TAB_ACT_RELU;
+  if (a == "gelu") return TAB_ACT_GELU;
+  if (a == "gelu_tanh") return TAB_ACT_GELU_TANH;
+  if (a == "silu") return TAB_ACT_SILU;
+  TORCH_CHECK(false, op, ": activation '", a, "' (one of none, relu, gelu, gelu_tanh, silu)");
+}
+
+int check16(const char* op, const Tensor& x) {
+  if (x.scalar_type() == at::kBFloat16) return TAB_BF16;
+  if (x.scalar_type() == at::kHalf) return TAB_F16;
+  TORCH_CHECK_NOT_IMPLEMENTED(false, op, ": x must be bf16 or fp16, got ", x.scalar_type());
+}
+
+void same(const char* op, const Tensor& x, const char* name, const Tensor& t) {
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), op, ": `", name, "` is ", t.scalar_type(), ", x is ", x.scalar_type(),
+              "; all 16-bit tensors of a call have one dtype");
+  TORCH_CHECK(t.device() == x.device(), op, ": `", name, "` is on ", t.device(), ", x is on ", x.device());
+}
+void same(const char* op, const Tensor& x, const char* name, const OptTensor& t) {
+  if (t.has_value()) same(op, x, name, *t);
+}
+
+// ---- layouts ----
+struct Call {
+  int dtype;
+  cudaStream_t stream;
+  at::TensorOptions opt;
+  explicit Call(const Tensor& x, int dtype_) : dtype(dtype_), stream(c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), opt(x.options().requires_grad(false)) {}
+  Tensor empty(at::IntArrayRef sizes) const { return at::empty(sizes, opt); }
+  Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const { return at::empty(sizes, opt.dtype(t)); }
+  Tensor workspace(size_t bytes) const { return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, opt.dtype(at::kByte)); }
+};
+
+bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
+
+// dst = src inside src's shape, zero elsewhere (2-D, 16-bit, any strides)
+void copy_2d(const Call& c, const Tensor& src, const Tensor& dst) {
+  ok(tab_copy_2d(src.data_ptr(), src.stride(0), src.stride(1), src.size(0), src.size(1), dst.data_ptr(), dst.stride(0), dst.stride(1), dst.size(0),
+                 dst.size(1), c.stream),
+     "tab_copy_2d");
+}
+
+// A matrix in memory that the tensor maps take: contiguous along its columns (row-major) or along its rows, the other stride
+// a multiple of 8 elements.
+struct Mat {
+  Tensor t;
+  int64_t ld;
+  bool row_major;
+  const void* ptr() const { return t.data_ptr(); }
+  // as operand [index of the product, contraction]: the rows of this matrix are the index ...
+  int mn_by_rows() const { return row_major ? 0 : 1; }
+  // ... or its columns are
+  int mn_by_cols() const { return row_major ? 1 : 0; }
+};
+
+// t [m, n] row-major with `cols` >= n columns (a multiple of 8): itself where its memory allows that, else a zero-padded copy
+Mat rows_of(const Call& c, const Tensor& t, int64_t cols) {
+  if (t.size(1) == cols && t.stride(1) == 1 && aligned(t)) {
+    if (t.size(0) <= 1) return {t, cols, true};
+    if (t.stride(0) % 8 == 0 && t.stride(0) >= cols) return {t, t.stride(0), true};
+  }
+  Tensor out = c.empty({t.size(0), cols});
+  copy_2d(c, t, out);
+  return {out, cols, true};
+}
+
+bool col_major(const Tensor& t) { return t.stride(0) == 1 && t.stride(1) != 1; }
+
+// a weight [r, c], padded to [rows, cols] if need be; keeps the order in memory that the weight (and so its gradient) has
+Mat matrix_of(const Call& c, const Tensor& t, int64_t rows, int64_t cols) {
+  if (t.size(0) == rows && t.size(1) == cols && aligned(t)) {
+    if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= cols) return {t, t.stride(0), true};
+    if (t.stride(0) == 1 && t.stride(1) % 8 == 0 && t.stride(1) >= rows) return {t, t.stride(1), false};
+  }
+  if (col_major(t)) {
+    Tensor out = c.empty({cols, rows}).t();
+    copy_2d(c, t, out);
+    return {out, rows, false};
+  }
+  Tensor out = c.empty({rows, cols});
+  copy_2d(c, t, out);
+  return {out, cols, true};
+}
+
+// weight1 [H, 2 I] with either half padded to `half` columns when I is not a multiple of 8
+Mat halves_of(const Call& c, const Tensor& t, int64_t rows, int64_t half) {
+  const int64_t inner = t.size(1) / 2;
+  if (inner == half) return matrix_of(c, t, rows, 2 * half);
+  const bool cm = col_major(t);
+  Tensor out = cm ? c.empty({2 * half, rows}).t() : c.empty({rows, 2 * half});
+  copy_2d(c, t.narrow(1, 0, inner), out.narrow(1, 0, half));
+  copy_2d(c, t.narrow(1, inner, inner), out.narrow(1, half, half));
+  return {out, cm ? rows : 2 * half, !cm};
+}
+
+// t [m, n] as [m, cols] without gaps between rows, 16-byte aligned
+Tensor dense_rows(const Call& c, const Tensor& t, int64_t cols) {
+  if (t.size(1) == cols && t.is_contiguous() && aligned(t)) return t;
+  Tensor out = c.empty({t.size(0), cols});
+  copy_2d(c, t, out);
+  return out;
+}
+
+// a bias of n (padded) values; halves: either half padded on its own
+Tensor vector_of(const Call& c, const OptTensor& t, int64_t n, bool halves = false) {
+  if (!t.has_value()) return Tensor();
+  if (t->size(0) == n && t->stride(0) == 1 && aligned(*t)) return *t;
+  if (halves) return halves_of(c, t->unsqueeze(0), 1, n / 2).t;
+  return dense_rows(c, t->unsqueeze(0), n);
+}
+
+// the unpadded corner of a padded result, without gaps, in the same order
+Tensor cut(const Call& c, const Tensor& t, int64_t rows, int64_t cols) {
+  if (t.size(0) == rows && t.size(1) == cols) return t;
+  if (col_major(t)) return cut(c, t.t(), cols, rows).t();
+  Tensor out = c.empty({rows, cols});
+  copy_2d(c, t.narrow(0, 0, rows).narrow(1, 0, cols), out);
+  return out;
+}
+Tensor cut_halves(const Call& c, const Tensor& t, int64_t rows, int64_t inner) {
+  const int64_t half = t.size(1) / 2;
+  if (t.size(0) == rows && half == inner) return t;
+  Tensor out = col_major(t) ? c.empty({2 * inner, rows}).t() : c.empty({rows, 2 * inner});
+  copy_2d(c, t.narrow(0, 0, rows).narrow(1, 0, inner), out.narrow(1, 0, inner));
+  copy_2d(c, t.narrow(0, 0, rows).narrow(1, half, inner), out.narrow(1, inner, inner));
+  return out;
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// what a forward pass keeps for its backward pass: 16-bit values, or int8 with scales
+struct Kept {
+  Tensor values, scale, x_q, x_scale;
+  bool int8() const { return values.defined() && values.scalar_type() == at::kChar; }
+  void* p16() const { return values.defined() && !int8() ? values.data_ptr() : nullptr; }
+  int8_t* p8() const { return int8() ? static_cast<int8_t*>(values.data_ptr()) : nullptr; }
+  float* ps() const { return int8() ? static_cast<float*>(scale.data_ptr()) : nullptr; }
+  int64_t ld() const { return values.defined() ? values.size(1) : 0; }
+};
+
+// act(a b^T + bias) + residual: a [m, k], b [n, k] as operands
+void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int64_t m, int64_t n, int64_t k, const Tensor& out,
+            const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept()) {
+  size_t bytes = 0;
+  ok(tab_dense_matmul_workspace_bytes(m, n, k, &bytes), "tab_dense_matmul_workspace_bytes");
+  Tensor ws = bytes ? c.workspace(bytes) : Tensor();
+  ok(tab_dense_matmul(a, lda, a_mn, b, ldb, b_mn, c.dtype, m, n, k, ptr(bias), ptr(residual), act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
+                      out.data_ptr(), ptr(ws), bytes, c.stream),
+     "tab_dense_matmul");
+}
+
+// x^T dz [k, n] (both row-major), in the memory order of the weight `like`
+Tensor weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_t n, const Tensor& like) {
+  const int64_t m = x.t.size(0);
+  if (col_major(like)) {
+    Tensor out = c.empty({n, k});
+    matmul(c, dz.ptr(), dz.ld, 1, x.ptr(), x.ld, 1, n, k, m, out);
+    return out.t();
+  }
+  Tensor out = c.empty({k, n});
+  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out);
+  return out;
+}
+
+// dz = grad act'(kept) (grad itself without an activation) and, if wanted, its column sums
+Mat act_grad(const Call& c, const Mat& grad, int64_t n, int act, const Kept& kept, bool want_dz, bool want_sums, Tensor& column_sums) {
+  const int64_t m = grad.t.size(0);
+  Tensor dz = want_dz && act ? c.empty({m, n}) : Tensor(), parts;
+  if (want_sums) {
+    size_t splits = 0;
+    ok(tab_act_grad_splits(m, n, &splits), "tab_act_grad_splits");
+    parts = c.empty({static_cast<int64_t>(splits), n}, at::kFloat);
+  }
+  if (dz.defined() || parts.defined())
+    ok(tab_act_grad(grad.ptr(), grad.ld, c.dtype, m, n, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), ptr(dz), static_cast<float*>(ptr(parts)),
+                    c.stream),
+       "tab_act_grad");
+  if (want_sums) {
+    column_sums = c.empty({1, n});
+    ok(tab_column_sums(static_cast<const float*>(parts.data_ptr()), parts.size(0), n, column_sums.data_ptr(), c.dtype, c.stream), "tab_column_sums");
+  }
+  return act ? Mat{dz, n, true} : grad;
+}
+
+int any_dtype(at::ScalarType t) { return t == at::kBFloat16 ? TAB_BF16 : t == at::kHalf ? TAB_F16 : t == at::kFloat ? TAB_F32 : 0; }
+
+void quantise(cudaStream_t stream, const Tensor& x, int64_t rows, int64_t cols, int64_t ldx, const Tensor& q, const Tensor& scale) {
+  ok(tab_checkpoint_quant(x.data_ptr(), any_dtype(x.scalar_type()), ldx, rows, cols, static_cast<int8_t*>(q.data_ptr()), cols,
+                          static_cast<float*>(scale.data_ptr()), up(cols, kBlock) / kBlock, stream),
+     "tab_checkpoint_quant");
+}
+
+// x [m, k] kept in 8 bits for the weight gradient
+void keep_x(const Call& c, const Tensor& x, Kept& kept) {
+  const Tensor xr = x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= x.size(1)) ? x : x.contiguous();
+  kept.x_q = c.empty({x.size(0), x.size(1)}, at::kChar);
+  kept.x_scale = c.empty({x.size(0), up(x.size(1), kBlock) / kBlock}, at::kFloat);
+  quantise(c.stream, xr, x.size(0), x.size(1), xr.stride(0), kept.x_q, kept.x_scale);
+}
+
+// int8 [m, k] with its scales (no gaps) -> 16 bits [m, cols], zero-padded
+Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale, int64_t cols) {
+  Tensor y = c.empty({q.size(0), cols});
+  ok(tab_checkpoint_dequant(static_cast<const int8_t*>(q.data_ptr()), q.size(1), static_cast<const float*>(scale.data_ptr()), scale.size(1), q.size(0),
+                            q.size(1), y.data_ptr(), c.dtype, cols, cols, c.stream),
+     "tab_checkpoint_dequant");
+  return {y, cols, true};
+}
+
+using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+Five keep_results(const Call& c, const Tensor& y, const Kept& k) {
+  auto or_empty = [&](const Tensor& t, at::ScalarType s) { return t.defined() ? t : c.empty({0}, s); };
+  return Five(y, k.values, or_empty(k.scale, at::kFloat), or_empty(k.x_q, at::kChar), or_empty(k.x_scale, at::kFloat));
+}
+
+// ---- npu_gated_ffn ----
+struct FfnSizes {
+  int dtype, act;
+  int64_t h, inner, m;
+};
+
+FfnSizes ffn_check(const Tensor& x, const Tensor& w1, const Tensor& w2, const OptTensor& b1, const OptTensor& b2, const OptTensor& r, c10::string_view act) {
+  const char* op = "npu_gated_ffn";
+  FfnSizes s;
+  s.dtype = check16(op, x);
+  TORCH_CHECK(x.dim() >= 1 && w1.dim() == 2 && w2.dim() == 2, op, ": x must be [..., H], weight1 [H, 2 I] and weight2 [I, H]");
+  s.h = x.size(-1);
+  s.inner = w2.size(0);
+  TORCH_CHECK(s.h > 0 && s.inner > 0 && w1.size(0) == s.h && w1.size(1) == 2 * s.inner && w2.size(1) == s.h, op, ": x ", x.sizes(), ", weight1 ", w1.sizes(),
+              " and weight2 ", w2.sizes(), " do not fit [..., H], [H, 2 I] and [I, H]");
+  TORCH_CHECK((!b1.has_value() || (b1->dim() == 1 && b1->size(0) == 2 * s.inner)) && (!b2.has_value() || (b2->dim() == 1 && b2->size(0) == s.h)), op,
+              ": bias1 must be [2 I] = [", 2 * s.inner, "] and bias2 [H] = [", s.h, "]");
+  TORCH_CHECK(!r.has_value() || r->sizes() == x.sizes(), op, ": residual must have the shape of x, got ", r.has_value() ? r->sizes() : x.sizes());
+  same(op, x, "weight1", w1);
+  same(op, x, "weight2", w2);
+  same(op, x, "bias1", b1);
+  same(op, x, "bias2", b2);
+  same(op, x, "residual", r);
+  s.act = act_code(op, act);
+  s.m = x.numel() / s.h;
+  return s;
+}
+
+Tensor ffn_forward(const Call& c, const FfnSizes& s, const Tensor& x, const Tensor& weight1, const Tensor& weight2, const OptTensor& bias1,
+                   const OptTensor& bias2, const OptTensor& residual, const Kept& kept) {
+  const int64_t h8 = up(s.h, 8), inner8 = up(s.inner, 8);
+  Tensor y = h8 == s.h ? c.empty(x.sizes()) : c.empty({s.m, h8});
+  if (s.m > 0) {
+    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.h}), h8);
+    const Mat w1 = halves_of(c, weight1, h8, inner8), w2 = matrix_of(c, weight2, inner8, h8);
+    const Tensor b1 = vector_of(c, bias1, 2 * inner8, s.inner != inner8), b2 = vector_of(c, bias2, h8);
+    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.h}), h8) : Tensor();
+    size_t bytes = 0;
+    ok(tab_gated_ffn_workspace_bytes(s.m, h8, inner8, &bytes), "tab_gated_ffn_workspace_bytes");
+    const Tensor ws = c.workspace(bytes);
+    ok(tab_gated_ffn(xm.ptr(), xm.ld, w1.ptr(), w1.ld, w1.mn_by_cols(), w2.ptr(), w2.ld, w2.mn_by_cols(), c.dtype, s.m, h8, inner8, ptr(b1), ptr(b2),
+                     ptr(r), s.act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), y.data_ptr(), ws.data_ptr(), ws.numel(), c.stream),
+       "tab_gated_ffn");
+  }
+  return h8 == s.h ? y : cut(c, y, s.m, s.h).view(x.sizes());
+}
+
+Tensor ffn_cuda(const Tensor& x, const Tensor& weight1, const Tensor& weight2, const OptTensor& bias1, const OptTensor& bias2, const OptTensor& residual,
+                c10::string_view activation, bool) {
+  const FfnSizes s = ffn_check(x, weight1, weight2, bias1, bias2, residual, activation);
+  const c10::cuda::CUDAGuard guard(x.device());
+  return ffn_forward(Call(x, s.dtype), s, x, weight1, weight2, bias1, bias2, residual, Kept());
+}
+
+Five ffn_keep_cuda(const Tensor& x, const Tensor& weight1, const Tensor& weight2, const OptTensor& bias1, const OptTensor& bias2, const OptTensor& residual,
+                   c10::string_view activation, bool int8) {
+  const FfnSizes s = ffn_check(x, weight1, weight2, bias1, bias2, residual, activation);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Call c(x, s.dtype);
+  Kept kept;
+  if (int8) {
+    keep_x(c, x.reshape({s.m, s.h}), kept);
+    const int64_t width = 2 * up(s.inner, kBlock);
+    kept.values = c.empty({s.m, width}, at::kChar);
+    kept.scale = c.empty({s.m, width / kBlock}, at::kFloat);
+  } else {
+    kept.values = c.empty({s.m, 2 * up(s.inner, 8)});
+  }
+  const Tensor y = ffn_forward(c, s, x, weight1, weight2, bias1, bias2, residual, kept);
+  return keep_results(c, y, kept);
+}
+
+Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_scale, const Tensor& weight1, const Tensor& weight2, const Tensor& kept_values,
+                       const Tensor& kept_scale, c10::string_view activation, std::array<bool, 5> want) {
+  const char* op = "npu_gated_ffn_backward";
+  const int dtype = check16(op, grad_), act = act_code(op, activation);
+  TORCH_CHECK(weight1.dim() == 2 && weight2.dim() == 2 && grad_.dim() >= 1, op, ": grad must be [..., H], weight1 [H, 2 I] and weight2 [I, H]");
+  const int64_t inner = weight2.size(0), h = weight2.size(1);
+  const bool int8 = kept_values.scalar_type() == at::kChar, x8 = x_.scalar_type() == at::kChar;
+  TORCH_CHECK(h > 0 && inner > 0 && grad_.size(-1) == h && weight1.size(0) == h && weight1.size(1) == 2 * inner, op, ": grad ", grad_.sizes(), ", weight1 ",
+              weight1.sizes(), " and weight2 ", weight2.sizes(), " do not fit [..., H], [H, 2 I] and [I, H]");
+  same(op, grad_, "weight1", weight1);
+  same(op, grad_, "weight2", weight2);
+  const int64_t m = grad_.numel() / h, h8 = up(h, 8), inner8 = up(inner, 8), width = 2 * up(inner, int8 ? kBlock : 8);
+  TORCH_CHECK(kept_values.dim() == 2 && kept_values.size(0) == m && kept_values.size(1) == width && kept_values.is_contiguous() &&
+                  (int8 ? kept_scale.numel() == m * width / kBlock && kept_scale.scalar_type() == at::kFloat && kept_scale.is_contiguous()
+                        : kept_values.scalar_type() == grad_.scalar_type()) &&
+                  kept_values.device() == grad_.device() && (!int8 || kept_scale.device() == grad_.device()),
+              op, ": kept ", kept_values.sizes(), " does not hold the gate and up values of ", m, " rows");
+  TORCH_CHECK(!want[1] || (x_.numel() == m * h && x_.device() == grad_.device() && (x8 ? x_.is_contiguous() && x_scale.is_contiguous() && x_scale.scalar_type() == at::kFloat && x_scale.numel() == m * (up(h, kBlock) / kBlock) && x_scale.device() == grad_.device() : x_.scalar_type() == grad_.scalar_type())), op,
+              ": x ", x_.sizes(), " does not fit grad ", grad_.sizes());
+  const c10::cuda::CUDAGuard guard(grad_.device());
+  const Call c(grad_, dtype);
+  Tensor none, dx, dw1, dw2, db1, db2;
+  auto result = [&](const Tensor& t) -> Tensor {
+    if (t.defined()) return t;
+    if (!none.defined()) none = c.empty({0});
+    return none;
+  };
+  if (m == 0) {
+    if (want[0]) dx = at::zeros(grad_.sizes(), c.opt);
+    if (want[1]) dw1 = at::zeros({h, 2 * inner}, c.opt);
+    if (want[2]) dw2 = at::zeros({inner, h}, c.opt);
+    if (want[3]) db1 = at::zeros({2 * inner}, c.opt);
+    if (want[4]) db2 = at::zeros({h}, c.opt);
+    return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
+  }
+  const Mat dy = rows_of(c, grad_.reshape({m, h}), h8);
+  Kept kept;
+  kept.values = kept_values;
+  kept.scale = kept_scale;
+  Mat dz{Tensor(), 2 * inner8, true}, hidden{Tensor(), inner8, true};
+  if (want[0] || want[1] || want[2] || want[3]) {
+    const Mat w2 = matrix_of(c, weight2, inner8, h8);
+    dz.t = c.empty({m, 2 * inner8});
+    hidden.t = c.empty({m, inner8});
+    size_t bytes = 0;
+    ok(tab_dense_matmul_workspace_bytes(m, inner8, h8, &bytes), "tab_dense_matmul_workspace_bytes");
+    const Tensor ws = bytes ? c.workspace(bytes) : Tensor();
+    ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h8, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
+                             dz.t.data_ptr(), hidden.t.data_ptr(), ptr(ws), bytes, c.stream),
+       "tab_gated_matmul_grad");
+  }
+  if (want[2]) dw2 = cut(c, weight_grad(c, hidden, dy, inner8, h8, weight2), inner, h);
+  if (want[0]) {
+    const Mat w1 = halves_of(c, weight1, h8, inner8);
+    Tensor out = c.empty({m, h8});
+    matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h8, 2 * inner8, out);
+    dx = cut(c, out, m, h).view(grad_.sizes());
+  }
+  if (want[1]) {
+    const Mat xm = x8 ? dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8) : rows_of(c, x_.reshape({m, h}), h8);
+    dw1 = cut_halves(c, weight_grad(c, xm, dz, h8, 2 * inner8, weight1), h, inner);
+  }
+  if (want[3]) {
+    act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
+    db1 = cut_halves(c, db1, 1, inner).view({2 * inner});
+  }
+  if (want[4]) {
+    act_grad(c, dy, h8, 0, Kept(), false, true, db2);
+    db2 = cut(c, db2, 1, h).view({h});
+  }
+  return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
+}
+
+// ---- npu_linear_act ----
+struct LinearSizes {
+  int dtype, act;
+  int64_t k, n, m;
+};
+
+LinearSizes linear_check(const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, c10::string_view act, at::DimVector& out_sizes) {
+  const char* op = "npu_linear_act";
+  LinearSizes s;
+  s.dtype = check16(op, x);
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(0) == x.size(-1) && w.size(0) > 0 && w.size(1) > 0, op, ": x ", x.sizes(), " and weight ", w.sizes(),
+              " do not fit [..., K] and [K, N]");
+  s.k = w.size(0);
+  s.n = w.size(1);
+  TORCH_CHECK(!b.has_value() || (b->dim() == 1 && b->size(0) == s.n), op, ": bias must be [N] = [", s.n, "]");
+  out_sizes = at::DimVector(x.sizes());
+  out_sizes.back() = s.n;
+  TORCH_CHECK(!r.has_value() || r->sizes() == at::IntArrayRef(out_sizes), op, ": residual must be ", at::IntArrayRef(out_sizes), ", got ",
+              r.has_value() ? r->sizes() : x.sizes());
+  same(op, x, "weight", w);
+  same(op, x, "bias", b);
+  same(op, x, "residual", r);
+  s.act = act_code(op, act);
+  s.m = x.numel() / s.k;
+  return s;
+}
+
+Tensor linear_forward(const Call& c, const LinearSizes& s, at::IntArrayRef out_sizes, const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                      const OptTensor& residual, const Kept& kept) {
+  const int64_t k8 = up(s.k, 8), n8 = up(s.n, 8);
+  Tensor y = n8 == s.n ? c.empty(out_sizes) : c.empty({s.m, n8});
+  if (s.m > 0) {
+    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.k}), k8);
+    const Mat w = matrix_of(c, weight, k8, n8);
+    const Tensor b = vector_of(c, bias, n8);
+    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.n}), n8) : Tensor();
+    matmul(c, xm.ptr(), xm.ld, 0, w.ptr(), w.ld, w.mn_by_cols(), s.m, n8, k8, y, b, r, s.act, kept);
+  }
+  return n8 == s.n ? y : cut(c, y, s.m, s.n).view(out_sizes);
+}
+
+Tensor linear_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, c10::string_view activation, bool) {
+  at::DimVector out_sizes;
+  const LinearSizes s = linear_check(x, weight, bias, residual, activation, out_sizes);
+  const c10::cuda::CUDAGuard guard(x.device());
+  return linear_forward(Call(x, s.dtype), s, out_sizes, x, weight, bias, residual, Kept());
+}
+
+Five linear_keep_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, c10::string_view activation, bool int8) {
+  at::DimVector out_sizes;
+  const LinearSizes s = linear_check(x, weight, bias, residual, activation, out_sizes);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Call c(x, s.dtype);
+  Kept kept;
+  if (int8) keep_x(c, x.reshape({s.m, s.k}), kept);
+  // without an activation the backward pass does not need its argument
+  const int64_t width = s.act ? up(s.n, int8 ? kBlock : 8) : 0;
+  Kept stored;
+  if (s.act) {
+    stored.values = c.empty({s.m, width}, int8 ? at::kChar : x.scalar_type());
+    if (int8) stored.scale = c.empty({s.m, width / kBlock}, at::kFloat);
+  }
+  const Tensor y = linear_forward(c, s, out_sizes, x, weight, bias, residual, stored);
+  kept.values = s.act ? stored.values : c.empty({s.m, 0}, int8 ? at::kChar : x.scalar_type());
+  kept.scale = stored.scale.defined() ? stored.scale : int8 ? c.empty({s.m, 0}, at::kFloat) : Tensor();
+  return keep_results(c, y, kept);
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_scale, const Tensor& weight,
+                                                        const Tensor& kept_values, const Tensor& kept_scale, c10::string_view activation,
+                                                        std::array<bool, 3> want) {
+  const char* op = "npu_linear_act_backward";
+  const int dtype = check16(op, grad_), act = act_code(op, activation);
+  TORCH_CHECK(weight.dim() == 2 && grad_.dim() >= 1 && grad_.size(-1) == weight.size(1) && weight.size(0) > 0 && weight.size(1) > 0, op, ": grad ",
+              grad_.sizes(), " and weight ", weight.sizes(), " do not fit [..., N] and [K, N]");
+  same(op, grad_, "weight", weight);
+  const int64_t k = weight.size(0), n = weight.size(1), m = grad_.numel() / n, k8 = up(k, 8), n8 = up(n, 8);
+  const bool int8 = kept_values.scalar_type() == at::kChar, x8 = x_.scalar_type() == at::kChar;
+  const int64_t width = up(n, int8 ? kBlock : 8);
+  TORCH_CHECK(act == TAB_ACT_NONE ||
+                  (kept_values.dim() == 2 && kept_values.size(0) == m && kept_values.size(1) == width && kept_values.is_contiguous() &&
+                   (int8 ? kept_scale.numel() == m * width / kBlock && kept_scale.scalar_type() == at::kFloat && kept_scale.is_contiguous()
+                         : kept_values.scalar_type() == grad_.scalar_type()) &&
+                   kept_values.device() == grad_.device() && (!int8 || kept_scale.device() == grad_.device())),
+              op, ": kept ", kept_values.sizes(), " does not hold the activation's arguments of ", m, " rows");
+  TORCH_CHECK(!want[1] || (x_.numel() == m * k && x_.device() == grad_.device() && (x8 ? x_.is_contiguous() && x_scale.is_contiguous() && x_scale.scalar_type() == at::kFloat && x_scale.numel() == m * (up(k, kBlock) / kBlock) && x_scale.device() == grad_.device() : x_.scalar_type() == grad_.scalar_type())), op,
+              ": x ", x_.sizes(), " does not fit grad ", grad_.sizes());
+  at::DimVector x_sizes(grad_.sizes());
+  x_sizes.back() = k;
+  const c10::cuda::CUDAGuard guard(grad_.device());
+  const Call c(grad_, dtype);
+  Tensor dx, dw, db;
+  if (m == 0) {
+    if (want[0]) dx = at::zeros(x_sizes, c.opt);
+    if (want[1]) dw = at::zeros({k, n}, c.opt);
+    if (want[2]) db = at::zeros({n}, c.opt);
+  } else {
+    Kept kept;
+    if (act) {
+      kept.values = kept_values;
+      kept.scale = kept_scale;
+    }
+    const Mat dz = act_grad(c, rows_of(c, grad_.reshape({m, n}), n8), n8, act, kept, want[0] || want[1], want[2], db);
+    if (want[0]) {
+      const Mat w = matrix_of(c, weight, k8, n8);
+      Tensor out = c.empty({m, k8});
+      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k8, n8, out);
+      dx = cut(c, out, m, k).view(x_sizes);
+    }
+    if (want[1]) {
+      const Mat xm = x8 ? dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8) : rows_of(c, x_.reshape({m, k}), k8);
+      dw = cut(c, weight_grad(c, xm, dz, k8, n8, weight), k, n);
+    }
+    if (want[2]) db = cut(c, db, 1, n).view({n});
+  }
+  auto result = [&](const Tensor& t) { return t.defined() ? t : c.empty({0}); };
+  return {result(dx), result(dw), result(db)};
+}
+
+// ---- 8-bit checkpoints ----
+void ck_check(const char* op, const Tensor& q, const Tensor& scale) {
+  TORCH_CHECK(q.scalar_type() == at::kChar && scale.scalar_type() == at::kFloat, op, ": q must be int8 and scale fp32, got ", q.scalar_type(), " and ",
+              scale.scalar_type());
+  bool fits = q.dim() >= 1 && scale.dim() == q.dim() && scale.size(-1) == up(q.size(-1), kBlock) / kBlock;
+  for (int64_t i = 0; fits && i + 1 < q.dim(); ++i) fits = q.size(i) == scale.size(i);
+  TORCH_CHECK(fits, op, ": scale ", scale.sizes(), " does not hold one value per row and 64 values of q ", q.sizes());
+  TORCH_CHECK(q.device() == scale.device(), op, ": q is on ", q.device(), ", scale is on ", scale.device());
+}
+
+std::tuple<Tensor, Tensor> ck_quant_cuda(const Tensor& x) {
+  const char* op = "npu_checkpoint_quant";
+  TORCH_CHECK_NOT_IMPLEMENTED(any_dtype(x.scalar_type()) != 0, op, ": x must be bf16, fp16 or fp32, got ", x.scalar_type());
+  TORCH_CHECK(x.dim() >= 1, op, ": x must have at least one dimension");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Call c(x, any_dtype(x.scalar_type()));
+  const int64_t cols = x.size(-1);
+  at::DimVector scale_sizes(x.sizes());
+  scale_sizes.back() = up(cols, kBlock) / kBlock;
+  Tensor q = c.empty(x.sizes(), at::kChar), scale = c.empty(scale_sizes, at::kFloat);
+  if (x.numel() > 0) {
+    const int64_t rows = x.numel() / cols;
+    const bool as_is = x.dim() == 2 && x.stride(1) == 1 && (rows == 1 || x.stride(0) >= cols);
+    const Tensor xc = as_is ? x : x.contiguous();
+    quantise(c.stream, xc, rows, cols, as_is ? x.stride(0) : cols, q, scale);
+  }
+  return {q, scale};
+}
+
+Tensor ck_dequant_cuda(const Tensor& q, const Tensor& scale, int64_t output_dtype) {
+  const char* op = "npu_checkpoint_dequant";
+  ck_check(op, q, scale);
+  TORCH_CHECK_NOT_IMPLEMENTED(output_dtype == TAB_F16 || output_dtype == TAB_F32 || output_dtype == TAB_BF16, op, ": output_dtype=", output_dtype,
+                              " (5 fp16, 6 fp32 or 15 bf16)");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const Call c(q, static_cast<int>(output_dtype));
+  Tensor y = c.empty(q.sizes(), output_dtype == TAB_F16 ? at::kHalf : output_dtype == TAB_F32 ? at::kFloat : at::kBFloat16);
+  if (y.numel() > 0) {
+    const int64_t cols = q.size(-1);
+    const Tensor qc = q.contiguous(), sc = scale.contiguous();
+    ok(tab_checkpoint_dequant(static_cast<const int8_t*>(qc.data_ptr()), cols, static_cast<const float*>(sc.data_ptr()), sc.size(-1), q.numel() / cols, cols,
+                              y.data_ptr(), c.dtype, cols, cols, c.stream),
+       "tab_checkpoint_dequant");
+  }
+  return y;
+}
+
+Tensor ck_weight_grad_cuda(const Tensor& q_, const Tensor& scale_, const Tensor& grad_) {
+  const char* op = "npu_checkpoint_weight_grad";
+  ck_check(op, q_, scale_);
+  const int dtype = check16(op, grad_);
+  bool fits = grad_.dim() == q_.dim() && grad_.size(-1) > 0 && q_.size(-1) > 0;
+  for (int64_t i = 0; fits && i + 1 < q_.dim(); ++i) fits = q_.size(i) == grad_.size(i);
+  TORCH_CHECK(fits, op, ": q ", q_.sizes(), " and grad ", grad_.sizes(), " must be [..., K] and [..., N] of the same rows");
+  TORCH_CHECK(grad_.device() == q_.device(), op, ": grad is on ", grad_.device(), ", q is on ", q_.device());
+  const int64_t k = q_.size(-1), n = grad_.size(-1), m = q_.numel() / k, k8 = up(k, 8), n8 = up(n, 8);
+  const c10::cuda::CUDAGuard guard(grad_.device());
+  const Call c(grad_, dtype);
+  if (m == 0) return at::zeros({k, n}, c.opt);
+  const Tensor q = q_.contiguous().view({m, k}), scale = scale_.contiguous().view({m, -1});
+  const Mat x = dequantise(c, q, scale, k8), dz = rows_of(c, grad_.reshape({m, n}), n8);
+  Tensor out = c.empty({k8, n8});
+  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k8, n8, m, out);
+  return cut(c, out, k, n);
+}
+
+// ---- autograd ----
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+template <typename Sig>
+c10::TypedOperatorHandle<Sig> handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+
+bool wants(const Tensor& t) { return t.requires_grad(); }
+bool wants(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+
+// Results of a backward pass that cannot be differentiated again: doing so raises, but only when it is done.
+void once_only(const char* name, const variable_list& inputs, variable_list& out) {
+  if (!at::GradMode::is_enabled()) return;
+  bool any = false;
+  for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
+  if (!any) return;
+  variable_list some;
+  for (const Tensor& t : out)
+    if (t.defined()) some.push_back(t.detach());
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " cannot be differentiated twice", static_cast<int64_t>(some.size()));
+  variable_list marked = (*node)(std::move(some));
+  size_t i = 0;
+  for (Tensor& t : out)
+    if (t.defined()) t = marked[i++];
+}
+
+using FfnSig = Tensor(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, c10::string_view, bool);
+using FfnKeepSig = Five(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, c10::string_view, bool);
+using FfnBackSig = Five(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::string_view,
+                        std::array<bool, 5>);
+
+struct GatedFfn : torch::autograd::Function<GatedFfn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w2, const OptTensor& b1, const OptTensor& b2,
+                        const OptTensor& r, const std::string& act, bool int8) {
+    static const auto op = handle<FfnKeepSig>("npu::npu_gated_ffn_keep");
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, kept, scale, x_q, x_scale] = op.call(x, w1, w2, b1, b2, r, act, int8);
+    ctx->save_for_backward({int8 ? x_q : x, x_scale, w1, w2, kept, scale});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["b1"] = b1.has_value();
+    ctx->saved_data["b2"] = b2.has_value();
+    ctx->saved_data["r"] = r.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = handle<FfnBackSig>("npu::npu_gated_ffn_backward");
+    const variable_list s = ctx->get_saved_variables();
+    // edges exist for the tensors that were given, in their order
+    size_t edge = 3;
+    std::array<bool, 5> want = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2), false, false};
+    if (ctx->saved_data["b1"].toBool()) want[3] = ctx->needs_input_grad(edge++);
+    if (ctx->saved_data["b2"].toBool()) want[4] = ctx->needs_input_grad(edge++);
+    const bool want_r = ctx->saved_data["r"].toBool() && ctx->needs_input_grad(edge);
+    const std::string act = ctx->saved_data["act"].toStringRef();
+    variable_list out(8);
+    if (!grads[0].defined()) return out;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw1, dw2, db1, db2] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], act, want);
+      if (want[0]) out[0] = dx;
+      if (want[1]) out[1] = dw1;
+      if (want[2]) out[2] = dw2;
+      if (want[3]) out[3] = db1;
+      if (want[4]) out[4] = db2;
+    }
+    once_only("npu_gated_ffn", {grads[0], s[0], s[2], s[3]}, out);
+    if (want_r) out[5] = grads[0];
+    return out;
+  }
+};
+
+Tensor ffn_autograd(const Tensor& x, const Tensor& w1, const Tensor& w2, const OptTensor& b1, const OptTensor& b2, const OptTensor& r,
+                    c10::string_view act, bool int8) {
+  if (at::GradMode::is_enabled() && (wants(x) || wants(w1) || wants(w2) || wants(b1) || wants(b2) || wants(r)))
+    return GatedFfn::apply(x, w1, w2, b1, b2, r, std::string(act), int8);
+  static const auto op = handle<FfnSig>("npu::npu_gated_ffn");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, w1, w2, b1, b2, r, act, int8);
+}
+
+using LinearSig = Tensor(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view, bool);
+using LinearKeepSig = Five(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::string_view, bool);
+using LinearBackSig = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                         c10::string_view, std::array<bool, 3>);
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, const std::string& act, bool int8) {
+    static const auto op = handle<LinearKeepSig>("npu::npu_linear_act_keep");
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, kept, scale, x_q, x_scale] = op.call(x, w, b, r, act, int8);
+    ctx->save_for_backward({int8 ? x_q : x, x_scale, w, kept, scale});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["b"] = b.has_value();
+    ctx->saved_data["r"] = r.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto op = handle<LinearBackSig>("npu::npu_linear_act_backward");
+    const variable_list s = ctx->get_saved_variables();
+    size_t edge = 2;
+    std::array<bool, 3> want = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), false};
+    if (ctx->saved_data["b"].toBool()) want[2] = ctx->needs_input_grad(edge++);
+    const bool want_r = ctx->saved_data["r"].toBool() && ctx->needs_input_grad(edge);
+    const std::string act = ctx->saved_data["act"].toStringRef();
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw, db] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], act, want);
+      if (want[0]) out[0] = dx;
+      if (want[1]) out[1] = dw;
+      if (want[2]) out[2] = db;
+    }
+    once_only("npu_linear_act", {grads[0], s[0], s[2]}, out);
+    if (want_r) out[3] = grads[0];
+    return out;
+  }
+};
+
+Tensor linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, c10::string_view act, bool int8) {
+  if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearAct::apply(x, w, b, r, std::string(act), int8);
+  static const auto op = handle<LinearSig>("npu::npu_linear_act");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, w, b, r, act, int8);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_IMPL(npu, CUDA, m) {
+  m.impl("npu_gated_ffn", TORCH_FN(ffn_cuda));
+  m.impl("npu_gated_ffn_keep", TORCH_FN(ffn_keep_cuda));
+  m.impl("npu_gated_ffn_backward", TORCH_FN(ffn_backward_cuda));
+  m.impl("npu_linear_act", TORCH_FN(linear_cuda));
+  m.impl("npu_linear_act_keep", TORCH_FN(linear_keep_cuda));
+  m.impl("npu_linear_act_backward", TORCH_FN(linear_backward_cuda));
+  m.impl("npu_checkpoint_quant", TORCH_FN(ck_quant_cuda));
+  m.impl("npu_checkpoint_dequant", TORCH_FN(ck_dequant_cuda));
+  m.impl("npu_checkpoint_weight_grad", TORCH_FN(ck_weight_grad_cuda));
+}
+
+TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
+  m.impl("npu_gated_ffn", TORCH_FN(ffn_autograd));
+  m.impl("npu_linear_act", TORCH_FN(linear_autograd));
+}
