@@ -464,17 +464,15 @@ TAB_API int tab_gmm_status_reset(tab_stream_t stream);
  *                         projection's [I, K] weight has mn = 0 here when its rows are contiguous);
  *                         from the kept gate g and up u: dz[M, 2 I] = [dh u act'(g) | dh act(g)] and h = act(g) u again
  * tab_gated_ffn:          y[M, H] = (act(z[:, :I]) * z[:, I:]) w2 + bias2[H] + residual, z = x w1 + bias1; h lives in the workspace */
-TAB_API int tab_dense_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes);
 TAB_API int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M,
                              int64_t N, int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q,
-                             float* keep_scale, int64_t keep_ld, void* out, void* workspace, size_t workspace_bytes,
-                             tab_stream_t stream);
+                             float* keep_scale, int64_t keep_ld, void* out, tab_stream_t stream);
 TAB_API int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
                              int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld,
-                             void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream);
+                             void* h, tab_stream_t stream);
 TAB_API int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M,
                                   int64_t I, int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale,
-                                  int64_t keep_ld, void* dz, void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream);
+                                  int64_t keep_ld, void* dz, void* h, tab_stream_t stream);
 TAB_API int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes);
 TAB_API int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ldw1, int w1_mn, const void* w2, int64_t ldw2, int w2_mn,
                           int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual,

@@ -1,5 +1,5 @@
-// Host side of the dense 16-bit GEMMs: argument checks, tensor maps, the choice between the narrow and the pair kernel, the
-// split of tiles, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
+// Host side of the dense 16-bit GEMMs: argument checks, tensor maps, the choice between the narrow and the pair kernel and
+// how many CTAs share a tile, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
 #include <stdlib.h>
 
 #include <atomic>
@@ -75,49 +75,16 @@ static int make_map(const char* op, const DenseOperand& o, int box_rows, CUtenso
   cuuint64_t strides[1] = {(cuuint64_t)((o.ld > 0 ? o.ld : 8) * 2)};
   cuuint32_t box[2] = {64, (cuuint32_t)(o.mn ? kDnBlockK : box_rows)};
   cuuint32_t es[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(o.ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();       // the thread (an autograd worker, say) had made no runtime call yet that binds the device's context
   if (r != CUDA_SUCCESS) return fail(TAB_ERR_CUDA, "%s: tensor map rejected (CUresult %d)", op, (int)r);
   return TAB_OK;
-}
-
-// ---- split of tiles (pair kernel) ----
-struct DensePlan {
-  int row_tiles, col_tiles, num_kb, pairs, sk_tiles;
-  size_t partial_bytes, arrival_bytes;
-};
-
-// Time in blocks of the contraction: whole tiles only take ceil(tiles / pairs) turns of num_kb.  Splitting the last, partly
-// filled turn (or that and one full turn) evenly costs its share plus the joins: about 8 blocks' time to store a part and 4
-// per part that the last CTA adds up.
-static DensePlan dense_plan(int64_t M, int64_t col_tiles, int64_t depth) {
-  DensePlan d = {};
-  d.row_tiles = (int)((M + 255) / 256);
-  d.col_tiles = (int)col_tiles;
-  d.num_kb = (int)((depth + kDnBlockK - 1) / kDnBlockK);
-  const int max_pairs = dense_sms() / 2;
-  const int64_t tiles = static_cast<int64_t>(d.row_tiles) * d.col_tiles;
-  d.pairs = (int)(tiles < max_pairs ? tiles : max_pairs);
-  const int64_t full = tiles / max_pairs, rem = tiles % max_pairs;
-  if (rem == 0) return d;
-  double best = static_cast<double>(full + 1) * d.num_kb;
-  for (int more = 0; more < 2; ++more) {
-    if (more > full) break;
-    const int64_t sk = rem + more * max_pairs;
-    if (sk * d.num_kb < 2 * max_pairs) continue;                   // every pair holds work
-    const double parts = static_cast<double>((max_pairs + sk - 1) / sk) + 1.0;
-    const double cost = static_cast<double>(full - more) * d.num_kb + static_cast<double>(sk) * d.num_kb / max_pairs + 8.0 + 4.0 * parts;
-    if (cost < best) {
-      best = cost;
-      d.sk_tiles = (int)sk;
-    }
-  }
-  if (d.sk_tiles) {
-    d.pairs = max_pairs;
-    d.partial_bytes = static_cast<size_t>(max_pairs) * 2 * 2 * kDpPartFloats * sizeof(float);
-    d.arrival_bytes = (static_cast<size_t>(d.sk_tiles) * 2 * sizeof(int) + 255) / 256 * 256;
-  }
-  return d;
 }
 
 // Raises a kernel's dynamic shared memory limit once per device.
@@ -131,41 +98,83 @@ static int allow_smem(const char* op, F* kernel, int bytes, std::atomic<unsigned
   return TAB_OK;
 }
 
-template <typename T, int EPI>
-static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMap& mb, const DenseParams& p, int pairs, cudaStream_t st) {
-  static std::atomic<unsigned long long> done{0};
-  const int rc = allow_smem(op, dense_pair_kernel<T, EPI>, kDpSmemBytes, done);
-  if (rc != TAB_OK) return rc;
-  dense_pair_kernel<T, EPI><<<2 * pairs, kDpThreads, kDpSmemBytes, st>>>(ma, mb, p);
+template <typename F>
+static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int smem, int cluster, bool under_previous, const CUtensorMap& ma,
+                          const CUtensorMap& mb, const DenseParams& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = under_previous ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TAB_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
   return check_launch(op);
 }
 
+// Pairs that share a tile's contraction when `tiles` tiles are all there is to do.  A cluster of 2 s CTAs needs 2 s free SMs in one
+// GPC: of the 148 SMs 72 fit into clusters of 8 or 4 alike.
+static int pair_split(int64_t tiles, int num_kb) {
+  for (int s = 4; s > 1; s /= 2)
+    if (tiles * s <= 72 && num_kb >= 4 * s) return s;
+  return 1;
+}
+
+template <typename T, int EPI>
+static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMap& mb, DenseParams& p, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0}, done_split{0};
+  const int64_t tiles = static_cast<int64_t>(p.row_tiles) * p.col_tiles;
+  const int pairs = dense_sms() / 2;
+  // whole tiles for the turns that fill all pairs, clusters for the rest where that is shorter than another whole turn
+  int64_t rest = tiles % pairs;
+  const int split = rest ? pair_split(rest, p.num_kb) : 1;
+  if (split == 1) rest = 0;
+  const int64_t whole = tiles - rest;
+  int rc = TAB_OK;
+  if (whole > 0) {
+    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, false>, kDpSmemBytes, done)) != TAB_OK) return rc;
+    p.tile_begin = 0;
+    p.tile_end = (int)whole;
+    p.split = 1;
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes, 2, false, ma, mb, p, st);
+    if (rc != TAB_OK) return rc;
+  }
+  if (rest > 0) {
+    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, true>, kDpSmemBytes, done_split)) != TAB_OK) return rc;
+    p.tile_begin = (int)whole;
+    p.tile_end = (int)tiles;
+    p.split = split;
+    // both launches read the same operands and write different tiles: the second may fill SMs that the first has left
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes, 2 * split, whole > 0, ma, mb, p, st);
+  }
+  return rc;
+}
+
 template <int EPI>
-static int launch_pair_epi(const char* op, int dtype, const DenseOperand& a, const DenseOperand& b, DenseParams& p, const DensePlan& plan, void* ws,
-                           size_t ws_bytes, cudaStream_t st) {
-  p.num_kb = plan.num_kb;
-  p.row_tiles = plan.row_tiles;
-  p.col_tiles = plan.col_tiles;
-  p.sk_tiles = plan.sk_tiles;
+static int launch_pair_epi(const char* op, int dtype, const DenseOperand& a, const DenseOperand& b, DenseParams& p, cudaStream_t st) {
+  p.num_kb = (int)((a.depth + kDnBlockK - 1) / kDnBlockK);
+  p.row_tiles = (p.M + 255) / 256;
+  p.col_tiles = (p.N + kDpTileCols<EPI> - 1) / kDpTileCols<EPI>;
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   p.idesc = ptx::idesc_f16(256, kDpCols, dtype == TAB_BF16 ? 1 : 0, a.mn, b.mn);
   p.wait_cycles = dense_wait_cycles();
-  if (plan.sk_tiles) {
-    if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u)) return fail(TAB_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", op);
-    if (ws_bytes < plan.partial_bytes + plan.arrival_bytes)
-      return fail(TAB_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", op, ws_bytes, plan.partial_bytes + plan.arrival_bytes);
-    p.arrivals = static_cast<int*>(ws);
-    p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.arrival_bytes);
-    const cudaError_t e = cudaMemsetAsync(ws, 0, plan.arrival_bytes, st);
-    if (e != cudaSuccess) return fail(TAB_ERR_CUDA, "%s: memset: %s", op, cudaGetErrorString(e));
-  }
   CUtensorMap ma, mb;
   int rc = make_map(op, a, 64, &ma);
   if (rc == TAB_OK) rc = make_map(op, b, 64, &mb);
   if (rc != TAB_OK) return rc;
-  return dtype == TAB_BF16 ? launch_pair_t<__nv_bfloat16, EPI>(op, ma, mb, p, plan.pairs, st)
-                           : launch_pair_t<__half, EPI>(op, ma, mb, p, plan.pairs, st);
+  return dtype == TAB_BF16 ? launch_pair_t<__nv_bfloat16, EPI>(op, ma, mb, p, st) : launch_pair_t<__half, EPI>(op, ma, mb, p, st);
 }
 
 // ---- narrow kernel ----
@@ -178,26 +187,7 @@ static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensor
   static std::atomic<unsigned long long> done{0};
   const int rc = allow_smem(op, dense_narrow_kernel<T, EPI>, kNwSmemTarget, done);
   if (rc != TAB_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * p.split));
-  cfg.blockDim = dim3(kNwThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)p.split;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = p.dependent ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, dense_narrow_kernel<T, EPI>, mw, mx, p);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return fail(TAB_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
-  }
-  return check_launch(op);
+  return launch_cluster(op, dense_narrow_kernel<T, EPI>, tiles * p.split, kNwThreads, smem, p.split, p.dependent != 0, mw, mx, p, st);
 }
 
 template <int EPI>
@@ -253,11 +243,8 @@ static int check_epilogue_ptrs(const char* op, const void* bias, const void* res
   return TAB_OK;
 }
 
-static size_t plan_bytes(const DensePlan& d) { return d.partial_bytes + d.arrival_bytes; }
-static size_t dense_ws(int64_t M, int64_t col_tiles, int64_t depth) { return M > 0 ? plan_bytes(dense_plan(M, col_tiles, depth)) : 0; }
-
 static int gated_matmul(const char* op, const DenseOperand& x, const DenseOperand& w, int dtype, int64_t M, int64_t I, const void* bias, int act,
-                        void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h, void* ws, size_t ws_bytes, cudaStream_t st) {
+                        void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h, cudaStream_t st) {
   DenseParams p = {};
   p.M = (int)M;
   p.N = (int)I;
@@ -270,12 +257,12 @@ static int gated_matmul(const char* op, const DenseOperand& x, const DenseOperan
   p.keep_ld = (int)keep_ld;
   p.keep_up = (int)(keep_q ? up64(I) : I);
   if (use_narrow(M, x)) return launch_narrow_epi<kEpiGlu>(op, dtype, x, w, p, st);
-  return launch_pair_epi<kEpiGlu>(op, dtype, x, w, p, dense_plan(M, (I + 127) / 128, x.depth), ws, ws_bytes, st);
+  return launch_pair_epi<kEpiGlu>(op, dtype, x, w, p, st);
 }
 
 static int linear_matmul(const char* op, const DenseOperand& a, const DenseOperand& b, int dtype, int64_t M, int64_t N, const void* bias,
                          const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* out, int dependent,
-                         void* ws, size_t ws_bytes, cudaStream_t st) {
+                         cudaStream_t st) {
   DenseParams p = {};
   p.M = (int)M;
   p.N = (int)N;
@@ -289,23 +276,16 @@ static int linear_matmul(const char* op, const DenseOperand& a, const DenseOpera
   p.keep_ld = (int)keep_ld;
   p.dependent = dependent;
   if (use_narrow(M, a)) return launch_narrow_epi<kEpiLinear>(op, dtype, a, b, p, st);
-  return launch_pair_epi<kEpiLinear>(op, dtype, a, b, p, dense_plan(M, (N + 255) / 256, a.depth), ws, ws_bytes, st);
+  return launch_pair_epi<kEpiLinear>(op, dtype, a, b, p, st);
 }
 
 }  // namespace tab
 
 using namespace tab;
 
-extern "C" int tab_dense_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, size_t* bytes) {
-  if (!bytes || M < 0 || N <= 0 || K <= 0) return fail(TAB_ERR_BAD_ARG, "dense_matmul: M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
-  const size_t linear = dense_ws(M, (N + 255) / 256, K), gated = dense_ws(M, (N + 127) / 128, K);
-  *bytes = linear > gated ? linear : gated;
-  return TAB_OK;
-}
-
 extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M, int64_t N,
                                 int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale,
-                                int64_t keep_ld, void* out, void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+                                int64_t keep_ld, void* out, tab_stream_t stream) {
   const char* op = "dense_matmul";
   int rc = check_dense(op, dtype, M, N, K, act);
   if (rc != TAB_OK || M == 0) return rc;
@@ -313,13 +293,12 @@ extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void
   if ((rc = check_operand(op, "a", oa)) != TAB_OK || (rc = check_operand(op, "b", ob)) != TAB_OK) return rc;
   if ((rc = check_epilogue_ptrs(op, bias, residual, out)) != TAB_OK) return rc;
   if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, keep_q ? up64(N) : N)) != TAB_OK) return rc;
-  return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0, workspace, workspace_bytes,
-                       as_stream(stream));
+  return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0, as_stream(stream));
 }
 
 extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
                                 int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h,
-                                void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+                                tab_stream_t stream) {
   const char* op = "gated_matmul";
   int rc = check_dense(op, dtype, M, I, K, act);
   if (rc != TAB_OK || M == 0) return rc;
@@ -327,12 +306,12 @@ extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, 
   if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
   if ((rc = check_epilogue_ptrs(op, bias, nullptr, h)) != TAB_OK) return rc;
   if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
-  return gated_matmul(op, ox, ow, dtype, M, I, bias, act, keep, keep_q, keep_scale, keep_ld, h, workspace, workspace_bytes, as_stream(stream));
+  return gated_matmul(op, ox, ow, dtype, M, I, bias, act, keep, keep_q, keep_scale, keep_ld, h, as_stream(stream));
 }
 
 extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
                                      int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld,
-                                     void* dz, void* h, void* workspace, size_t workspace_bytes, tab_stream_t stream) {
+                                     void* dz, void* h, tab_stream_t stream) {
   const char* op = "gated_matmul_grad";
   int rc = check_dense(op, dtype, M, I, K, act);
   if (rc != TAB_OK || M == 0) return rc;
@@ -352,16 +331,12 @@ extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* w
   p.keep_scale = const_cast<float*>(keep_scale);
   p.keep_ld = (int)keep_ld;
   p.keep_up = (int)(keep_q ? up64(I) : I);
-  return launch_pair_epi<kEpiGluGrad>(op, dtype, oa, ow, p, dense_plan(M, (I + 255) / 256, K), workspace, workspace_bytes, as_stream(stream));
+  return launch_pair_epi<kEpiGluGrad>(op, dtype, oa, ow, p, as_stream(stream));
 }
-
-// workspace of tab_gated_ffn: the hidden rows h [M, I], then what the split tiles of either product need
-static size_t ffn_h_bytes(int64_t M, int64_t I) { return (static_cast<size_t>(M) * I * 2 + 255) / 256 * 256; }
 
 extern "C" int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes) {
   if (!bytes || M < 0 || H <= 0 || I <= 0) return fail(TAB_ERR_BAD_ARG, "gated_ffn: M=%lld H=%lld I=%lld", (long long)M, (long long)H, (long long)I);
-  const size_t up = dense_ws(M, (I + 127) / 128, H), down = dense_ws(M, (H + 255) / 256, I);
-  *bytes = ffn_h_bytes(M, I) + (up > down ? up : down);
+  *bytes = static_cast<size_t>(M) * I * 2;                        // the hidden rows
   return TAB_OK;
 }
 
@@ -382,14 +357,11 @@ extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t
   tab_gated_ffn_workspace_bytes(M, H, I, &need);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u)) return fail(TAB_ERR_ALIGNMENT, "%s: workspace must be 256-byte aligned", op);
   if (workspace_bytes < need) return fail(TAB_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", op, workspace_bytes, need);
-  const size_t h_bytes = ffn_h_bytes(M, I);
-  void* rest = static_cast<uint8_t*>(workspace) + h_bytes;
-  const size_t rest_bytes = workspace_bytes - h_bytes;
   cudaStream_t st = as_stream(stream);
-  rc = gated_matmul(op, ox, o1, dtype, M, I, bias1, act, keep, keep_q, keep_scale, keep_ld, workspace, rest, rest_bytes, st);
+  rc = gated_matmul(op, ox, o1, dtype, M, I, bias1, act, keep, keep_q, keep_scale, keep_ld, workspace, st);
   if (rc != TAB_OK) return rc;
   const DenseOperand oh = {workspace, I, M, I, 0};
-  return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, rest, rest_bytes, st);
+  return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, st);
 }
 
 extern "C" int tab_dense_status_reset(tab_stream_t stream) {

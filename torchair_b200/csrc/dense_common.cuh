@@ -30,7 +30,7 @@ struct DenseParams {
   int N;             // columns of the product (kEpiGlu, kEpiGluGrad: inner features I); a multiple of 8
   int num_kb;        // blocks of 64 along the contraction
   int row_tiles, col_tiles;
-  int sk_tiles;      // tiles whose contraction is split evenly over the pairs (dense_pair.cuh)
+  int tile_begin, tile_end;   // tiles of this launch (dense_pair.cuh)
   int a_mn, b_mn;    // operand is contiguous along the product's rows / columns instead of along the contraction
   uint32_t idesc;
   int act;           // TAB_ACT_*
@@ -44,9 +44,7 @@ struct DenseParams {
   float* keep_scale;
   int keep_ld, keep_up;
   void* dgate;           // kEpiGluGrad: d(gate) in columns [0, N), d(up) in [N, 2 N) of rows of 2 N values
-  float* partials;       // split tiles: fp32 accumulators, one slot per CTA and partial tile
-  int* arrivals;         // split tiles: arrivals per tile and CTA rank, zero before the launch
-  int split;             // dense_narrow.cuh: CTAs of a cluster that share one tile's contraction
+  int split;             // CTAs (dense_pair.cuh: pairs) of a cluster that share one tile's contraction
   int stages, nt;        // dense_narrow.cuh: shared-memory stages, token columns of a tile
   int dependent;         // launched as dependent of the kernel that writes the token operand
   long long wait_cycles;

@@ -25,12 +25,6 @@ constexpr int kNwMaxSplit = 8;
 
 __host__ __device__ constexpr int dense_narrow_stage_bytes(int nt) { return kDnOperandBytes + nt * 128; }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 // 8 consecutive features of one token, summed over the cluster in rank order
 __device__ __forceinline__ void sum_parts8(uint32_t part_addr, int token, int feature, int split, float (&v)[8]) {
   const uint32_t off = part_addr + static_cast<uint32_t>(token * 128 + feature) * 4u;
@@ -39,8 +33,8 @@ __device__ __forceinline__ void sum_parts8(uint32_t part_addr, int token, int fe
   for (int r = 0; r < kNwMaxSplit; ++r)
     if (r < split) {
       const uint32_t at = ptx::mapa(off, static_cast<uint32_t>(r));
-      a[r] = ld_cluster_f4(at);
-      b[r] = ld_cluster_f4(at + 16);
+      a[r] = ptx::ld_cluster_f4(at);
+      b[r] = ptx::ld_cluster_f4(at + 16);
     }
   v[0] = a[0].x; v[1] = a[0].y; v[2] = a[0].z; v[3] = a[0].w;
   v[4] = b[0].x; v[5] = b[0].y; v[6] = b[0].z; v[7] = b[0].w;
@@ -127,60 +121,63 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   ptx::launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      const int f0 = EPI == kEpiGlu ? tile * 64 : tile * 128;
-      const int f1 = EPI == kEpiGlu ? p.N + f0 : f0 + 64;
-      auto load_w = [&](int s, int kb) {
-        const uint32_t st = tiles_addr + s * stage_bytes;
-        const int k = kb * kDnBlockK;
-        ptx::mbar_expect_tx(bar_full(s), static_cast<uint32_t>(stage_bytes));
-        if (p.a_mn) {
-          ptx::tma_load_2d(st, &tm_w, bar_full(s), f0, k);
-          ptx::tma_load_2d(st + kDnBoxBytes, &tm_w, bar_full(s), f1, k);
-        } else {
-          ptx::tma_load_2d(st, &tm_w, bar_full(s), k, f0);
-          ptx::tma_load_2d(st + kDnBoxBytes, &tm_w, bar_full(s), k, f1);
-        }
-      };
-      auto load_x = [&](int s, int kb) {
-        ptx::tma_load_2d(tiles_addr + s * stage_bytes + kDnOperandBytes, &tm_x, bar_full(s), kb * kDnBlockK, 0);
-      };
-      const int head = min(p.stages, n_kb);
+    const int f0 = EPI == kEpiGlu ? tile * 64 : tile * 128;
+    const int f1 = EPI == kEpiGlu ? p.N + f0 : f0 + 64;
+    auto load_w = [&](int s, int kb) {                   // by the elected lane
+      const uint32_t st = tiles_addr + s * stage_bytes;
+      const int k = kb * kDnBlockK;
+      ptx::mbar_expect_tx(bar_full(s), static_cast<uint32_t>(stage_bytes));
+      ptx::tma_load_2d(st, &tm_w, bar_full(s), p.a_mn ? f0 : k, p.a_mn ? k : f0);
+      ptx::tma_load_2d(st + kDnBoxBytes, &tm_w, bar_full(s), p.a_mn ? f1 : k, p.a_mn ? k : f1);
+    };
+    auto load_x = [&](int s, int kb) {
+      ptx::tma_load_2d(tiles_addr + s * stage_bytes + kDnOperandBytes, &tm_x, bar_full(s), kb * kDnBlockK, 0);
+    };
+    const int head = min(p.stages, n_kb);
+    if (ptx::elect_one()) {
       for (int i = 0; i < head; ++i) load_w(i, kb0 + i);
       ptx::dependency_wait();
       for (int i = 0; i < head; ++i) load_x(i, kb0 + i);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int i = head; i < n_kb; ++i) {
-        if (!dense_wait(bar_empty(stage), phase, s_abort, 41, p.wait_cycles)) break;
+    }
+    __syncwarp();
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = head; i < n_kb; ++i) {
+      if (!__all_sync(0xffffffffu, dense_wait(bar_empty(stage), phase, s_abort, 41, p.wait_cycles))) break;
+      if (ptx::elect_one()) {
         load_w(stage, kb0 + i);
         load_x(stage, kb0 + i);
-        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t a_step = p.a_mn ? 128u : 2u;
-      for (int i = 0; i < n_kb; ++i) {
-        if (!dense_wait(bar_full(stage), phase, s_abort, 42, p.wait_cycles)) { ok = false; break; }
-        ptx::tc_fence_after();
-        const uint32_t st = tiles_addr + stage * stage_bytes;
-        const uint64_t a = p.a_mn ? ptx::smem_desc_mn128(st, kDnBoxBytes) : ptx::smem_desc_k128(st);
-        const uint64_t b = ptx::smem_desc_k128(st + kDnOperandBytes);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t a_step = p.a_mn ? 128u : 2u;
+    for (int i = 0; i < n_kb; ++i) {
+      ok = __all_sync(0xffffffffu, dense_wait(bar_full(stage), phase, s_abort, 42, p.wait_cycles));
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t st = tiles_addr + stage * stage_bytes;
+      const uint64_t a = p.a_mn ? ptx::smem_desc_mn128(st, kDnBoxBytes) : ptx::smem_desc_k128(st);
+      const uint64_t b = ptx::smem_desc_k128(st + kDnOperandBytes);
+      if (ptx::elect_one()) {
 #pragma unroll
         for (int k = 0; k < kDnBlockK / 16; ++k) ptx::mma_f16(tmem_base, a + k * a_step, b + k * 2, p.idesc, (i | k) != 0 ? 1u : 0u);
         ptx::mma_commit(bar_empty(stage));
-        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
-      // also after a wait that gave up: the barrier then says that no MMA is in flight any more
-      ptx::mma_commit(bar_tfull);
-      if (!ok) {
-        const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(bar_tfull, 0) && clock64() - t0 < p.wait_cycles) {}
-      }
+      __syncwarp();
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+    }
+    // also after a wait that gave up: the barrier then says that no MMA is in flight any more
+    if (ptx::elect_one()) ptx::mma_commit(bar_tfull);
+    __syncwarp();
+    if (!ok) {
+      const long long t0 = clock64();
+      while (!ptx::mbar_try_wait(bar_tfull, 0) && clock64() - t0 < p.wait_cycles) {}
+      __syncwarp();
     }
   } else {
     const bool got = dense_wait(bar_tfull, 0, s_abort, 43, p.wait_cycles) && *s_abort == 0;

@@ -13,11 +13,15 @@
 // kinds of stage consist of 8 KB TMA boxes of 64 rows x 128 bytes with the 128-byte swizzle; only the coordinates, the
 // matrix descriptors and the step from one 16-wide MMA slice to the next differ.
 //
-// Split tiles.  With one tile per pair and turn, the last turn leaves pairs idle (88 tiles on 74 pairs take two turns).
-// The host may hand the first sk_tiles tiles out by contraction blocks instead: pair p takes blocks [p U / P, (p+1) U / P)
-// of the U = sk_tiles * num_kb blocks.  A CTA that holds only part of a tile stores its fp32 accumulators to a slot of its
-// own and counts its arrival; the CTA that arrives last adds all parts in the order of the contraction (so the result does
-// not depend on who came last) and runs the epilogue.  Nobody waits for anybody: the kernel needs no co-residency.
+// Few tiles.  A product with fewer tiles than pairs leaves SMs idle, and so does the last, partly filled turn of a larger one.
+// SPLIT launches give such tiles to clusters of `split` pairs: each pair takes a part of the contraction, leaves its fp32
+// accumulators in its own shared memory, and after a cluster barrier finishes its share of the tile's columns, adding the
+// parts from distributed shared memory in the order of the contraction.  No workspace, no atomics, no waiting for CTAs that may
+// not be resident.  (An earlier form handed out blocks of the contraction evenly over all pairs and joined the parts through
+// global memory: 136.9 us instead of 104.5 us for 4096 x 2048 x 8192, where whole tiles fill 1.73 turns.)
+//
+// Issue.  The producer and MMA loops run on whole warps and elect a lane around the issuing instructions.  Run by a single
+// lane, the same loops took 640 cycles per block of the contraction, the MMAs themselves 512 (now 520; 8192^3: 762 -> 728 us).
 //
 // Protocol of the pair: as in gmm_i8_pair.cuh (loads of both CTAs complete on the leader's full barrier, the leader issues
 // the MMAs and commits to both CTAs' empty / accumulator-full barriers, a bounded hand-shake ends the kernel).
@@ -38,53 +42,7 @@ constexpr int kDpPitch = 80;                           // staged row: 32 16-bit 
 constexpr int kDpPatchBytes = 32 * kDpPitch;           // one epilogue warp's 32 rows
 constexpr int kDpSmemBytes = 1024 + kDpStages * kDpStageBytes + kDpCtrlBytes + kDpEpiWarps * kDpPatchBytes;
 static_assert(kDpSmemBytes <= kDnSmemLimit, "dense pair GEMM shared memory");
-constexpr int64_t kDpPartFloats = 128 * kDpCols;       // accumulators of one CTA and tile
-
-// Work of one pair: segments of tiles.  Split tiles come first, so that their joins run under the whole tiles behind them.
-struct DenseWork {
-  int tile, kb0, kb1;
-};
-__host__ __device__ __forceinline__ int64_t dense_unit_begin(int p, int64_t units, int pairs) { return p * units / pairs; }
-// pair that holds unit u
-__host__ __device__ __forceinline__ int dense_unit_owner(int64_t u, int64_t units, int pairs) {
-  int p = static_cast<int>(u * pairs / units);
-  while (p + 1 < pairs && dense_unit_begin(p + 1, units, pairs) <= u) ++p;
-  while (p > 0 && dense_unit_begin(p, units, pairs) > u) --p;
-  return p;
-}
-struct DenseSched {
-  int64_t u, u_end;
-  int next_tile, tiles, num_kb, pairs;
-  __host__ __device__ DenseSched(int pair, int pairs_, int sk_tiles, int tiles_, int num_kb_) {
-    const int64_t units = static_cast<int64_t>(sk_tiles) * num_kb_;
-    u = dense_unit_begin(pair, units, pairs_);
-    u_end = dense_unit_begin(pair + 1, units, pairs_);
-    next_tile = sk_tiles + pair;
-    tiles = tiles_;
-    num_kb = num_kb_;
-    pairs = pairs_;
-  }
-  __host__ __device__ bool next(DenseWork& w) {
-    if (u < u_end) {
-      w.tile = static_cast<int>(u / num_kb);
-      w.kb0 = static_cast<int>(u - static_cast<int64_t>(w.tile) * num_kb);
-      const int64_t left = u_end - u;
-      w.kb1 = left < num_kb - w.kb0 ? w.kb0 + static_cast<int>(left) : num_kb;
-      u += w.kb1 - w.kb0;
-      return true;
-    }
-    if (next_tile < tiles) {
-      w.tile = next_tile;
-      w.kb0 = 0;
-      w.kb1 = num_kb;
-      next_tile += pairs;
-      return true;
-    }
-    return false;
-  }
-};
-// A pair has at most one part that does not begin its tile (slot 0) and one that does but does not end it (slot 1).
-__host__ __device__ __forceinline__ int dense_slot(int pair, int kb0) { return 2 * pair + (kb0 == 0 ? 1 : 0); }
+static_assert(128 * kDpCols * 4 <= kDpStages * kDpStageBytes, "a CTA's accumulators fit into its ring");
 
 // Tiles are numbered so that the tiles in flight share operands: column by column inside bands of kDpBand row tiles.
 constexpr int kDpBand = 8;
@@ -205,140 +163,119 @@ __device__ __forceinline__ void load_q32(float (&v)[32], const int8_t* q, float 
     for (int i = 0; i < 4; ++i) v[4 * k + i] = static_cast<float>(static_cast<int8_t>(w[k] >> (8 * i))) * scale;
 }
 
-// Where the epilogue takes a tile's accumulators from: tensor memory, or (split tiles) the parts of all contributors in the
-// order of the contraction, its own part from tensor memory.
+// Where the epilogue takes a tile's accumulators from: tensor memory, or (split tiles) the parts of all pairs of the cluster,
+// added in the order of the contraction.
 struct DenseAcc {
   uint32_t taddr;          // this warp's lanes, first column of the buffer
-  const float* parts;      // null: whole tile in tensor memory
-  int64_t units;
-  int pairs, num_kb, tile, self, first, last;
-  int rank, row_local;
+  uint32_t part;           // 0, or the shared-memory address of this thread's row in the parts: float4 [column / 4][128 rows]
+  int split, parity;       // pairs of the cluster, which CTA of its pair this is
   __device__ __forceinline__ void fetch(int c, float (&v)[32]) const {
     __syncwarp();
-    if (parts == nullptr) {
+    if (part == 0) {
       ptx::tmem_ld32f(taddr + c, v);
       ptx::tmem_ld_wait();
       return;
     }
-    const int64_t tile_u = static_cast<int64_t>(tile) * num_kb;
-    for (int p = first; p <= last; ++p) {
-      float t[32];
-      if (p == self) {
-        ptx::tmem_ld32f(taddr + c, t);
-        ptx::tmem_ld_wait();
-      } else {
-        const int64_t b = dense_unit_begin(p, units, pairs);
-        const int kb0 = b > tile_u ? static_cast<int>(b - tile_u) : 0;
-        const float4* src = reinterpret_cast<const float4*>(parts + (static_cast<int64_t>(dense_slot(p, kb0)) * 2 + rank) * kDpPartFloats) +
-                            static_cast<int64_t>(c >> 2) * 128 + row_local;
+    const uint32_t at = part + static_cast<uint32_t>(c >> 2) * 2048u;
+#pragma unroll 1
+    for (int s = 0; s < split; ++s) {
+      const uint32_t from = ptx::mapa(at, static_cast<uint32_t>(2 * s + parity));
+      float4 t[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float4 x = __ldcg(src + k * 128);
-          t[4 * k] = x.x;
-          t[4 * k + 1] = x.y;
-          t[4 * k + 2] = x.z;
-          t[4 * k + 3] = x.w;
-        }
-      }
-      if (p == first) {
+      for (int k = 0; k < 8; ++k) t[k] = ptx::ld_cluster_f4(from + k * 2048u);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = t[j];
-      } else {
+      for (int k = 0; k < 8; ++k) {
+        const float x[4] = {t[k].x, t[k].y, t[k].z, t[k].w};
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] += t[j];
+        for (int j = 0; j < 4; ++j) v[4 * k + j] = s == 0 ? x[j] : v[4 * k + j] + x[j];
       }
     }
   }
 };
 
-// Epilogue of one warp: 32 rows (row_base ..) x half of the tile's accumulator columns.
+// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 32; of 64
+// where 8-bit blocks are written).
 template <typename T, int EPI>
 __device__ __forceinline__ void dense_epilogue(const DenseParams& p, const DenseAcc& acc, uint8_t* patch, int lane, int row_base, int ct,
-                                               int chalf) {
+                                               int col_begin, int col_end) {
   const int row = row_base + lane;
   const bool rvalid = row < p.M;
   if constexpr (EPI == kEpiLinear) {
+    RowQuant rq;
 #pragma unroll 1
-    for (int blk = chalf * 128; blk < chalf * 128 + 128; blk += 64) {       // 64 columns: one 8-bit block
-      const int col0 = ct * 256 + blk;
-      if (col0 >= p.N) break;
-      RowQuant rq;
-      if (p.keep_q != nullptr) {
+    for (int c = col_begin; c < col_end; c += 32) {
+      const int col = ct * 256 + c;
+      if (col >= p.N && (p.keep_q == nullptr || (col & ~63) >= p.N)) break;
+      if (p.keep_q != nullptr && (c & 63) == 0) {                        // amax of the 64-value block first
         uint32_t m = 0;
 #pragma unroll 1
-        for (int c = 0; c < 64; c += 32) {
+        for (int h = 0; h < 64; h += 32) {
           float v[32];
-          acc.fetch(blk + c, v);
-          add_bias32<T>(v, p.bias, col0 + c, p.N);
-          m = max(m, chunk_amax_bits(v, col0 + c, p.N));
+          acc.fetch(c + h, v);
+          add_bias32<T>(v, p.bias, col + h, p.N);
+          m = max(m, chunk_amax_bits(v, col + h, p.N));
         }
         rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
-        if (rvalid) p.keep_scale[static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col0 / kKeepBlock] = rq.scale;
+        if (rvalid) p.keep_scale[static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col / kKeepBlock] = rq.scale;
       }
-#pragma unroll 1
-      for (int c = 0; c < 64; c += 32) {
-        const int col = col0 + c;
-        if (col >= p.N && p.keep_q == nullptr) break;
-        float v[32];
-        acc.fetch(blk + c, v);
-        add_bias32<T>(v, p.bias, col, p.N);
-        if (p.keep_q != nullptr) {
-          if (rvalid) store_q32(v, rq, p.keep_q + static_cast<int64_t>(row) * p.keep_ld + col, col, p.N);
-        } else if (p.keep != nullptr) {
-          store_rows32<T>(patch, lane, v, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
-        }
-        if (col >= p.N) continue;
-        if (p.act != TAB_ACT_NONE)
-          with_act(p.act, [&](auto tag) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
-          });
-        if (p.residual != nullptr) {
-          uint32_t r[16];
-          load_rows32<T>(patch, lane, r, static_cast<const T*>(p.residual), p.N, row_base, p.M, col, p.N);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 f = unpack2<T>(r[j]);
-            v[2 * j] += f.x;
-            v[2 * j + 1] += f.y;
-          }
-        }
-        store_rows32<T>(patch, lane, v, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      float v[32];
+      acc.fetch(c, v);
+      add_bias32<T>(v, p.bias, col, p.N);
+      if (p.keep_q != nullptr) {
+        if (rvalid) store_q32(v, rq, p.keep_q + static_cast<int64_t>(row) * p.keep_ld + col, col, p.N);
+      } else if (p.keep != nullptr) {
+        store_rows32<T>(patch, lane, v, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
       }
+      if (col >= p.N) continue;
+      if (p.act != TAB_ACT_NONE)
+        with_act(p.act, [&](auto tag) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
+        });
+      if (p.residual != nullptr) {
+        uint32_t r[16];
+        load_rows32<T>(patch, lane, r, static_cast<const T*>(p.residual), p.N, row_base, p.M, col, p.N);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float2 f = unpack2<T>(r[j]);
+          v[2 * j] += f.x;
+          v[2 * j + 1] += f.y;
+        }
+      }
+      store_rows32<T>(patch, lane, v, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
     }
   } else if constexpr (EPI == kEpiGlu) {
-    // accumulator columns [128 chalf, +64) are gate features col0 .., [128 chalf + 64, +64) the matching up features
-    const int col0 = ct * 128 + chalf * 64;
-    if (col0 >= p.N) return;
+    // output column c of the tile: its gate is accumulator column (c / 64) * 128 + c % 64, its up value 64 columns further
     const T* bias_up = p.bias ? static_cast<const T*>(p.bias) + p.N : nullptr;
     RowQuant rg, ru;
-    if (p.keep_q != nullptr) {
-      uint32_t mg = 0, mu = 0;
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 32) {
-        float v[32];
-        acc.fetch(chalf * 128 + c, v);
-        add_bias32<T>(v, p.bias, col0 + c, p.N);
-        mg = max(mg, chunk_amax_bits(v, col0 + c, p.N));
-        acc.fetch(chalf * 128 + 64 + c, v);
-        add_bias32<T>(v, bias_up, col0 + c, p.N);
-        mu = max(mu, chunk_amax_bits(v, col0 + c, p.N));
-      }
-      rg = make_block_quant(__uint_as_float(mg), mg < 0x7f800000u);
-      ru = make_block_quant(__uint_as_float(mu), mu < 0x7f800000u);
-      if (rvalid) {
-        float* s = p.keep_scale + static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col0 / kKeepBlock;
-        s[0] = rg.scale;
-        s[p.keep_up / kKeepBlock] = ru.scale;
-      }
-    }
+    for (int c = col_begin; c < col_end; c += 32) {
+      const int col = ct * 128 + c;
+      if (col >= p.N && (p.keep_q == nullptr || (col & ~63) >= p.N)) break;
+      const int at = (c >> 6) * 128 + (c & 63);
+      if (p.keep_q != nullptr && (c & 63) == 0) {
+        uint32_t mg = 0, mu = 0;
 #pragma unroll 1
-    for (int c = 0; c < 64; c += 32) {
-      const int col = col0 + c;
-      if (col >= p.N && p.keep_q == nullptr) break;
+        for (int h = 0; h < 64; h += 32) {
+          float v[32];
+          acc.fetch(at + h, v);
+          add_bias32<T>(v, p.bias, col + h, p.N);
+          mg = max(mg, chunk_amax_bits(v, col + h, p.N));
+          acc.fetch(at + 64 + h, v);
+          add_bias32<T>(v, bias_up, col + h, p.N);
+          mu = max(mu, chunk_amax_bits(v, col + h, p.N));
+        }
+        rg = make_block_quant(__uint_as_float(mg), mg < 0x7f800000u);
+        ru = make_block_quant(__uint_as_float(mu), mu < 0x7f800000u);
+        if (rvalid) {
+          float* s = p.keep_scale + static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
+          s[0] = rg.scale;
+          s[p.keep_up / kKeepBlock] = ru.scale;
+        }
+      }
       float g[32], u[32];
-      acc.fetch(chalf * 128 + c, g);
-      acc.fetch(chalf * 128 + 64 + c, u);
+      acc.fetch(at, g);
+      acc.fetch(at + 64, u);
       add_bias32<T>(g, p.bias, col, p.N);
       add_bias32<T>(u, bias_up, col, p.N);
       if (p.keep_q != nullptr) {
@@ -360,7 +297,7 @@ __device__ __forceinline__ void dense_epilogue(const DenseParams& p, const Dense
     }
   } else {
 #pragma unroll 1
-    for (int c = chalf * 128; c < chalf * 128 + 128; c += 32) {
+    for (int c = col_begin; c < col_end; c += 32) {
       const int col = ct * 256 + c;
       if (col >= p.N) break;
       float g[32], u[32], dh[32];
@@ -411,8 +348,12 @@ __device__ __forceinline__ void dense_epilogue(const DenseParams& p, const Dense
   }
 }
 
-template <typename T, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDpThreads, 1)
+// Output columns of a tile: 256, or 128 where gate and up share the accumulator.
+template <int EPI>
+constexpr int kDpTileCols = EPI == kEpiGlu ? 128 : 256;
+
+template <typename T, int EPI, bool SPLIT>
+__global__ void __launch_bounds__(kDpThreads, 1)
 dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const DenseParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
@@ -430,14 +371,19 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(ctrl + 224);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_got = reinterpret_cast<volatile int*>(s_tmem + 2);     // [2] outcome of the epilogue's wait, per buffer
-  volatile int* s_last = reinterpret_cast<volatile int*>(s_tmem + 4);    // this CTA arrived last at the split tile
   uint8_t* s_out = ctrl + kDpCtrlBytes;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const uint32_t cta = ptx::cluster_ctarank();
+  const int rank = static_cast<int>(cta & 1u);           // within the pair
+  const uint32_t leader_cta = cta & ~1u;
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = p.row_tiles * p.col_tiles;
+  // this pair's tiles: one of them for the whole cluster, or every `step`-th one
+  const int split = SPLIT ? p.split : 1, part = SPLIT ? static_cast<int>(cta >> 1) : 0;
+  const int first = p.tile_begin + static_cast<int>(blockIdx.x) / (2 * split);
+  const int step = SPLIT ? p.tile_end : static_cast<int>(gridDim.x >> 1);
+  const int kb_begin = SPLIT ? static_cast<int>(static_cast<int64_t>(part) * p.num_kb / split) : 0;
+  const int kb_end = SPLIT ? static_cast<int>(static_cast<int64_t>(part + 1) * p.num_kb / split) : p.num_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kDpStages; ++s) {
@@ -461,160 +407,164 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   ptx::cluster_sync_all();          // both CTAs' barriers exist before anything signals across the pair
   ptx::tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  ptx::launch_dependents();
 
   if (warp == 0) {
     // ---------------- TMA producer (one per CTA): own 128 rows of A, own half of the tile's rows of B ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      DenseSched sched(pair, pairs, p.sk_tiles, tiles, p.num_kb);
-      DenseWork w;
-      while (ok && sched.next(w)) {
-        int rt, ct;
-        dense_tile_coord(w.tile, p.row_tiles, p.col_tiles, rt, ct);
-        const int a0 = rt * 256 + rank * 128;
-        const int b0 = EPI == kEpiGlu ? ct * 128 + rank * 64 : ct * 256 + rank * 128;
-        const int b1 = EPI == kEpiGlu ? p.N + b0 : b0 + 64;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!dense_wait(bar_empty(stage), phase ^ 1u, s_abort, 31, p.wait_cycles)) { ok = false; break; }
-          const uint32_t st = tiles_addr + stage * kDpStageBytes;
-          const uint32_t full_leader = ptx::mapa(bar_full(stage), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full0 = ptx::mapa(bar_full(0), leader_cta);
+    for (int tile = first; ok && tile < p.tile_end; tile += step) {
+      int rt, ct;
+      dense_tile_coord(tile, p.row_tiles, p.col_tiles, rt, ct);
+      const int a0 = rt * 256 + rank * 128;
+      const int b0 = EPI == kEpiGlu ? ct * 128 + rank * 64 : ct * 256 + rank * 128;
+      const int b1 = EPI == kEpiGlu ? p.N + b0 : b0 + 64;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        ok = __all_sync(0xffffffffu, dense_wait(bar_empty(stage), phase ^ 1u, s_abort, 31, p.wait_cycles));
+        if (!ok) break;
+        const uint32_t st = tiles_addr + stage * kDpStageBytes;
+        const uint32_t sb = st + kDnOperandBytes;
+        const uint32_t full_leader = full0 + 8u * stage;
+        const int k = kb * kDnBlockK;
+        if (ptx::elect_one()) {
           if (leader) ptx::mbar_expect_tx(bar_full(stage), 2 * kDpStageBytes);
-          const int k = kb * kDnBlockK;
-          if (p.a_mn) {
-            ptx::tma_load_2d_pair(st, &tm_a, full_leader, a0, k);
-            ptx::tma_load_2d_pair(st + kDnBoxBytes, &tm_a, full_leader, a0 + 64, k);
-          } else {
-            ptx::tma_load_2d_pair(st, &tm_a, full_leader, k, a0);
-            ptx::tma_load_2d_pair(st + kDnBoxBytes, &tm_a, full_leader, k, a0 + 64);
-          }
-          const uint32_t sb = st + kDnOperandBytes;
-          if (p.b_mn) {
-            ptx::tma_load_2d_pair(sb, &tm_b, full_leader, b0, k);
-            ptx::tma_load_2d_pair(sb + kDnBoxBytes, &tm_b, full_leader, b1, k);
-          } else {
-            ptx::tma_load_2d_pair(sb, &tm_b, full_leader, k, b0);
-            ptx::tma_load_2d_pair(sb + kDnBoxBytes, &tm_b, full_leader, k, b1);
-          }
-          if (++stage == kDpStages) { stage = 0; phase ^= 1u; }
+          // coordinates: contiguous index first
+          ptx::tma_load_2d_pair(st, &tm_a, full_leader, p.a_mn ? a0 : k, p.a_mn ? k : a0);
+          ptx::tma_load_2d_pair(st + kDnBoxBytes, &tm_a, full_leader, p.a_mn ? a0 + 64 : k, p.a_mn ? k : a0 + 64);
+          ptx::tma_load_2d_pair(sb, &tm_b, full_leader, p.b_mn ? b0 : k, p.b_mn ? k : b0);
+          ptx::tma_load_2d_pair(sb + kDnBoxBytes, &tm_b, full_leader, p.b_mn ? b1 : k, p.b_mn ? k : b1);
         }
+        __syncwarp();
+        if (++stage == kDpStages) { stage = 0; phase ^= 1u; }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer: the leader's warp, for both CTAs ----------------
-    if (lane == 0 && leader) {
+    if (leader) {
       int stage = 0, buf = 0;
       uint32_t phase = 0, tphase = 0;
       bool ok = true;
+      const uint16_t both = static_cast<uint16_t>(3u << leader_cta);
       const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;    // 16 contraction elements, in 16-byte units
-      DenseSched sched(pair, pairs, p.sk_tiles, tiles, p.num_kb);
-      DenseWork w;
-      while (sched.next(w)) {
-        if (!dense_wait(bar_tempty(buf), tphase ^ 1u, s_abort, 32, p.wait_cycles)) { ok = false; break; }
+      const uint64_t a_first = p.a_mn ? ptx::smem_desc_mn128(tiles_addr, kDnBoxBytes) : ptx::smem_desc_k128(tiles_addr);
+      const uint64_t b_first = p.b_mn ? ptx::smem_desc_mn128(tiles_addr + kDnOperandBytes, kDnBoxBytes) : ptx::smem_desc_k128(tiles_addr + kDnOperandBytes);
+      for (int tile = first; ok && tile < p.tile_end; tile += step) {
+        ok = __all_sync(0xffffffffu, dense_wait(bar_tempty(buf), tphase ^ 1u, s_abort, 32, p.wait_cycles));
+        if (!ok) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem_base + buf * kDpCols;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!dense_wait(bar_full(stage), phase, s_abort, 33, p.wait_cycles)) { ok = false; break; }
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          ok = __all_sync(0xffffffffu, dense_wait(bar_full(stage), phase, s_abort, 33, p.wait_cycles));
+          if (!ok) break;
           ptx::tc_fence_after();
-          const uint32_t st = tiles_addr + stage * kDpStageBytes;
-          const uint64_t a = p.a_mn ? ptx::smem_desc_mn128(st, kDnBoxBytes) : ptx::smem_desc_k128(st);
-          const uint64_t b = p.b_mn ? ptx::smem_desc_mn128(st + kDnOperandBytes, kDnBoxBytes) : ptx::smem_desc_k128(st + kDnOperandBytes);
+          const uint64_t a = a_first + static_cast<uint64_t>(stage * (kDpStageBytes >> 4));
+          const uint64_t b = b_first + static_cast<uint64_t>(stage * (kDpStageBytes >> 4));
+          if (ptx::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kDnBlockK / 16; ++k)
-            ptx::mma_f16_pair(d, a + k * a_step, b + k * b_step, p.idesc, (kb > w.kb0 || k > 0) ? 1u : 0u);
-          ptx::mma_commit_pair(bar_empty(stage));
+            for (int k = 0; k < kDnBlockK / 16; ++k)
+              ptx::mma_f16_pair(d, a + k * a_step, b + k * b_step, p.idesc, (kb > kb_begin || k > 0) ? 1u : 0u);
+            ptx::mma_commit_mask(bar_empty(stage), both);
+          }
+          __syncwarp();
           if (++stage == kDpStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        ptx::mma_commit_pair(bar_tfull(buf));
+        if (ptx::elect_one()) ptx::mma_commit_mask(bar_tfull(buf), both);
+        __syncwarp();
         if (++buf == kDpBufs) { buf = 0; tphase ^= 1u; }
       }
-      if (!ok) {
-        ptx::mma_commit_pair(bar_drain);
+      if (!ok && lane == 0) {
+        ptx::mma_commit_mask(bar_drain, both);
         const long long t0 = clock64();
         while (!ptx::mbar_try_wait(bar_drain, 0) && clock64() - t0 < p.wait_cycles) {}
       }
     }
   } else {
-    // ---------------- epilogue: warps 2..9, thread = row, two warps split the columns of a row ----------------
+    // ---------------- epilogue: warps 2..9, thread = row, two warps share the columns of a row ----------------
     const int quarter = warp & 3;
-    const int chalf = (warp - 2) >> 2;
+    const int half = (warp - 2) >> 2;
     const int et = threadIdx.x - 64;
-    uint8_t* patch = s_out + (warp - 2) * kDpPatchBytes;
     int buf = 0;
     uint32_t tphase = 0;
     DenseAcc acc;
-    acc.units = static_cast<int64_t>(p.sk_tiles) * p.num_kb;
-    acc.pairs = pairs;
-    acc.num_kb = p.num_kb;
-    acc.self = pair;
-    acc.rank = rank;
-    acc.row_local = quarter * 32 + lane;
-    DenseSched sched(pair, pairs, p.sk_tiles, tiles, p.num_kb);
-    DenseWork w;
-    while (sched.next(w)) {
+    acc.part = 0;
+    for (int tile = first; tile < p.tile_end; tile += step) {
       if (et == 0) s_got[buf] = dense_wait(bar_tfull(buf), tphase, s_abort, 34, p.wait_cycles) ? 1 : 0;
       dense_epi_bar();
       if (!s_got[buf]) break;
       ptx::tc_fence_after();
-      int rt, ct;
-      dense_tile_coord(w.tile, p.row_tiles, p.col_tiles, rt, ct);
       acc.taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kDpCols;
-      acc.parts = nullptr;
-      acc.tile = w.tile;
-      bool finish = true;
-      if (w.kb1 - w.kb0 < p.num_kb) {
-        // part of a split tile: store it, count the arrival, and only the last CTA to arrive goes on
-        float4* dst = reinterpret_cast<float4*>(p.partials + (static_cast<int64_t>(dense_slot(pair, w.kb0)) * 2 + rank) * kDpPartFloats);
+      if constexpr (SPLIT) {
+        // all MMAs of this pair are done, so its ring is free: it takes the 128 x 256 accumulators
+        const uint32_t dst = tiles_addr + static_cast<uint32_t>(quarter * 32 + lane) * 16u;
 #pragma unroll 1
-        for (int c = chalf * 128; c < chalf * 128 + 128; c += 32) {
+        for (int c = half * 128; c < half * 128 + 128; c += 32) {
           float v[32];
           acc.fetch(c, v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) __stcg(dst + ((c >> 2) + k) * 128 + acc.row_local, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+          for (int k = 0; k < 8; ++k) ptx::st_shared_f4(dst + static_cast<uint32_t>((c >> 2) + k) * 2048u, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
         }
-        const int64_t u0 = static_cast<int64_t>(w.tile) * p.num_kb;
-        acc.first = dense_unit_owner(u0, acc.units, pairs);
-        acc.last = dense_unit_owner(u0 + p.num_kb - 1, acc.units, pairs);
-        __threadfence();
-        dense_epi_bar();
-        if (et == 0) {
-          const int before = atomicAdd(p.arrivals + w.tile * 2 + rank, 1);
-          *s_last = before == acc.last - acc.first ? 1 : 0;
-          __threadfence();
-        }
-        dense_epi_bar();
-        finish = *s_last != 0;
-        acc.parts = p.partials;
+      } else {
+        int rt, ct;
+        dense_tile_coord(tile, p.row_tiles, p.col_tiles, rt, ct);
+        const int row_base = rt * 256 + rank * 128 + quarter * 32;
+        constexpr int kHalf = kDpTileCols<EPI> / 2;
+        if (row_base < p.M) dense_epilogue<T, EPI>(p, acc, s_out + (warp - 2) * kDpPatchBytes, lane, row_base, ct, half * kHalf, half * kHalf + kHalf);
       }
-      const int row_base = rt * 256 + rank * 128 + quarter * 32;
-      if (finish && row_base < p.M) dense_epilogue<T, EPI>(p, acc, patch, lane, row_base, ct, chalf);
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(bar_tempty(buf), 0));   // the leader counts both CTAs' warps
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(bar_tempty(buf), leader_cta));   // the leader counts both CTAs' warps
       if (++buf == kDpBufs) { buf = 0; tphase ^= 1u; }
     }
   }
 
-  // End of the pair's work: tell the peer, wait (bounded) for the peer, then release tensor memory (gmm_i8_pair.cuh).
   ptx::tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    ptx::mbar_arrive_cluster(ptx::mapa(bar_done, static_cast<uint32_t>(rank) ^ 1u));
-    const long long t0 = clock64();
-    while (!ptx::mbar_try_wait(bar_done, 0)) {
-      if (clock64() - t0 > p.wait_cycles) {
-        atomicCAS(&g_dense_status, 0, 35);
-        break;
+  if constexpr (SPLIT) {
+    ptx::cluster_sync_all();          // every pair's part is in place
+    if (warp >= 2) {
+      // this pair's share of the tile's columns, halved again between the two warps of a row; 64-value blocks are not cut, so
+      // with four pairs some hold no share (which pairs share a tile must not depend on what is kept: the sums would differ)
+      int rt, ct;
+      dense_tile_coord(first, p.row_tiles, p.col_tiles, rt, ct);
+      const int quarter = warp & 3, half = (warp - 2) >> 2;
+      const int unit = p.keep_q != nullptr && EPI != kEpiGluGrad ? 64 : 32;
+      const int share = max(kDpTileCols<EPI> / split, unit);
+      const int mid = share / 2 % unit == 0 ? share / 2 : share;
+      const int begin = part * share + (half ? mid : 0);
+      const int end = min(part * share + (half ? share : mid), kDpTileCols<EPI>);
+      const int row_base = rt * 256 + rank * 128 + quarter * 32;
+      DenseAcc acc;
+      acc.taddr = 0;
+      acc.part = tiles_addr + static_cast<uint32_t>(quarter * 32 + lane) * 16u;
+      acc.split = split;
+      acc.parity = rank;
+      if (row_base < p.M) dense_epilogue<T, EPI>(p, acc, s_out + (warp - 2) * kDpPatchBytes, lane, row_base, ct, begin, end);
+    }
+    __syncthreads();
+    ptx::cluster_sync_all();          // nobody leaves while another still reads its part or its operands
+  } else {
+    // The peer may still read this CTA's shared memory (its MMAs) or signal its barriers: tell the peer, wait (bounded) for it.
+    if (threadIdx.x == 0) {
+      ptx::mbar_arrive_cluster(ptx::mapa(bar_done, cta ^ 1u));
+      const long long t0 = clock64();
+      while (!ptx::mbar_try_wait(bar_done, 0)) {
+        if (clock64() - t0 > p.wait_cycles) {
+          atomicCAS(&g_dense_status, 0, 35);
+          break;
+        }
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair<kDpBufs * kDpCols>(tmem_base);
   }
+  // a launch that was allowed to start under the one before it ends only after that one has
+  if (threadIdx.x == 0) ptx::dependency_wait();
 }
 
 }  // namespace tab

@@ -189,6 +189,20 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
                ::"r"(bar), "h"(mask) : "memory");
 }
 
+// True in one lane of a converged warp.  Loops that issue copies or MMAs run on the whole warp and branch on this around the
+// issuing instructions only: their operands are then visibly uniform over the warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // ---- 16-bit floating-point operands ----
 
 // D[tmem] (+)= A[smem desc] x B[smem desc], bf16 or fp16 operands (the same type for both), fp32 accumulators.
@@ -212,6 +226,22 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, u
       "}\n"
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// Arrives on the mbarrier at this shared-memory offset in the CTAs of `mask` once the MMAs issued so far are done.
+__device__ __forceinline__ void mma_commit_mask(uint32_t bar, uint16_t mask) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"(mask) : "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_f4(uint32_t addr, float4 v) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // 32 consecutive fp32 columns of this thread's TMEM lane.

@@ -174,11 +174,8 @@ struct Kept {
 // act(a b^T + bias) + residual: a [m, k], b [n, k] as operands
 void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int64_t m, int64_t n, int64_t k, const Tensor& out,
             const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept()) {
-  size_t bytes = 0;
-  ok(tab_dense_matmul_workspace_bytes(m, n, k, &bytes), "tab_dense_matmul_workspace_bytes");
-  Tensor ws = bytes ? c.workspace(bytes) : Tensor();
   ok(tab_dense_matmul(a, lda, a_mn, b, ldb, b_mn, c.dtype, m, n, k, ptr(bias), ptr(residual), act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
-                      out.data_ptr(), ptr(ws), bytes, c.stream),
+                      out.data_ptr(), c.stream),
      "tab_dense_matmul");
 }
 
@@ -363,11 +360,8 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     const Mat w2 = matrix_of(c, weight2, inner8, h8);
     dz.t = c.empty({m, 2 * inner8});
     hidden.t = c.empty({m, inner8});
-    size_t bytes = 0;
-    ok(tab_dense_matmul_workspace_bytes(m, inner8, h8, &bytes), "tab_dense_matmul_workspace_bytes");
-    const Tensor ws = bytes ? c.workspace(bytes) : Tensor();
     ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h8, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
-                             dz.t.data_ptr(), hidden.t.data_ptr(), ptr(ws), bytes, c.stream),
+                             dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
   }
   if (want[2]) dw2 = cut(c, weight_grad(c, hidden, dy, inner8, h8, weight2), inner, h);
