@@ -123,11 +123,13 @@ static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int 
   return check_launch(op);
 }
 
-// Pairs that share a tile's contraction when `tiles` tiles are all there is to do.  A cluster of 2 s CTAs needs 2 s free SMs in one
-// GPC: of the 148 SMs 72 fit into clusters of 8 or 4 alike.
+// Pairs that share a tile's contraction when `tiles` tiles are all there is to do.  The GPCs of a B200 hold 33 clusters of 4 such
+// CTAs or 15 of 8 at a time; one more costs a second turn (16 tiles of K = 7168: 26.1 us with two pairs, 38.7 with four).  Joining
+// the parts takes the time of some 20 blocks of the contraction with two pairs and 35 with four: one tile of K = 1024 takes
+// 11.0 / 11.3 / 13.0 us with 1 / 2 / 4 pairs, K = 4096 24.4 / 18.1 / 15.8.
 static int pair_split(int64_t tiles, int num_kb) {
-  for (int s = 4; s > 1; s /= 2)
-    if (tiles * s <= 72 && num_kb >= 4 * s) return s;
+  if (tiles <= 15 && num_kb >= 48) return 4;
+  if (tiles <= 33 && num_kb >= 24) return 2;
   return 1;
 }
 
@@ -196,9 +198,13 @@ static int launch_narrow_epi(const char* op, int dtype, const DenseOperand& x, c
   p.nt = 16;
   while (p.nt < p.M) p.nt *= 2;
   const int tiles = EPI == kEpiGlu ? (p.N + 63) / 64 : (p.N + 127) / 128;
-  // two CTAs per SM as long as each keeps a few blocks of the contraction
-  p.split = 1;
-  while (p.split < kNwMaxSplit && tiles * p.split * 2 <= 2 * dense_sms() && p.split * 2 * 4 <= p.num_kb) p.split *= 2;
+  // CTAs per tile: as many as fill the SMs, two of them on some.  Measured over weights that come from HBM (us): one row, 56 tiles
+  // of K = 2048: 10.4 / 9.3 / 9.7 / 11.4 with 2 / 3 / 4 / 5 CTAs; 32 tiles of K = 7168: 15.6 / 14.8 / 14.4 / 14.2 with 3 / 4 / 5 / 6;
+  // from 64 rows on the parts to exchange weigh more: 128 rows, 56 tiles: 15.7 / 17.2 with 2 / 3; 32 tiles: 21.2 / 24.0 with 4 / 5.
+  p.split = (p.nt <= 32 ? 176 : 132) / tiles;
+  if (p.split > kNwMaxSplit) p.split = kNwMaxSplit;
+  if (p.split > p.num_kb / 2) p.split = p.num_kb / 2;
+  if (p.split < 1) p.split = 1;
   p.stages = (kNwSmemTarget - 1024 - kNwCtrlBytes) / dense_narrow_stage_bytes(p.nt);
   if (p.stages > kNwMaxStages) p.stages = kNwMaxStages;
   p.a_mn = w.mn;
