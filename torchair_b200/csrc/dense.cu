@@ -145,20 +145,20 @@ static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMa
   const int64_t whole = tiles - rest;
   int rc = TAB_OK;
   if (whole > 0) {
-    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, false>, kDpSmemBytes, done)) != TAB_OK) return rc;
+    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, false>, kDpSmemBytes<EPI>, done)) != TAB_OK) return rc;
     p.tile_begin = 0;
     p.tile_end = (int)whole;
     p.split = 1;
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes, 2, false, ma, mb, p, st);
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes<EPI>, 2, false, ma, mb, p, st);
     if (rc != TAB_OK) return rc;
   }
   if (rest > 0) {
-    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, true>, kDpSmemBytes, done_split)) != TAB_OK) return rc;
+    if ((rc = allow_smem(op, dense_pair_kernel<T, EPI, true>, kDpSmemBytes<EPI>, done_split)) != TAB_OK) return rc;
     p.tile_begin = (int)whole;
     p.tile_end = (int)tiles;
     p.split = split;
     // both launches read the same operands and write different tiles: the second may fill SMs that the first has left
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes, 2 * split, whole > 0, ma, mb, p, st);
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes<EPI>, 2 * split, whole > 0, ma, mb, p, st);
   }
   return rc;
 }

@@ -32,17 +32,21 @@
 namespace tab {
 
 constexpr int kDpStageBytes = 2 * kDnOperandBytes;     // 16 KB of A + 16 KB of B per CTA
-constexpr int kDpStages = 6;
+// The epilogue of kEpiGluGrad stages three streams of values instead of two, at the price of one stage of the ring.
+template <int EPI>
+constexpr int kDpStages = EPI == kEpiGluGrad ? 5 : 6;
 constexpr int kDpBufs = 2;
 constexpr int kDpCols = 256;
-constexpr int kDpEpiWarps = 8;                         // two per TMEM lane quarter, each takes half of the columns
+constexpr int kDpEpiWarps = 16;                        // four per TMEM lane quarter, each takes a quarter of the columns
 constexpr int kDpThreads = 64 + kDpEpiWarps * 32;
 constexpr int kDpCtrlBytes = 256;
-constexpr int kDpPitch = 80;                           // staged row: 32 16-bit values + 16 bytes of padding
-constexpr int kDpPatchBytes = 32 * kDpPitch;           // one epilogue warp's 32 rows
-constexpr int kDpSmemBytes = 1024 + kDpStages * kDpStageBytes + kDpCtrlBytes + kDpEpiWarps * kDpPatchBytes;
-static_assert(kDpSmemBytes <= kDnSmemLimit, "dense pair GEMM shared memory");
-static_assert(128 * kDpCols * 4 <= kDpStages * kDpStageBytes, "a CTA's accumulators fit into its ring");
+constexpr int kDpPatch = 1024;                         // staging area of an epilogue warp: 32 rows x 16 16-bit values
+template <int EPI>
+constexpr int kDpPatches = EPI == kEpiGluGrad ? 3 : 2;
+template <int EPI>
+constexpr int kDpSmemBytes = 1024 + kDpStages<EPI> * kDpStageBytes + kDpCtrlBytes + kDpEpiWarps * kDpPatches<EPI> * kDpPatch;
+static_assert(kDpSmemBytes<kEpiLinear> <= kDnSmemLimit && kDpSmemBytes<kEpiGluGrad> <= kDnSmemLimit, "dense pair GEMM shared memory");
+static_assert(128 * kDpCols * 4 <= 5 * kDpStageBytes, "a CTA's accumulators fit into its ring");
 
 // Tiles are numbered so that the tiles in flight share operands: column by column inside bands of kDpBand row tiles.
 constexpr int kDpBand = 8;
@@ -55,110 +59,122 @@ __device__ __forceinline__ void dense_tile_coord(int t, int row_tiles, int col_t
   rt = band * kDpBand + (in - ct * h);
 }
 
-__device__ __forceinline__ void dense_epi_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kDpEpiWarps * 32) : "memory"); }
+// ---- epilogue ------------------------------------------------------------------------------------------------------------
+// Sixteen warps, four to a scheduler: a step (16 accumulator columns of a row per thread: read, bias, activation, pack, store) is
+// a chain of latencies, and with half the warps a tile's plain epilogue took 6400 cycles, its silu 11300, against 8300 for the
+// main loop at K = 1024.  16-bit values pass between registers and row-major memory through patches of 32 rows x 16 columns, so
+// that global accesses are 16 bytes per lane, two lanes to a row's 32-byte sector.  Rows >= M and columns >= N are left alone
+// (loads give zeros); N is a multiple of 8, no 16-byte piece is ever cut.
+__device__ __forceinline__ uint32_t patch_at(int row, int piece) { return static_cast<uint32_t>(row * 32 + ((piece ^ ((row >> 2) & 1)) << 4)); }
 
-// ---- moving 32 rows x 32 columns of 16-bit values between registers (thread = row) and row-major memory, through the warp's
-// patch: global accesses are 16 bytes per lane, four lanes to a row's 64 bytes.  Rows >= rows_end and columns >= cols are left
-// alone (loads give zeros); cols and col are multiples of 8, so a 16-byte piece is never cut.
 template <typename T>
-__device__ __forceinline__ void store_rows32(uint8_t* patch, int lane, const float (&v)[32], T* base, int64_t ld, int row_base, int rows_end,
-                                             int col, int cols) {
-  uint4* prow = reinterpret_cast<uint4*>(patch + lane * kDpPitch);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    prow[k] = make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]), pack2<T>(v[8 * k + 4], v[8 * k + 5]),
-                         pack2<T>(v[8 * k + 6], v[8 * k + 7]));
-  __syncwarp();
-  const int c = col + (lane & 3) * 8;
-  if (c < cols) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2);
-      if (row_base + r < rows_end)
-        *reinterpret_cast<uint4*>(base + static_cast<int64_t>(row_base + r) * ld + c) =
-            *reinterpret_cast<const uint4*>(patch + r * kDpPitch + (lane & 3) * 16);
-    }
-  }
-  __syncwarp();
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
-
 template <typename T>
-__device__ __forceinline__ void load_rows32(uint8_t* patch, int lane, uint32_t (&v)[16], const T* base, int64_t ld, int row_base, int rows_end,
-                                            int col, int cols) {
-  const int c = col + (lane & 3) * 8;
+__device__ __forceinline__ void unpack8(const uint4& x, float* v) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (c < cols && row_base + r < rows_end) x = __ldg(reinterpret_cast<const uint4*>(base + static_cast<int64_t>(row_base + r) * ld + c));
-    *reinterpret_cast<uint4*>(patch + r * kDpPitch + (lane & 3) * 16) = x;
+    const float2 f = unpack2<T>(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
   }
-  __syncwarp();
-  const uint4* prow = reinterpret_cast<const uint4*>(patch + lane * kDpPitch);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint4 x = prow[k];
-    v[4 * k] = x.x;
-    v[4 * k + 1] = x.y;
-    v[4 * k + 2] = x.z;
-    v[4 * k + 3] = x.w;
-  }
-  __syncwarp();
 }
 
-// v[0..31] += bias[col .. col + 31] (columns beyond cols hold nothing that is stored)
 template <typename T>
-__device__ __forceinline__ void add_bias32(float (&v)[32], const void* bias, int col, int cols) {
-  if (bias == nullptr) return;
+__device__ __forceinline__ void patch_put(uint8_t* patch, int lane, const float (&v)[16]) {
+  *reinterpret_cast<uint4*>(patch + patch_at(lane, 0)) = pack8<T>(v);
+  *reinterpret_cast<uint4*>(patch + patch_at(lane, 1)) = pack8<T>(v + 8);
+}
+template <typename T>
+__device__ __forceinline__ void patch_get(const uint8_t* patch, int lane, float (&v)[16]) {
+  unpack8<T>(*reinterpret_cast<const uint4*>(patch + patch_at(lane, 0)), v);
+  unpack8<T>(*reinterpret_cast<const uint4*>(patch + patch_at(lane, 1)), v + 8);
+}
+
+// patch -> memory; the warp has met since the patch was written and meets again before it is written anew
+template <typename T>
+__device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, T* base, int64_t ld, int row_base, int rows_end, int col, int cols) {
+  const int c = col + (lane & 1) * 8;
+  if (c < cols) {
+    T* dst = base + static_cast<int64_t>(row_base + (lane >> 1)) * ld + c;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (col + 8 * k < cols) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + col + 8 * k));
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(w[i]);
-        v[8 * k + 2 * i] += f.x;
-        v[8 * k + 2 * i + 1] += f.y;
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int r = i * 16 + (lane >> 1);
+      if (row_base + r < rows_end) *reinterpret_cast<uint4*>(dst + i * 16 * ld) = *reinterpret_cast<const uint4*>(patch + patch_at(r, lane & 1));
     }
   }
 }
 
-// largest magnitude of a chunk as bits (NaN > infinity > every finite value); columns beyond cols do not count
-__device__ __forceinline__ uint32_t chunk_amax_bits(const float (&v)[32], int col, int cols) {
+// memory -> registers, as the patch will be filled from them
+struct Ahead {
+  uint4 x[2];
+  template <typename T>
+  __device__ __forceinline__ void load(int lane, const T* base, int64_t ld, int row_base, int rows_end, int col, int cols) {
+    const int c = col + (lane & 1) * 8;
+    const T* src = base + static_cast<int64_t>(row_base + (lane >> 1)) * ld + c;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < cols && row_base + i * 16 + (lane >> 1) < rows_end) x[i] = __ldg(reinterpret_cast<const uint4*>(src + i * 16 * ld));
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* patch, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(patch + patch_at(i * 16 + (lane >> 1), lane & 1)) = x[i];
+  }
+};
+
+// v[0..15] += bias[col .. col + 15]; the loads are asked for before the accumulators (columns beyond cols are not stored)
+template <typename T>
+struct Bias16 {
+  uint4 x[2];
+  __device__ __forceinline__ void load(const void* bias, int col, int cols) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      x[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (bias != nullptr && col + 8 * k < cols) x[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + col + 8 * k));
+    }
+  }
+  __device__ __forceinline__ void add(float (&v)[16]) const {
+    float b[16];
+    unpack8<T>(x[0], b);
+    unpack8<T>(x[1], b + 8);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += b[i];
+  }
+};
+
+// largest magnitude as bits (NaN > infinity > every finite value); columns beyond cols do not count
+__device__ __forceinline__ uint32_t amax_bits16(const float (&v)[16], int col, int cols) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
+  for (int j = 0; j < 16; ++j)
     if (col + (j & ~7) < cols) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
   return m;
 }
 
-// 32 values of this thread's row -> 32 int8 at q (16-byte aligned); columns beyond cols become 0
-__device__ __forceinline__ void store_q32(const float (&v)[32], const RowQuant& rq, int8_t* q, int col, int cols) {
-  uint32_t w[8];
+// 16 values of this thread's row -> 16 int8 at q (16-byte aligned); columns beyond cols become 0
+__device__ __forceinline__ void store_q16(const float (&v)[16], const RowQuant& rq, int8_t* q, int col, int cols) {
+  uint2 o[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    uint2 o = make_uint2(0u, 0u);
+  for (int k = 0; k < 2; ++k) {
+    o[k] = make_uint2(0u, 0u);
     if (col + 8 * k < cols) {
       float t[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = v[8 * k + i];
-      o = quant8(t, rq);
+      o[k] = quant8(t, rq);
     }
-    w[2 * k] = o.x;
-    w[2 * k + 1] = o.y;
   }
-  *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
-  *reinterpret_cast<uint4*>(q + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+  *reinterpret_cast<uint4*>(q) = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
 }
 
-// 32 kept int8 of this thread's row as fp32
-__device__ __forceinline__ void load_q32(float (&v)[32], const int8_t* q, float scale) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(q)), b = __ldg(reinterpret_cast<const uint4*>(q + 16));
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+__device__ __forceinline__ void unpack_q16(const uint4& a, float scale, float (&v)[16]) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[4 * k + i] = static_cast<float>(static_cast<int8_t>(w[k] >> (8 * i))) * scale;
 }
@@ -169,10 +185,12 @@ struct DenseAcc {
   uint32_t taddr;          // this warp's lanes, first column of the buffer
   uint32_t part;           // 0, or the shared-memory address of this thread's row in the parts: float4 [column / 4][128 rows]
   int split, parity;       // pairs of the cluster, which CTA of its pair this is
-  __device__ __forceinline__ void fetch(int c, float (&v)[32]) const {
+  uint32_t release_bar;    // the leader's barrier that counts this buffer's readers (0: nothing to release)
+
+  __device__ __forceinline__ void fetch(int c, float (&v)[16]) const {
     __syncwarp();
     if (part == 0) {
-      ptx::tmem_ld32f(taddr + c, v);
+      ptx::tmem_ld16f(taddr + c, v);
       ptx::tmem_ld_wait();
       return;
     }
@@ -180,159 +198,220 @@ struct DenseAcc {
 #pragma unroll 1
     for (int s = 0; s < split; ++s) {
       const uint32_t from = ptx::mapa(at, static_cast<uint32_t>(2 * s + parity));
-      float4 t[8];
+      float4 t[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t[k] = ptx::ld_cluster_f4(from + k * 2048u);
+      for (int k = 0; k < 4; ++k) t[k] = ptx::ld_cluster_f4(from + k * 2048u);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const float x[4] = {t[k].x, t[k].y, t[k].z, t[k].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[4 * k + j] = s == 0 ? x[j] : v[4 * k + j] + x[j];
       }
     }
   }
+  // this warp has read all it needs: the next tile's MMAs may overwrite the buffer while its results are still being stored
+  __device__ __forceinline__ void release(int lane) {
+    if (release_bar == 0) return;
+    ptx::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive_cluster_relaxed(release_bar);
+    release_bar = 0;
+  }
 };
 
-// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 32; of 64
-// where 8-bit blocks are written).
+// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 16; of 64
+// where 8-bit blocks are written).  What it reads from global memory (residual, kept values) is asked for before the
+// accumulators are waited for, then one step ahead.
 template <typename T, int EPI>
-__device__ __forceinline__ void dense_epilogue(const DenseParams& p, const DenseAcc& acc, uint8_t* patch, int lane, int row_base, int ct,
-                                               int col_begin, int col_end) {
-  const int row = row_base + lane;
-  const bool rvalid = row < p.M;
-  if constexpr (EPI == kEpiLinear) {
+struct TileEpilogue {
+  const DenseParams& p;
+  uint8_t* patch;
+  int lane, row_base, ct, col_begin, col_end;
+  bool rvalid;
+  Ahead r0, r1;            // residual (kEpiLinear); kept gate and up (kEpiGluGrad)
+
+  __device__ __forceinline__ TileEpilogue(const DenseParams& p_, uint8_t* patch_, int lane_, int row_base_, int ct_, int begin, int end)
+      : p(p_), patch(patch_), lane(lane_), row_base(row_base_), ct(ct_), col_begin(begin), col_end(end), rvalid(row_base_ + lane_ < p_.M) {}
+
+  __device__ __forceinline__ void look_ahead(int c) {
+    const int col = ct * 256 + c;
+    if constexpr (EPI == kEpiLinear) {
+      if (p.residual != nullptr) r0.load(lane, static_cast<const T*>(p.residual), p.N, row_base, p.M, col, p.N);
+    }
+    if constexpr (EPI == kEpiGluGrad) {
+      if (p.keep_q == nullptr) {
+        r0.load(lane, static_cast<const T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
+        r1.load(lane, static_cast<const T*>(p.keep) + p.keep_up, p.keep_ld, row_base, p.M, col, p.N);
+      }
+    }
+  }
+
+  // before the wait for the accumulators
+  __device__ __forceinline__ void prefetch() {
+    if (row_base < p.M && col_begin < col_end) look_ahead(col_begin);
+  }
+
+  __device__ __forceinline__ void run(DenseAcc& acc) {
+    if (row_base < p.M && col_begin < col_end) {
+      if constexpr (EPI == kEpiLinear) linear(acc);
+      if constexpr (EPI == kEpiGlu) glu(acc);
+      if constexpr (EPI == kEpiGluGrad) glu_grad(acc);
+    }
+    acc.release(lane);
+  }
+
+  // the quantiser of 64 columns from accumulator column `at` on, whose output columns begin at col
+  __device__ __forceinline__ RowQuant block_quant(const DenseAcc& acc, const void* bias, int at, int col, float* scale) const {
+    uint32_t m = 0;
+#pragma unroll 1
+    for (int h = 0; h < 64; h += 16) {
+      float v[16];
+      Bias16<T> b;
+      b.load(bias, col + h, p.N);
+      acc.fetch(at + h, v);
+      b.add(v);
+      m = max(m, amax_bits16(v, col + h, p.N));
+    }
+    const RowQuant rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
+    if (rvalid) *scale = rq.scale;
+    return rq;
+  }
+
+  __device__ __forceinline__ void linear(DenseAcc& acc) {
+    const int64_t row = row_base + lane;
+    const bool has_bias = p.bias != nullptr, has_res = p.residual != nullptr, keep8 = p.keep_q != nullptr, keep16 = !keep8 && p.keep != nullptr;
+    const int act = p.act;
+    uint8_t *main_patch = patch, *side_patch = patch + kDpPatch;
     RowQuant rq;
 #pragma unroll 1
-    for (int c = col_begin; c < col_end; c += 32) {
+    for (int c = col_begin; c < col_end; c += 16) {
       const int col = ct * 256 + c;
-      if (col >= p.N && (p.keep_q == nullptr || (col & ~63) >= p.N)) break;
-      if (p.keep_q != nullptr && (c & 63) == 0) {                        // amax of the 64-value block first
-        uint32_t m = 0;
-#pragma unroll 1
-        for (int h = 0; h < 64; h += 32) {
-          float v[32];
-          acc.fetch(c + h, v);
-          add_bias32<T>(v, p.bias, col + h, p.N);
-          m = max(m, chunk_amax_bits(v, col + h, p.N));
-        }
-        rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
-        if (rvalid) p.keep_scale[static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col / kKeepBlock] = rq.scale;
+      if (col >= p.N && (!keep8 || (col & ~63) >= p.N)) break;
+      if (keep8 && (c & 63) == 0) rq = block_quant(acc, p.bias, c, col, p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock);
+      float v[16];
+      Bias16<T> b;
+      if (has_bias) b.load(p.bias, col, p.N);
+      if (has_res) r0.put(main_patch, lane);
+      acc.fetch(c, v);                                   // (the warp meets in there)
+      if (c + 16 >= col_end) acc.release(lane);
+      if (has_bias) b.add(v);
+      if (keep8) {
+        if (rvalid) store_q16(v, rq, p.keep_q + row * p.keep_ld + col, col, p.N);
+      } else if (keep16) {
+        patch_put<T>(side_patch, lane, v);
       }
-      float v[32];
-      acc.fetch(c, v);
-      add_bias32<T>(v, p.bias, col, p.N);
-      if (p.keep_q != nullptr) {
-        if (rvalid) store_q32(v, rq, p.keep_q + static_cast<int64_t>(row) * p.keep_ld + col, col, p.N);
-      } else if (p.keep != nullptr) {
-        store_rows32<T>(patch, lane, v, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
-      }
-      if (col >= p.N) continue;
-      if (p.act != TAB_ACT_NONE)
-        with_act(p.act, [&](auto tag) {
+      if (act != TAB_ACT_NONE)
+        with_act(act, [&](auto tag) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
+          for (int j = 0; j < 16; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
         });
-      if (p.residual != nullptr) {
-        uint32_t r[16];
-        load_rows32<T>(patch, lane, r, static_cast<const T*>(p.residual), p.N, row_base, p.M, col, p.N);
+      if (has_res) {
+        float r[16];
+        patch_get<T>(main_patch, lane, r);
+        if (c + 16 < col_end) look_ahead(c + 16);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = unpack2<T>(r[j]);
-          v[2 * j] += f.x;
-          v[2 * j + 1] += f.y;
-        }
+        for (int j = 0; j < 16; ++j) v[j] += r[j];
       }
-      store_rows32<T>(patch, lane, v, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      patch_put<T>(main_patch, lane, v);
+      __syncwarp();
+      if (keep16) patch_store<T>(side_patch, lane, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
+      patch_store<T>(main_patch, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      __syncwarp();
     }
-  } else if constexpr (EPI == kEpiGlu) {
+  }
+
+  __device__ __forceinline__ void glu(DenseAcc& acc) {
     // output column c of the tile: its gate is accumulator column (c / 64) * 128 + c % 64, its up value 64 columns further
-    const T* bias_up = p.bias ? static_cast<const T*>(p.bias) + p.N : nullptr;
+    const int64_t row = row_base + lane;
+    const bool has_bias = p.bias != nullptr, keep8 = p.keep_q != nullptr, keep16 = !keep8 && p.keep != nullptr;
+    const T* bias_up = static_cast<const T*>(p.bias) + p.N;
+    uint8_t *pg = patch, *pu = patch + kDpPatch;
     RowQuant rg, ru;
 #pragma unroll 1
-    for (int c = col_begin; c < col_end; c += 32) {
+    for (int c = col_begin; c < col_end; c += 16) {
       const int col = ct * 128 + c;
-      if (col >= p.N && (p.keep_q == nullptr || (col & ~63) >= p.N)) break;
+      if (col >= p.N && (!keep8 || (col & ~63) >= p.N)) break;
       const int at = (c >> 6) * 128 + (c & 63);
-      if (p.keep_q != nullptr && (c & 63) == 0) {
-        uint32_t mg = 0, mu = 0;
-#pragma unroll 1
-        for (int h = 0; h < 64; h += 32) {
-          float v[32];
-          acc.fetch(at + h, v);
-          add_bias32<T>(v, p.bias, col + h, p.N);
-          mg = max(mg, chunk_amax_bits(v, col + h, p.N));
-          acc.fetch(at + 64 + h, v);
-          add_bias32<T>(v, bias_up, col + h, p.N);
-          mu = max(mu, chunk_amax_bits(v, col + h, p.N));
-        }
-        rg = make_block_quant(__uint_as_float(mg), mg < 0x7f800000u);
-        ru = make_block_quant(__uint_as_float(mu), mu < 0x7f800000u);
-        if (rvalid) {
-          float* s = p.keep_scale + static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
-          s[0] = rg.scale;
-          s[p.keep_up / kKeepBlock] = ru.scale;
-        }
+      if (keep8 && (c & 63) == 0) {
+        float* scale = p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
+        rg = block_quant(acc, p.bias, at, col, scale);
+        ru = block_quant(acc, has_bias ? bias_up : nullptr, at + 64, col, scale + p.keep_up / kKeepBlock);
       }
-      float g[32], u[32];
+      float g[16], u[16];
+      Bias16<T> bg, bu;
+      if (has_bias) {
+        bg.load(p.bias, col, p.N);
+        bu.load(bias_up, col, p.N);
+      }
       acc.fetch(at, g);
       acc.fetch(at + 64, u);
-      add_bias32<T>(g, p.bias, col, p.N);
-      add_bias32<T>(u, bias_up, col, p.N);
-      if (p.keep_q != nullptr) {
-        if (rvalid) {
-          int8_t* q = p.keep_q + static_cast<int64_t>(row) * p.keep_ld + col;
-          store_q32(g, rg, q, col, p.N);
-          store_q32(u, ru, q + p.keep_up, col, p.N);
-        }
-      } else if (p.keep != nullptr) {
-        store_rows32<T>(patch, lane, g, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
-        store_rows32<T>(patch, lane, u, static_cast<T*>(p.keep) + p.keep_up, p.keep_ld, row_base, p.M, col, p.N);
+      if (c + 16 >= col_end) acc.release(lane);
+      if (has_bias) {
+        bg.add(g);
+        bu.add(u);
       }
-      if (col >= p.N) continue;
+      if (keep8) {
+        if (rvalid) {
+          int8_t* q = p.keep_q + row * p.keep_ld + col;
+          store_q16(g, rg, q, col, p.N);
+          store_q16(u, ru, q + p.keep_up, col, p.N);
+        }
+      } else if (keep16) {
+        patch_put<T>(pg, lane, g);
+        patch_put<T>(pu, lane, u);
+        __syncwarp();
+        patch_store<T>(pg, lane, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
+        patch_store<T>(pu, lane, static_cast<T*>(p.keep) + p.keep_up, p.keep_ld, row_base, p.M, col, p.N);
+        __syncwarp();
+      }
       with_act(p.act, [&](auto tag) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) g[j] = act_value<decltype(tag)::value>(g[j]) * u[j];
+        for (int j = 0; j < 16; ++j) g[j] = act_value<decltype(tag)::value>(g[j]) * u[j];
       });
-      store_rows32<T>(patch, lane, g, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      patch_put<T>(pg, lane, g);
+      __syncwarp();
+      patch_store<T>(pg, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      __syncwarp();
     }
-  } else {
+  }
+
+  __device__ __forceinline__ void glu_grad(DenseAcc& acc) {
+    const int64_t row = row_base + lane;
+    const int64_t ld2 = 2 * static_cast<int64_t>(p.N);
+    const bool keep8 = p.keep_q != nullptr;
+    uint8_t *pg = patch, *pu = patch + kDpPatch, *ph = patch + 2 * kDpPatch;
 #pragma unroll 1
-    for (int c = col_begin; c < col_end; c += 32) {
+    for (int c = col_begin; c < col_end; c += 16) {
       const int col = ct * 256 + c;
       if (col >= p.N) break;
-      float g[32], u[32], dh[32];
-      if (p.keep_q != nullptr) {
+      float g[16], u[16], dh[16];
+      if (keep8) {
+        uint4 qg = make_uint4(0u, 0u, 0u, 0u), qu = qg;
+        float sg = 0.f, su = 0.f;
         if (rvalid) {
-          const int8_t* q = p.keep_q + static_cast<int64_t>(row) * p.keep_ld + col;
-          const float* s = p.keep_scale + static_cast<int64_t>(row) * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
-          load_q32(g, q, __ldg(s));
-          load_q32(u, q + p.keep_up, __ldg(s + p.keep_up / kKeepBlock));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = u[j] = 0.f;
+          const int8_t* q = p.keep_q + row * p.keep_ld + col;
+          const float* s = p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
+          qg = __ldg(reinterpret_cast<const uint4*>(q));
+          qu = __ldg(reinterpret_cast<const uint4*>(q + p.keep_up));
+          sg = __ldg(s);
+          su = __ldg(s + p.keep_up / kKeepBlock);
         }
+        unpack_q16(qg, sg, g);
+        unpack_q16(qu, su, u);
+        acc.fetch(c, dh);
       } else {
-        uint32_t r[16];
-        load_rows32<T>(patch, lane, r, static_cast<const T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = unpack2<T>(r[j]);
-          g[2 * j] = f.x;
-          g[2 * j + 1] = f.y;
-        }
-        load_rows32<T>(patch, lane, r, static_cast<const T*>(p.keep) + p.keep_up, p.keep_ld, row_base, p.M, col, p.N);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = unpack2<T>(r[j]);
-          u[2 * j] = f.x;
-          u[2 * j + 1] = f.y;
-        }
+        r0.put(pg, lane);
+        r1.put(pu, lane);
+        acc.fetch(c, dh);                                // (the warp meets in there)
+        patch_get<T>(pg, lane, g);
+        patch_get<T>(pu, lane, u);
+        if (c + 16 < col_end) look_ahead(c + 16);
       }
-      acc.fetch(c, dh);
+      if (c + 16 >= col_end) acc.release(lane);
       // h = a u, d(gate) = dh u a', d(up) = dh a; g, u and dh are overwritten in turn
       with_act(p.act, [&](auto tag) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < 16; ++j) {
           float a, d;
           act_both<decltype(tag)::value>(g[j], a, d);
           const float h = a * u[j];
@@ -341,36 +420,54 @@ __device__ __forceinline__ void dense_epilogue(const DenseParams& p, const Dense
           dh[j] = h;
         }
       });
-      store_rows32<T>(patch, lane, g, static_cast<T*>(p.dgate), 2 * static_cast<int64_t>(p.N), row_base, p.M, col, p.N);
-      store_rows32<T>(patch, lane, u, static_cast<T*>(p.dgate) + p.N, 2 * static_cast<int64_t>(p.N), row_base, p.M, col, p.N);
-      store_rows32<T>(patch, lane, dh, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      patch_put<T>(pg, lane, g);
+      patch_put<T>(pu, lane, u);
+      patch_put<T>(ph, lane, dh);
+      __syncwarp();
+      patch_store<T>(pg, lane, static_cast<T*>(p.dgate), ld2, row_base, p.M, col, p.N);
+      patch_store<T>(pu, lane, static_cast<T*>(p.dgate) + p.N, ld2, row_base, p.M, col, p.N);
+      patch_store<T>(ph, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      __syncwarp();
     }
   }
-}
+};
 
 // Output columns of a tile: 256, or 128 where gate and up share the accumulator.
 template <int EPI>
 constexpr int kDpTileCols = EPI == kEpiGlu ? 128 : 256;
 
+// Columns that stay with one warp: 16, or a whole 8-bit block.
+template <int EPI>
+__device__ __forceinline__ int dense_column_unit(const DenseParams& p) {
+  return p.keep_q != nullptr && EPI != kEpiGluGrad ? kKeepBlock : 16;
+}
+// The part of columns [from, to) that warp `share` of the four warps of a lane quarter takes.
+template <int EPI>
+__device__ __forceinline__ void dense_columns(const DenseParams& p, int from, int to, int share, int& begin, int& end) {
+  const int each = max((to - from) / 4, dense_column_unit<EPI>(p));
+  begin = min(from + share * each, to);
+  end = min(begin + each, to);
+}
+
 template <typename T, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(kDpThreads, 1)
 dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const DenseParams p) {
+  constexpr int kStages = kDpStages<EPI>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t tiles_addr = ptx::smem_u32(smem);
-  uint8_t* ctrl = smem + kDpStages * kDpStageBytes;
+  uint8_t* ctrl = smem + kStages * kDpStageBytes;
   const uint32_t bar0 = ptx::smem_u32(ctrl);
   auto bar_full = [&](int s) { return bar0 + 8u * s; };
-  auto bar_empty = [&](int s) { return bar0 + 8u * (kDpStages + s); };
-  auto bar_tfull = [&](int b) { return bar0 + 8u * (2 * kDpStages + b); };
-  auto bar_tempty = [&](int b) { return bar0 + 8u * (2 * kDpStages + kDpBufs + b); };
-  const uint32_t bar_drain = bar0 + 8u * (2 * kDpStages + 2 * kDpBufs);
+  auto bar_empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto bar_tfull = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
+  auto bar_tempty = [&](int b) { return bar0 + 8u * (2 * kStages + kDpBufs + b); };
+  const uint32_t bar_drain = bar0 + 8u * (2 * kStages + 2 * kDpBufs);
   const uint32_t bar_done = bar_drain + 8u;            // the peer no longer touches this CTA's shared state
-  static_assert(8 * (2 * kDpStages + 2 * kDpBufs + 2) <= 224, "barriers overflow the control block");
+  static_assert(8 * (2 * kStages + 2 * kDpBufs + 2) <= 224, "barriers overflow the control block");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(ctrl + 224);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  volatile int* s_got = reinterpret_cast<volatile int*>(s_tmem + 2);     // [2] outcome of the epilogue's wait, per buffer
   uint8_t* s_out = ctrl + kDpCtrlBytes;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -386,7 +483,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const int kb_end = SPLIT ? static_cast<int>(static_cast<int64_t>(part + 1) * p.num_kb / split) : p.num_kb;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kDpStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       ptx::mbar_init(bar_full(s), 1);                      // armed by the leader's producer for the bytes of both CTAs
       ptx::mbar_init(bar_empty(s), 1);
     }
@@ -437,7 +534,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           ptx::tma_load_2d_pair(sb + kDnBoxBytes, &tm_b, full_leader, p.b_mn ? b1 : k, p.b_mn ? k : b1);
         }
         __syncwarp();
-        if (++stage == kDpStages) { stage = 0; phase ^= 1u; }
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
     }
   } else if (warp == 1) {
@@ -468,7 +565,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             ptx::mma_commit_mask(bar_empty(stage), both);
           }
           __syncwarp();
-          if (++stage == kDpStages) { stage = 0; phase ^= 1u; }
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
         if (ptx::elect_one()) ptx::mma_commit_mask(bar_tfull(buf), both);
@@ -484,38 +581,38 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   } else {
     // ---------------- epilogue: warps 2..9, thread = row, two warps share the columns of a row ----------------
     const int quarter = warp & 3;
-    const int half = (warp - 2) >> 2;
-    const int et = threadIdx.x - 64;
+    const int share = (warp - 2) >> 2;
     int buf = 0;
     uint32_t tphase = 0;
     DenseAcc acc;
     acc.part = 0;
     for (int tile = first; tile < p.tile_end; tile += step) {
-      if (et == 0) s_got[buf] = dense_wait(bar_tfull(buf), tphase, s_abort, 34, p.wait_cycles) ? 1 : 0;
-      dense_epi_bar();
-      if (!s_got[buf]) break;
-      ptx::tc_fence_after();
       acc.taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * kDpCols;
+      acc.release_bar = ptx::mapa(bar_tempty(buf), leader_cta);          // the leader counts both CTAs' warps
       if constexpr (SPLIT) {
+        if (!__all_sync(0xffffffffu, dense_wait(bar_tfull(buf), tphase, s_abort, 34, p.wait_cycles))) break;
+        ptx::tc_fence_after();
         // all MMAs of this pair are done, so its ring is free: it takes the 128 x 256 accumulators
         const uint32_t dst = tiles_addr + static_cast<uint32_t>(quarter * 32 + lane) * 16u;
 #pragma unroll 1
-        for (int c = half * 128; c < half * 128 + 128; c += 32) {
-          float v[32];
+        for (int c = share * 64; c < share * 64 + 64; c += 16) {
+          float v[16];
           acc.fetch(c, v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) ptx::st_shared_f4(dst + static_cast<uint32_t>((c >> 2) + k) * 2048u, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+          for (int k = 0; k < 4; ++k) ptx::st_shared_f4(dst + static_cast<uint32_t>((c >> 2) + k) * 2048u, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
         }
+        acc.release(lane);
       } else {
         int rt, ct;
         dense_tile_coord(tile, p.row_tiles, p.col_tiles, rt, ct);
-        const int row_base = rt * 256 + rank * 128 + quarter * 32;
-        constexpr int kHalf = kDpTileCols<EPI> / 2;
-        if (row_base < p.M) dense_epilogue<T, EPI>(p, acc, s_out + (warp - 2) * kDpPatchBytes, lane, row_base, ct, half * kHalf, half * kHalf + kHalf);
+        int begin, end;
+        dense_columns<EPI>(p, 0, kDpTileCols<EPI>, share, begin, end);
+        TileEpilogue<T, EPI> epi(p, s_out + (warp - 2) * kDpPatches<EPI> * kDpPatch, lane, rt * 256 + rank * 128 + quarter * 32, ct, begin, end);
+        epi.prefetch();
+        if (!__all_sync(0xffffffffu, dense_wait(bar_tfull(buf), tphase, s_abort, 34, p.wait_cycles))) break;
+        ptx::tc_fence_after();
+        epi.run(acc);
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(bar_tempty(buf), leader_cta));   // the leader counts both CTAs' warps
       if (++buf == kDpBufs) { buf = 0; tphase ^= 1u; }
     }
   }
@@ -525,23 +622,22 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   if constexpr (SPLIT) {
     ptx::cluster_sync_all();          // every pair's part is in place
     if (warp >= 2) {
-      // this pair's share of the tile's columns, halved again between the two warps of a row; 64-value blocks are not cut, so
-      // with four pairs some hold no share (which pairs share a tile must not depend on what is kept: the sums would differ)
-      int rt, ct;
+      // this pair's columns of the tile; 64-value blocks are not cut, so with four pairs some hold none (which pairs share a
+      // tile must not depend on what is kept: the sums would differ)
+      int rt, ct, begin, end;
       dense_tile_coord(first, p.row_tiles, p.col_tiles, rt, ct);
-      const int quarter = warp & 3, half = (warp - 2) >> 2;
-      const int unit = p.keep_q != nullptr && EPI != kEpiGluGrad ? 64 : 32;
-      const int share = max(kDpTileCols<EPI> / split, unit);
-      const int mid = share / 2 % unit == 0 ? share / 2 : share;
-      const int begin = part * share + (half ? mid : 0);
-      const int end = min(part * share + (half ? share : mid), kDpTileCols<EPI>);
-      const int row_base = rt * 256 + rank * 128 + quarter * 32;
+      const int quarter = warp & 3;
+      const int cols = max(kDpTileCols<EPI> / split, dense_column_unit<EPI>(p));
+      dense_columns<EPI>(p, min(part * cols, kDpTileCols<EPI>), min(part * cols + cols, kDpTileCols<EPI>), (warp - 2) >> 2, begin, end);
       DenseAcc acc;
       acc.taddr = 0;
       acc.part = tiles_addr + static_cast<uint32_t>(quarter * 32 + lane) * 16u;
       acc.split = split;
       acc.parity = rank;
-      if (row_base < p.M) dense_epilogue<T, EPI>(p, acc, s_out + (warp - 2) * kDpPatchBytes, lane, row_base, ct, begin, end);
+      acc.release_bar = 0;
+      TileEpilogue<T, EPI> epi(p, s_out + (warp - 2) * kDpPatches<EPI> * kDpPatch, lane, rt * 256 + rank * 128 + quarter * 32, ct, begin, end);
+      epi.prefetch();
+      epi.run(acc);
     }
     __syncthreads();
     ptx::cluster_sync_all();          // nobody leaves while another still reads its part or its operands
