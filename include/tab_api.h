@@ -489,7 +489,8 @@ TAB_API int tab_dense_status_reset(tab_stream_t stream);
  * tab_act_grad: dz[M, N] = dy[M, N] act'(z), z kept in 16 bits (keep) or 8 (keep_q, keep_scale); dz null: nothing is stored (then act
  *   must be 0).  column_sums null, or fp32 [splits, N]: partial column sums of dz, one row per slice of the rows, summed by
  *   tab_column_sums into out[N] of `dtype` in slice order; the number of slices is tab_act_grad_splits(M, N).
- * tab_copy_2d: 16-bit elements; dst(r, c) = src(r, c) inside [src_rows, src_cols), 0 elsewhere in [dst_rows, dst_cols); any strides. */
+ * tab_copy_2d: up to 8 copies of 16-bit matrices in one launch (`copies` is a host array): dst(r, c) = src(r, c) inside
+ *   [src_rows, src_cols), 0 elsewhere in [dst_rows, dst_cols); any strides. */
 TAB_API int tab_checkpoint_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
                                  int64_t lds, tab_stream_t stream);
 TAB_API int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t lds, int64_t rows, int64_t cols, void* y,
@@ -498,8 +499,13 @@ TAB_API int tab_act_grad_splits(int64_t M, int64_t N, size_t* splits);
 TAB_API int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, int64_t N, int act, const void* keep, const int8_t* keep_q,
                          const float* keep_scale, int64_t keep_ld, void* dz, float* column_sums, tab_stream_t stream);
 TAB_API int tab_column_sums(const float* column_sums, int64_t splits, int64_t N, void* out, int dtype, tab_stream_t stream);
-TAB_API int tab_copy_2d(const void* src, int64_t src_row_stride, int64_t src_col_stride, int64_t src_rows, int64_t src_cols, void* dst,
-                        int64_t dst_row_stride, int64_t dst_col_stride, int64_t dst_rows, int64_t dst_cols, tab_stream_t stream);
+typedef struct tab_copy {
+  const void* src; /* device; strides and sizes in elements */
+  int64_t src_row_stride, src_col_stride, src_rows, src_cols;
+  void* dst;
+  int64_t dst_row_stride, dst_col_stride, dst_rows, dst_cols;
+} tab_copy;
+TAB_API int tab_copy_2d(const tab_copy* copies, int count, tab_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -2,9 +2,9 @@
 // HBM: a value is read once and written once.
 //
 // Mapping of the 8-bit kernels: 8 lanes hold the 64 values of a block, 8 each (16 bytes of 16-bit data), so the block's
-// amax is three shuffles and every lane stores 8 bytes of q.  A warp takes 4 blocks side by side and kUnroll such groups in
-// flight, loads first.  When rows are whole numbers of blocks and lie back to back, the matrix is one long row and no
-// division is left in the loop.
+// amax is three shuffles and every lane stores 8 bytes of q.  A warp takes 4 blocks side by side and several such groups in
+// flight, loads first, the values in their raw form until they are quantised.  When rows are whole numbers of blocks and lie
+// back to back, the matrix is one long row and no division is left in the loop.
 #include "dense_math.cuh"
 
 namespace tab {
@@ -13,24 +13,42 @@ constexpr int kCkThreads = 256;
 constexpr int kCkUnroll = 4;
 constexpr int kCkChunk = 4 * kCkUnroll;          // blocks of 64 per warp and iteration
 
-// 8 values at column `col` of a row; columns >= cols are zero.  VEC: 16-byte loads (aligned, cols a multiple of 8).
+// 8 values at column `col` of a row, as they lie in memory; columns >= cols are zero.  VEC: 16-byte loads (aligned, cols a
+// multiple of 8).
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_cols8(const T* row, int64_t col, int64_t cols, float (&v)[8]) {
+__device__ __forceinline__ void load_cols8(const T* row, int64_t col, int64_t cols, Raw8<T>& raw) {
   if constexpr (VEC) {
-    if (col < cols) {
-      Elem<T>::load8(row + col, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
+    if (col < cols) raw.load(row + col); else raw = Raw8<T>{};
   } else {
+    T t[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? Elem<T>::to_f32(row[col + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) t[i] = col + i < cols ? row[col + i] : Elem<T>::from_f32(0.f);
+    raw = *reinterpret_cast<const Raw8<T>*>(t);
   }
 }
 
+// largest magnitude of 8 values as fp32 bits: NaN > infinity > every finite value
+__device__ __forceinline__ uint32_t raw_amax_bits(const Raw8<__nv_bfloat16>& raw) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw.r);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+  return max(__float_as_uint(__low2float(m)) & 0x7fffffffu, __float_as_uint(__high2float(m)) & 0x7fffffffu);
+}
+__device__ __forceinline__ uint32_t raw_amax_bits(const Raw8<__half>& raw) {
+  const __half2* h = reinterpret_cast<const __half2*>(&raw.r);
+  const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+  return max(__float_as_uint(__low2float(m)) & 0x7fffffffu, __float_as_uint(__high2float(m)) & 0x7fffffffu);
+}
+__device__ __forceinline__ uint32_t raw_amax_bits(const Raw8<float>& raw) {
+  float v[8];
+  raw.unpack(v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  return m;
+}
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kCkThreads) checkpoint_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols,
+__global__ void __launch_bounds__(kCkThreads, VEC ? 4 : 2) checkpoint_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols,
                                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
                                                                       int64_t lds) {
   const int lane = threadIdx.x & 31;
@@ -39,24 +57,24 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_quant_kernel(const T* _
   const int64_t total = rows * chunks;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kCkThreads / 32);
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
-    const int64_t row = chunks == 1 ? w : w / chunks;
-    const int64_t b0 = (chunks == 1 ? 0 : w - row * chunks) * kCkChunk;
+    const int64_t row = chunks == 1 ? w : rows == 1 ? 0 : w / chunks;
+    const int64_t b0 = (w - row * chunks) * kCkChunk;
     const T* xr = x + row * ldx;
-    float v[kCkUnroll][8];
+    Raw8<T> raw[kCkUnroll];
 #pragma unroll
-    for (int i = 0; i < kCkUnroll; ++i) load_cols8<T, VEC>(xr, (b0 + i * 4 + (lane >> 3)) * 64 + (lane & 7) * 8, cols, v[i]);
+    for (int i = 0; i < kCkUnroll; ++i) load_cols8<T, VEC>(xr, (b0 + i * 4 + (lane >> 3)) * 64 + (lane & 7) * 8, cols, raw[i]);
 #pragma unroll
     for (int i = 0; i < kCkUnroll; ++i) {
       const int64_t blk = b0 + i * 4 + (lane >> 3);
       const int64_t col = blk * 64 + (lane & 7) * 8;
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+      uint32_t m = raw_amax_bits(raw[i]);
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (blk >= blocks) continue;
       const RowQuant rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
-      const uint2 o = quant8(v[i], rq);
+      float v[8];
+      raw[i].unpack(v);
+      const uint2 o = quant8(v, rq);
       if constexpr (VEC) {
         if (col < cols) *reinterpret_cast<uint2*>(q + row * ldq + col) = o;
       } else {
@@ -80,8 +98,8 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const in
   const int64_t total = rows * chunks;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kCkThreads / 32);
   for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kCkThreads / 32) + (threadIdx.x >> 5); w < total; w += warps) {
-    const int64_t row = chunks == 1 ? w : w / chunks;
-    const int64_t b0 = (chunks == 1 ? 0 : w - row * chunks) * kCkChunk;
+    const int64_t row = chunks == 1 ? w : rows == 1 ? 0 : w / chunks;
+    const int64_t b0 = (w - row * chunks) * kCkChunk;
     uint2 raw[kCkUnroll];
     float s[kCkUnroll];
 #pragma unroll
@@ -122,14 +140,40 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const in
 }
 
 // dz = dy act'(z) and partial column sums of dz.  A CTA owns 128 columns (16 lanes x 8) and a slice of the rows; 16 rows per
-// step, so a warp reads two rows' 256-byte segments.  Column sums stay in registers over the slice and are added over the
-// 16 row lanes once, in a fixed order.
+// step, so a warp reads two rows' 256-byte segments.  The next step's values are loaded before this step's are used.  Column sums
+// stay in registers over the slice and are added over the 16 row lanes once, in a fixed order.  The slices are chosen so that all
+// CTAs are resident at once: with 1.4 turns of CTAs and no load ahead, 8192 x 7168 with GELU took 171 us, now XX (its bytes: 54).
 constexpr int kAgThreads = 256;
 constexpr int kAgCols = 128;
 constexpr int kAgRows = kAgThreads / (kAgCols / 8);
+constexpr int kAgCtasPerSm = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kAgThreads) act_grad_kernel(const T* __restrict__ dy, int64_t lddy, int64_t M, int64_t N, int act,
+// what one step reads of the activation's argument
+template <typename T, bool KEEP8>
+struct KeptArg {
+  Raw8<T> raw;
+  uint2 q;
+  float s;
+  __device__ __forceinline__ void load(const T* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld, int64_t r, int64_t col) {
+    if constexpr (KEEP8) {
+      q = __ldg(reinterpret_cast<const uint2*>(keep_q + r * keep_ld + col));
+      s = __ldg(keep_scale + r * (keep_ld / kKeepBlock) + col / kKeepBlock);
+    } else {
+      raw.load(keep + r * keep_ld + col);
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&z)[8]) const {
+    if constexpr (KEEP8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = static_cast<float>(static_cast<int8_t>(j < 4 ? q.x >> (8 * j) : q.y >> (8 * j - 32))) * s;
+    } else {
+      raw.unpack(z);
+    }
+  }
+};
+
+template <typename T, bool KEEP8>
+__global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(const T* __restrict__ dy, int64_t lddy, int64_t M, int64_t N, int act,
                                                               const T* __restrict__ keep, const int8_t* __restrict__ keep_q,
                                                               const float* __restrict__ keep_scale, int64_t keep_ld, T* __restrict__ dz,
                                                               float* __restrict__ sums) {
@@ -138,34 +182,38 @@ __global__ void __launch_bounds__(kAgThreads) act_grad_kernel(const T* __restric
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kAgCols + cl * 8;
   const int64_t r_begin = M * blockIdx.y / gridDim.y, r_end = M * (blockIdx.y + 1) / gridDim.y;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (col < N) {
-#pragma unroll 2
-    for (int64_t r = r_begin + rl; r < r_end; r += kAgRows) {
-      float g[8];
-      Elem<T>::load8(dy + r * lddy + col, g);
-      if (act != TAB_ACT_NONE) {
-        float z[8];
-        if (keep_q != nullptr) {
-          const uint2 raw = __ldg(reinterpret_cast<const uint2*>(keep_q + r * keep_ld + col));
-          const float s = __ldg(keep_scale + r * (keep_ld / kKeepBlock) + col / kKeepBlock);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) z[j] = static_cast<float>(static_cast<int8_t>(j < 4 ? raw.x >> (8 * j) : raw.y >> (8 * j - 32))) * s;
-        } else {
-          Elem<T>::load8(keep + r * keep_ld + col, z);
+  if (col < N && r_begin + rl < r_end) {
+    with_act(act, [&](auto tag) {
+      constexpr int ACT = decltype(tag)::value;
+      int64_t r = r_begin + rl;
+      Raw8<T> g_next;
+      KeptArg<T, KEEP8> z_next;
+      g_next.load(dy + r * lddy + col);
+      if constexpr (ACT != TAB_ACT_NONE) z_next.load(keep, keep_q, keep_scale, keep_ld, r, col);
+      for (; r < r_end; r += kAgRows) {
+        const Raw8<T> g_raw = g_next;
+        const KeptArg<T, KEEP8> z_raw = z_next;
+        if (r + kAgRows < r_end) {
+          g_next.load(dy + (r + kAgRows) * lddy + col);
+          if constexpr (ACT != TAB_ACT_NONE) z_next.load(keep, keep_q, keep_scale, keep_ld, r + kAgRows, col);
         }
-        with_act(act, [&](auto tag) {
+        float g[8];
+        g_raw.unpack(g);
+        if constexpr (ACT != TAB_ACT_NONE) {
+          float z[8];
+          z_raw.unpack(z);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             float a, d;
-            act_both<decltype(tag)::value>(z[j], a, d);
+            act_both<ACT>(z[j], a, d);
             g[j] *= d;
           }
-        });
-      }
-      if (dz != nullptr) Elem<T>::store8(dz + r * N + col, g);
+        }
+        if (dz != nullptr) Elem<T>::store8(dz + r * N + col, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += g[j];
-    }
+        for (int j = 0; j < 8; ++j) acc[j] += g[j];
+      }
+    });
   }
   if (sums == nullptr) return;
 #pragma unroll
@@ -192,22 +240,60 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float* __restric
   out[c] = Elem<T>::from_f32(s);
 }
 
-// 16-bit copy between any strides, 64 x 64 tiles through shared memory so that both sides run along their contiguous index.
-__global__ void __launch_bounds__(256) copy_2d_kernel(const uint16_t* __restrict__ src, int64_t srs, int64_t scs, int64_t src_rows, int64_t src_cols,
-                                                      uint16_t* __restrict__ dst, int64_t drs, int64_t dcs, int64_t dst_rows, int64_t dst_cols,
-                                                      int64_t col_tiles, int64_t tiles) {
-  __shared__ uint16_t tile[64][66];
-  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t rt = t / col_tiles;
-    const int64_t r0 = rt * 64, c0 = (t - rt * col_tiles) * 64;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-      const int r = scs == 1 ? i >> 6 : i & 63, c = scs == 1 ? i & 63 : i >> 6;
-      tile[r][c] = (r0 + r < src_rows && c0 + c < src_cols) ? src[(r0 + r) * srs + (c0 + c) * scs] : static_cast<uint16_t>(0);
+// Up to kMaxCopies 16-bit copies between any strides in one launch, 64 x 64 tiles through shared memory so that both sides run
+// along their contiguous index; rows that begin anywhere are read 2 bytes per lane, 16 loads of a thread in flight, and
+// 16-byte aligned destination rows are written 16 bytes per lane.
+constexpr int kMaxCopies = 8;
+struct CopyItem {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t srs, scs, drs, dcs;
+  int src_rows, src_cols, dst_rows, dst_cols, col_tiles, first_tile;
+};
+struct CopyList {
+  CopyItem item[kMaxCopies];
+  int count, tiles;
+};
+
+__global__ void __launch_bounds__(256) copy_2d_kernel(const __grid_constant__ CopyList list) {
+  __shared__ __align__(16) uint16_t tile[64][72];
+  for (int t = blockIdx.x; t < list.tiles; t += gridDim.x) {
+    int k = 0;
+    while (k + 1 < list.count && list.item[k + 1].first_tile <= t) ++k;
+    const CopyItem& it = list.item[k];
+    const int local = t - it.first_tile;
+    const int rt = local / it.col_tiles;
+    const int r0 = rt * 64, c0 = (local - rt * it.col_tiles) * 64;
+    const bool along_cols = it.scs == 1;
+    uint16_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = i * 256 + threadIdx.x;
+      const int r = along_cols ? e >> 6 : e & 63, c = along_cols ? e & 63 : e >> 6;
+      v[i] = (r0 + r < it.src_rows && c0 + c < it.src_cols) ? it.src[(r0 + r) * it.srs + (c0 + c) * it.scs] : static_cast<uint16_t>(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = i * 256 + threadIdx.x;
+      tile[along_cols ? e >> 6 : e & 63][along_cols ? e & 63 : e >> 6] = v[i];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-      const int r = dcs == 1 ? i >> 6 : i & 63, c = dcs == 1 ? i & 63 : i >> 6;
-      if (r0 + r < dst_rows && c0 + c < dst_cols) dst[(r0 + r) * drs + (c0 + c) * dcs] = tile[r][c];
+    if (it.dcs == 1 && (it.drs & 7) == 0 && (it.dst_cols & 7) == 0 && (reinterpret_cast<uintptr_t>(it.dst) & 15u) == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = i * 256 + threadIdx.x;
+        const int r = e >> 3, c = (e & 7) * 8;
+        if (r0 + r < it.dst_rows && c0 + c < it.dst_cols)
+          *reinterpret_cast<uint4*>(it.dst + (r0 + r) * it.drs + c0 + c) = *reinterpret_cast<const uint4*>(&tile[r][c]);
+      }
+    } else {
+      const bool out_cols = it.dcs == 1;
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int e = i * 256 + threadIdx.x;
+        const int r = out_cols ? e >> 6 : e & 63, c = out_cols ? e & 63 : e >> 6;
+        if (r0 + r < it.dst_rows && c0 + c < it.dst_cols) it.dst[(r0 + r) * it.drs + (c0 + c) * it.dcs] = tile[r][c];
+      }
     }
     __syncthreads();
   }
@@ -233,10 +319,10 @@ static void launch_dequant(const int8_t* q, int64_t ldq, const float* scale, int
   checkpoint_dequant_kernel<T, VEC><<<grid, kCkThreads, 0, st>>>(q, ldq, scale, lds, rows, cols, static_cast<T*>(y), ldy, pad_cols);
 }
 
-// slices of the rows: enough CTAs for a few per SM, at least 64 rows each
+// slices of the rows: as many as keep all CTAs resident at once, at least 64 rows each
 static int64_t act_grad_splits(int64_t M, int64_t N) {
   const int64_t col_ctas = (N + kAgCols - 1) / kAgCols;
-  int64_t s = (4 * kNumSMs + col_ctas - 1) / col_ctas;
+  int64_t s = kAgCtasPerSm * kNumSMs / col_ctas;
   const int64_t most = (M + 63) / 64;
   if (s > most) s = most;
   if (s > 65535) s = 65535;
@@ -323,12 +409,15 @@ extern "C" int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, 
   if (M == 0 && !column_sums) return TAB_OK;
   const dim3 grid((unsigned)((N + kAgCols - 1) / kAgCols), (unsigned)act_grad_splits(M, N));
   cudaStream_t st = as_stream(stream);
-  if (dtype == TAB_BF16)
-    act_grad_kernel<__nv_bfloat16><<<grid, kAgThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(dy), lddy, M, N, act, static_cast<const __nv_bfloat16*>(keep),
-                                                                keep_q, keep_scale, keep_ld, static_cast<__nv_bfloat16*>(dz), column_sums);
-  else
-    act_grad_kernel<__half><<<grid, kAgThreads, 0, st>>>(static_cast<const __half*>(dy), lddy, M, N, act, static_cast<const __half*>(keep), keep_q,
-                                                         keep_scale, keep_ld, static_cast<__half*>(dz), column_sums);
+#define TAB_AG(T, K8) \
+  act_grad_kernel<T, K8><<<grid, kAgThreads, 0, st>>>(static_cast<const T*>(dy), lddy, M, N, act, static_cast<const T*>(keep), keep_q, keep_scale, \
+                                                      keep_ld, static_cast<T*>(dz), column_sums)
+  if (dtype == TAB_BF16) {
+    if (keep_q) TAB_AG(__nv_bfloat16, true); else TAB_AG(__nv_bfloat16, false);
+  } else {
+    if (keep_q) TAB_AG(__half, true); else TAB_AG(__half, false);
+  }
+#undef TAB_AG
   return check_launch(op);
 }
 
@@ -343,17 +432,37 @@ extern "C" int tab_column_sums(const float* column_sums, int64_t splits, int64_t
   return check_launch(op);
 }
 
-extern "C" int tab_copy_2d(const void* src, int64_t src_row_stride, int64_t src_col_stride, int64_t src_rows, int64_t src_cols, void* dst,
-                           int64_t dst_row_stride, int64_t dst_col_stride, int64_t dst_rows, int64_t dst_cols, tab_stream_t stream) {
+extern "C" int tab_copy_2d(const tab_copy* copies, int count, tab_stream_t stream) {
   const char* op = "copy_2d";
-  if (src_rows < 0 || src_cols < 0 || dst_rows < 0 || dst_cols < 0 || src_rows > kMaxDim || src_cols > kMaxDim || dst_rows > kMaxDim || dst_cols > kMaxDim)
-    return fail(TAB_ERR_BAD_ARG, "%s: negative or huge size", op);
-  if (dst_rows == 0 || dst_cols == 0) return TAB_OK;
-  if (!dst || (!src && src_rows > 0 && src_cols > 0)) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
-  if (!natural(src, 2) || !natural(dst, 2)) return fail(TAB_ERR_ALIGNMENT, "%s: misaligned pointer", op);
-  const int64_t col_tiles = (dst_cols + 63) / 64, tiles = (dst_rows + 63) / 64 * col_tiles;
-  copy_2d_kernel<<<grid_for(tiles, 8), 256, 0, as_stream(stream)>>>(static_cast<const uint16_t*>(src), src_row_stride, src_col_stride, src_rows,
-                                                                    src_cols, static_cast<uint16_t*>(dst), dst_row_stride, dst_col_stride,
-                                                                    dst_rows, dst_cols, col_tiles, tiles);
+  if (count < 0 || count > kMaxCopies || (count > 0 && !copies)) return fail(TAB_ERR_BAD_ARG, "%s: %d copies (at most %d)", op, count, kMaxCopies);
+  CopyList list = {};
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i) {
+    const tab_copy& c = copies[i];
+    if (c.src_rows < 0 || c.src_cols < 0 || c.dst_rows < 0 || c.dst_cols < 0) return fail(TAB_ERR_BAD_ARG, "%s: negative size", op);
+    const int64_t most = 1LL << 30;
+    if (c.src_rows > most || c.src_cols > most || c.dst_rows > most || c.dst_cols > most) return fail(TAB_ERR_UNSUPPORTED, "%s: dimension too large", op);
+    if (c.dst_rows == 0 || c.dst_cols == 0) continue;
+    if (!c.dst || (!c.src && c.src_rows > 0 && c.src_cols > 0)) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
+    if (!natural(c.src, 2) || !natural(c.dst, 2)) return fail(TAB_ERR_ALIGNMENT, "%s: misaligned pointer", op);
+    CopyItem& it = list.item[list.count++];
+    it.src = static_cast<const uint16_t*>(c.src);
+    it.dst = static_cast<uint16_t*>(c.dst);
+    it.srs = c.src_row_stride;
+    it.scs = c.src_col_stride;
+    it.drs = c.dst_row_stride;
+    it.dcs = c.dst_col_stride;
+    it.src_rows = (int)c.src_rows;
+    it.src_cols = (int)c.src_cols;
+    it.dst_rows = (int)c.dst_rows;
+    it.dst_cols = (int)c.dst_cols;
+    it.col_tiles = (int)((c.dst_cols + 63) / 64);
+    it.first_tile = (int)tiles;
+    tiles += (c.dst_rows + 63) / 64 * it.col_tiles;
+    if (tiles > (1LL << 30)) return fail(TAB_ERR_UNSUPPORTED, "%s: too many elements", op);
+  }
+  if (tiles == 0) return TAB_OK;
+  list.tiles = (int)tiles;
+  copy_2d_kernel<<<grid_for(tiles, 8), 256, 0, as_stream(stream)>>>(list);
   return check_launch(op);
 }

@@ -91,7 +91,7 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 constexpr int kKeepBlock = 64;
 
 __device__ __forceinline__ RowQuant make_block_quant(float amax, bool finite) {
-  RowQuant rq = make_row_quant(amax);
+  RowQuant rq = make_row_quant_fast(amax);
   if (!finite) {
     rq.scale = __int_as_float(0x7fc00000);
     rq.inv = 0.f;

@@ -219,8 +219,7 @@ struct DenseAcc {
   }
 };
 
-// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 16; of 64
-// where 8-bit blocks are written).  What it reads from global memory (residual, kept values) is asked for before the
+// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 16).  What it reads from global memory (residual, kept values) is asked for before the
 // accumulators are waited for, then one step ahead.
 template <typename T, int EPI>
 struct TileEpilogue {
@@ -260,20 +259,21 @@ struct TileEpilogue {
     acc.release(lane);
   }
 
-  // the quantiser of 64 columns from accumulator column `at` on, whose output columns begin at col
-  __device__ __forceinline__ RowQuant block_quant(const DenseAcc& acc, const void* bias, int at, int col, float* scale) const {
+  // The quantiser of the 64 columns from accumulator column `at` on, whose output columns begin at col.  A block may be shared by
+  // several warps: each takes the amax of all of it, the one that holds its first column stores the scale.
+  __device__ __forceinline__ RowQuant block_quant(const DenseAcc& acc, const void* bias, int at, int col, float* scale, bool first) const {
     uint32_t m = 0;
 #pragma unroll 1
     for (int h = 0; h < 64; h += 16) {
       float v[16];
       Bias16<T> b;
-      b.load(bias, col + h, p.N);
+      if (bias != nullptr) b.load(bias, col + h, p.N);
       acc.fetch(at + h, v);
-      b.add(v);
+      if (bias != nullptr) b.add(v);
       m = max(m, amax_bits16(v, col + h, p.N));
     }
     const RowQuant rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
-    if (rvalid) *scale = rq.scale;
+    if (rvalid && first) *scale = rq.scale;
     return rq;
   }
 
@@ -287,7 +287,8 @@ struct TileEpilogue {
     for (int c = col_begin; c < col_end; c += 16) {
       const int col = ct * 256 + c;
       if (col >= p.N && (!keep8 || (col & ~63) >= p.N)) break;
-      if (keep8 && (c & 63) == 0) rq = block_quant(acc, p.bias, c, col, p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock);
+      if (keep8 && ((c & 63) == 0 || c == col_begin))
+        rq = block_quant(acc, p.bias, c & ~63, col & ~63, p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock, (c & 63) == 0);
       float v[16];
       Bias16<T> b;
       if (has_bias) b.load(p.bias, col, p.N);
@@ -332,10 +333,11 @@ struct TileEpilogue {
       const int col = ct * 128 + c;
       if (col >= p.N && (!keep8 || (col & ~63) >= p.N)) break;
       const int at = (c >> 6) * 128 + (c & 63);
-      if (keep8 && (c & 63) == 0) {
+      if (keep8 && ((c & 63) == 0 || c == col_begin)) {
         float* scale = p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock;
-        rg = block_quant(acc, p.bias, at, col, scale);
-        ru = block_quant(acc, has_bias ? bias_up : nullptr, at + 64, col, scale + p.keep_up / kKeepBlock);
+        const int block_at = (c >> 6) * 128;
+        rg = block_quant(acc, p.bias, block_at, col & ~63, scale, (c & 63) == 0);
+        ru = block_quant(acc, has_bias ? bias_up : nullptr, block_at + 64, col & ~63, scale + p.keep_up / kKeepBlock, (c & 63) == 0);
       }
       float g[16], u[16];
       Bias16<T> bg, bu;
@@ -436,15 +438,9 @@ struct TileEpilogue {
 template <int EPI>
 constexpr int kDpTileCols = EPI == kEpiGlu ? 128 : 256;
 
-// Columns that stay with one warp: 16, or a whole 8-bit block.
-template <int EPI>
-__device__ __forceinline__ int dense_column_unit(const DenseParams& p) {
-  return p.keep_q != nullptr && EPI != kEpiGluGrad ? kKeepBlock : 16;
-}
-// The part of columns [from, to) that warp `share` of the four warps of a lane quarter takes.
-template <int EPI>
-__device__ __forceinline__ void dense_columns(const DenseParams& p, int from, int to, int share, int& begin, int& end) {
-  const int each = max((to - from) / 4, dense_column_unit<EPI>(p));
+// The part of a pair's columns [from, to) that warp `share` of the four warps of a lane quarter takes.
+__device__ __forceinline__ void dense_columns(int from, int to, int share, int& begin, int& end) {
+  const int each = max((to - from) / 4, 16);
   begin = min(from + share * each, to);
   end = min(begin + each, to);
 }
@@ -606,7 +602,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         int rt, ct;
         dense_tile_coord(tile, p.row_tiles, p.col_tiles, rt, ct);
         int begin, end;
-        dense_columns<EPI>(p, 0, kDpTileCols<EPI>, share, begin, end);
+        dense_columns(0, kDpTileCols<EPI>, share, begin, end);
         TileEpilogue<T, EPI> epi(p, s_out + (warp - 2) * kDpPatches<EPI> * kDpPatch, lane, rt * 256 + rank * 128 + quarter * 32, ct, begin, end);
         epi.prefetch();
         if (!__all_sync(0xffffffffu, dense_wait(bar_tfull(buf), tphase, s_abort, 34, p.wait_cycles))) break;
@@ -622,13 +618,11 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   if constexpr (SPLIT) {
     ptx::cluster_sync_all();          // every pair's part is in place
     if (warp >= 2) {
-      // this pair's columns of the tile; 64-value blocks are not cut, so with four pairs some hold none (which pairs share a
-      // tile must not depend on what is kept: the sums would differ)
       int rt, ct, begin, end;
       dense_tile_coord(first, p.row_tiles, p.col_tiles, rt, ct);
       const int quarter = warp & 3;
-      const int cols = max(kDpTileCols<EPI> / split, dense_column_unit<EPI>(p));
-      dense_columns<EPI>(p, min(part * cols, kDpTileCols<EPI>), min(part * cols + cols, kDpTileCols<EPI>), (warp - 2) >> 2, begin, end);
+      const int cols = kDpTileCols<EPI> / split;             // this pair's columns of the tile
+      dense_columns(part * cols, part * cols + cols, (warp - 2) >> 2, begin, end);
       DenseAcc acc;
       acc.taddr = 0;
       acc.part = tiles_addr + static_cast<uint32_t>(quarter * 32 + lane) * 16u;

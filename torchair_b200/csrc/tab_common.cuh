@@ -248,6 +248,21 @@ __device__ __forceinline__ RowQuant make_row_quant(float amax) {
   return rq;
 }
 
+// amax / 127 and its reciprocal without the library's checked division: q = RN(amax / 127) by one correction step from
+// the correctly rounded reciprocal of 127 (exact for every amax whose quotient and remainder are normal), inv by
+// rcp_rn_normal.  Rows outside the safe range, and scales whose significand is all ones, take make_row_quant.
+__device__ __forceinline__ RowQuant make_row_quant_fast(float amax) {
+  if (!(amax > 1e-24f && amax < 1e30f)) return make_row_quant(amax);
+  constexpr float kInv127 = 0x1.020408p-7f;    // RN(1 / 127)
+  const float q0 = __fmul_rn(amax, kInv127);
+  const float r = __fmaf_rn(-127.0f, q0, amax);
+  RowQuant rq;
+  rq.scale = __fmaf_rn(r, kInv127, q0);
+  rq.inv = rcp_rn_normal(rq.scale);
+  rq.exact = (__float_as_uint(rq.scale) & 0x7fffffu) == 0x7fffffu;
+  return rq;
+}
+
 constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23
 
 // Word whose low byte is clamp(rint(v / scale)), by the library's IEEE division.

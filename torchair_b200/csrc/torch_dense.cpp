@@ -14,6 +14,7 @@
 #include <array>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/tab_api.h"
 
@@ -58,6 +59,17 @@ struct Call {
   int dtype;
   cudaStream_t stream;
   at::TensorOptions opt;
+  // copies that put operands into a layout the kernels take, gathered so that one launch does them all
+  mutable std::array<tab_copy, 8> copies;
+  mutable int pending = 0;
+  mutable std::vector<Tensor> held;      // what the gathered copies read and write lives until they are launched
+  void flush() const {
+    if (pending == 0) return;
+    const int n = pending;
+    pending = 0;
+    ok(tab_copy_2d(copies.data(), n, stream), "tab_copy_2d");
+    held.clear();
+  }
   explicit Call(const Tensor& x, int dtype_) : dtype(dtype_), stream(c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), opt(x.options().requires_grad(false)) {}
   Tensor empty(at::IntArrayRef sizes) const { return at::empty(sizes, opt); }
   Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const { return at::empty(sizes, opt.dtype(t)); }
@@ -66,19 +78,21 @@ struct Call {
 
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 
-// dst = src inside src's shape, zero elsewhere (2-D, 16-bit, any strides)
+// dst = src inside src's shape, zero elsewhere (2-D, 16-bit, any strides); done by the next flush
 void copy_2d(const Call& c, const Tensor& src, const Tensor& dst) {
-  ok(tab_copy_2d(src.data_ptr(), src.stride(0), src.stride(1), src.size(0), src.size(1), dst.data_ptr(), dst.stride(0), dst.stride(1), dst.size(0),
-                 dst.size(1), c.stream),
-     "tab_copy_2d");
+  if (c.pending == static_cast<int>(c.copies.size())) c.flush();
+  c.copies[c.pending++] = tab_copy{src.data_ptr(), src.stride(0), src.stride(1), src.size(0), src.size(1),
+                                   dst.data_ptr(), dst.stride(0), dst.stride(1), dst.size(0), dst.size(1)};
+  c.held.push_back(src);
+  c.held.push_back(dst);
 }
 
 // A matrix in memory that the tensor maps take: contiguous along its columns (row-major) or along its rows, the other stride
 // a multiple of 8 elements.
 struct Mat {
   Tensor t;
-  int64_t ld;
-  bool row_major;
+  int64_t ld = 0;
+  bool row_major = true;
   const void* ptr() const { return t.data_ptr(); }
   // as operand [index of the product, contraction]: the rows of this matrix are the index ...
   int mn_by_rows() const { return row_major ? 0 : 1; }
@@ -174,6 +188,7 @@ struct Kept {
 // act(a b^T + bias) + residual: a [m, k], b [n, k] as operands
 void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int64_t m, int64_t n, int64_t k, const Tensor& out,
             const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept()) {
+  c.flush();
   ok(tab_dense_matmul(a, lda, a_mn, b, ldb, b_mn, c.dtype, m, n, k, ptr(bias), ptr(residual), act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                       out.data_ptr(), c.stream),
      "tab_dense_matmul");
@@ -201,10 +216,12 @@ Mat act_grad(const Call& c, const Mat& grad, int64_t n, int act, const Kept& kep
     ok(tab_act_grad_splits(m, n, &splits), "tab_act_grad_splits");
     parts = c.empty({static_cast<int64_t>(splits), n}, at::kFloat);
   }
-  if (dz.defined() || parts.defined())
+  if (dz.defined() || parts.defined()) {
+    c.flush();
     ok(tab_act_grad(grad.ptr(), grad.ld, c.dtype, m, n, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), ptr(dz), static_cast<float*>(ptr(parts)),
                     c.stream),
        "tab_act_grad");
+  }
   if (want_sums) {
     column_sums = c.empty({1, n});
     ok(tab_column_sums(static_cast<const float*>(parts.data_ptr()), parts.size(0), n, column_sums.data_ptr(), c.dtype, c.stream), "tab_column_sums");
@@ -284,11 +301,15 @@ Tensor ffn_forward(const Call& c, const FfnSizes& s, const Tensor& x, const Tens
     size_t bytes = 0;
     ok(tab_gated_ffn_workspace_bytes(s.m, h8, inner8, &bytes), "tab_gated_ffn_workspace_bytes");
     const Tensor ws = c.workspace(bytes);
-    ok(tab_gated_ffn(xm.ptr(), xm.ld, w1.ptr(), w1.ld, w1.mn_by_cols(), w2.ptr(), w2.ld, w2.mn_by_cols(), c.dtype, s.m, h8, inner8, ptr(b1), ptr(b2),
+    c.flush();
+  ok(tab_gated_ffn(xm.ptr(), xm.ld, w1.ptr(), w1.ld, w1.mn_by_cols(), w2.ptr(), w2.ld, w2.mn_by_cols(), c.dtype, s.m, h8, inner8, ptr(b1), ptr(b2),
                      ptr(r), s.act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), y.data_ptr(), ws.data_ptr(), ws.numel(), c.stream),
        "tab_gated_ffn");
   }
-  return h8 == s.h ? y : cut(c, y, s.m, s.h).view(x.sizes());
+  if (h8 == s.h) return y;
+  y = cut(c, y, s.m, s.h).view(x.sizes());
+  c.flush();
+  return y;
 }
 
 Tensor ffn_cuda(const Tensor& x, const Tensor& weight1, const Tensor& weight2, const OptTensor& bias1, const OptTensor& bias2, const OptTensor& residual,
@@ -352,6 +373,9 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
   }
   const Mat dy = rows_of(c, grad_.reshape({m, h}), h8);
+  Mat w1, xm;
+  if (want[0]) w1 = halves_of(c, weight1, h8, inner8);
+  if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, h}), h8);
   Kept kept;
   kept.values = kept_values;
   kept.scale = kept_scale;
@@ -360,19 +384,19 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     const Mat w2 = matrix_of(c, weight2, inner8, h8);
     dz.t = c.empty({m, 2 * inner8});
     hidden.t = c.empty({m, inner8});
-    ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h8, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
+    c.flush();
+  ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h8, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
   }
   if (want[2]) dw2 = cut(c, weight_grad(c, hidden, dy, inner8, h8, weight2), inner, h);
   if (want[0]) {
-    const Mat w1 = halves_of(c, weight1, h8, inner8);
     Tensor out = c.empty({m, h8});
     matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h8, 2 * inner8, out);
     dx = cut(c, out, m, h).view(grad_.sizes());
   }
   if (want[1]) {
-    const Mat xm = x8 ? dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8) : rows_of(c, x_.reshape({m, h}), h8);
+    if (x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8);
     dw1 = cut_halves(c, weight_grad(c, xm, dz, h8, 2 * inner8, weight1), h, inner);
   }
   if (want[3]) {
@@ -383,6 +407,7 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     act_grad(c, dy, h8, 0, Kept(), false, true, db2);
     db2 = cut(c, db2, 1, h).view({h});
   }
+  c.flush();
   return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
 }
 
@@ -424,7 +449,10 @@ Tensor linear_forward(const Call& c, const LinearSizes& s, at::IntArrayRef out_s
     const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.n}), n8) : Tensor();
     matmul(c, xm.ptr(), xm.ld, 0, w.ptr(), w.ld, w.mn_by_cols(), s.m, n8, k8, y, b, r, s.act, kept);
   }
-  return n8 == s.n ? y : cut(c, y, s.m, s.n).view(out_sizes);
+  if (n8 == s.n) return y;
+  y = cut(c, y, s.m, s.n).view(out_sizes);
+  c.flush();
+  return y;
 }
 
 Tensor linear_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, c10::string_view activation, bool) {
@@ -488,18 +516,21 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
       kept.values = kept_values;
       kept.scale = kept_scale;
     }
+    Mat w, xm;
+    if (want[0]) w = matrix_of(c, weight, k8, n8);
+    if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, k}), k8);
     const Mat dz = act_grad(c, rows_of(c, grad_.reshape({m, n}), n8), n8, act, kept, want[0] || want[1], want[2], db);
     if (want[0]) {
-      const Mat w = matrix_of(c, weight, k8, n8);
       Tensor out = c.empty({m, k8});
       matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k8, n8, out);
       dx = cut(c, out, m, k).view(x_sizes);
     }
     if (want[1]) {
-      const Mat xm = x8 ? dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8) : rows_of(c, x_.reshape({m, k}), k8);
+      if (x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8);
       dw = cut(c, weight_grad(c, xm, dz, k8, n8, weight), k, n);
     }
     if (want[2]) db = cut(c, db, 1, n).view({n});
+    c.flush();
   }
   auto result = [&](const Tensor& t) { return t.defined() ? t : c.empty({0}); };
   return {result(dx), result(dw), result(db)};
@@ -568,7 +599,9 @@ Tensor ck_weight_grad_cuda(const Tensor& q_, const Tensor& scale_, const Tensor&
   const Mat x = dequantise(c, q, scale, k8), dz = rows_of(c, grad_.reshape({m, n}), n8);
   Tensor out = c.empty({k8, n8});
   matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k8, n8, m, out);
-  return cut(c, out, k, n);
+  out = cut(c, out, k, n);
+  c.flush();
+  return out;
 }
 
 // ---- autograd ----
