@@ -2,6 +2,7 @@
 // how many CTAs share a tile, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
 #include <stdlib.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "dense_common.cuh"
@@ -123,14 +124,12 @@ static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int 
   return check_launch(op);
 }
 
-// Pairs that share a tile's contraction when `tiles` tiles are all there is to do.  The GPCs of a B200 hold 33 clusters of 4 such
-// CTAs or 15 of 8 at a time; one more costs a second turn (16 tiles of K = 7168: 26.1 us with two pairs, 38.7 with four).  Joining
-// the parts takes the time of some 20 blocks of the contraction with two pairs and 35 with four: one tile of K = 1024 takes
-// 11.0 / 11.3 / 13.0 us with 1 / 2 / 4 pairs, K = 4096 24.4 / 18.1 / 15.8.
+// Pairs that share a tile's contraction in the last, partly filled turn.  The GPCs of a B200 hold 33 clusters of 4 such CTAs or 15 of
+// 8 at a time; one more costs a second turn.  The join takes longer than it saves on short contractions: 14 tiles left of 88 at
+// K = 3008 take 40.4 / 43.5 / 42.2 us with 1 / 2 / 4 pairs, 16 left of 90 at K = 8192 98.4 / 91.3, 2 left of 224 178.8 / 171.7 / 167.9.
 static int pair_split(int64_t tiles, int num_kb) {
-  if (tiles <= 15 && num_kb >= 48) return 4;
-  if (tiles <= 33 && num_kb >= 24) return 2;
-  return 1;
+  if (num_kb < 64) return 1;
+  return tiles <= 15 ? 4 : tiles <= 33 ? 2 : 1;
 }
 
 template <typename T, int EPI>
@@ -180,46 +179,111 @@ static int launch_pair_epi(const char* op, int dtype, const DenseOperand& a, con
 }
 
 // ---- narrow kernel ----
-// Up to 128 rows the weights are read once either way and the narrow kernel pads nothing to 256 rows.
-static bool use_narrow(int64_t M, const DenseOperand& x) { return M <= kNwMaxTokens && x.mn == 0; }
+struct NarrowPlan {
+  int nt, split, row_tiles, col_tiles;
+  double cost;               // estimated SM cycles
+};
 
-template <typename T, int EPI>
-static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensorMap& mx, const DenseParams& p, int tiles, cudaStream_t st) {
-  const int smem = 1024 + p.stages * dense_narrow_stage_bytes(p.nt) + kNwCtrlBytes;
+// CTAs of the wide form that the GPCs of a B200 hold at a time in clusters of 1 .. 8 (occupancy queries on the GPU).
+constexpr int kClusterRoom[kNwMaxSplit + 1] = {0, 148, 148, 135, 132, 130, 132, 105, 120};
+
+static NarrowPlan narrow_plan(int64_t M, int64_t N, int num_kb, int epi, bool x_mn) {
+  NarrowPlan best = {};
+  const int64_t features = epi == kEpiGlu ? 64 : 128;
+  const int64_t col_tiles = (N + features - 1) / features;
+  if (M <= 64) {
+    best.nt = x_mn ? 64 : M <= 16 ? 16 : M <= 32 ? 32 : 64;       // (boxes of 64 rows where x is contiguous along its rows)
+    best.row_tiles = 1;
+    best.col_tiles = (int)col_tiles;
+    // CTAs per tile: as many as fill the SMs, two of them on some.  Measured over weights that come from HBM (us): one row, 56 tiles
+    // of K = 2048: 10.4 / 9.3 / 9.7 / 11.4 with 2 / 3 / 4 / 5 CTAs; 32 tiles of K = 7168: 15.6 / 14.8 / 14.4 / 14.2 with 3 / 4 / 5 / 6;
+    // with 64 rows the parts to exchange weigh more: 56 tiles 13.1 / 13.1 / 13.3 with 2 / 3 / 4.
+    int64_t split = (best.nt <= 32 ? 176 : 132) / col_tiles;
+    if (split > kNwMaxSplit) split = kNwMaxSplit;
+    if (split > num_kb / 4) split = num_kb / 4;
+    best.split = split < 1 ? 1 : (int)split;
+    best.cost = 0.0;                           // never slower than a 256-row tile: the same weights, less of everything else
+    return best;
+  }
+  // Estimates in SM cycles, from stamps inside the kernel: 58 bytes of operands a cycle reach an SM, a block takes at least 400; 3500 cycles until the first
+  // block and after the last, 30 per row of the tile for the epilogue; the exchange of parts 1500 and 64 per row.
+  for (int nt = x_mn ? 64 : 32; nt <= kNwMaxTokens; nt *= 2) {
+    const int64_t row_tiles = (M + nt - 1) / nt, tiles = row_tiles * col_tiles;
+    if (tiles > 8 * 148) continue;
+    const int per_sm = nt <= 64 ? 2 : 1;
+    for (int split = 1; split <= kNwMaxSplit; ++split) {
+      if (split > 1 && (nt > 128 || split * 4 > num_kb || tiles * split > kClusterRoom[split])) continue;
+      const int64_t ctas = tiles * split, room = static_cast<int64_t>(kClusterRoom[split]) * per_sm;
+      const double turns = static_cast<double>((ctas + room - 1) / room);
+      const double together = ctas > kClusterRoom[split] ? per_sm : 1;
+      const double cost = turns * ((num_kb + split - 1) / split * std::max(400.0, together * dense_narrow_stage_bytes(nt) / 58.0) + 3500.0 + 30.0 * nt * together +
+                                   (split > 1 ? 1500.0 + 64.0 * nt : 0.0));
+      if (best.nt == 0 || cost < best.cost) best = NarrowPlan{nt, split, (int)row_tiles, (int)col_tiles, cost};
+    }
+  }
+  return best;
+}
+
+// The pair kernel's estimate in the same unit.
+static double pair_cost(int64_t M, int64_t N, int num_kb, int epi, int pairs) {
+  const int64_t cols = epi == kEpiGlu ? 128 : 256;
+  const int64_t tiles = ((M + 255) / 256) * ((N + cols - 1) / cols);
+  const int64_t turns = tiles / pairs, rest = tiles % pairs;
+  const int split = rest ? pair_split(rest, num_kb) : 1;
+  const double last = rest == 0 ? 0.0 : split > 1 ? num_kb / split * 520.0 + 9000.0 : num_kb * 520.0;
+  return turns * num_kb * 520.0 + last + 11000.0;
+}
+
+template <typename T, int EPI, bool WIDE>
+static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensorMap& mx, const DenseParams& p, cudaStream_t st) {
+  const int smem = 1024 + p.stages * dense_narrow_stage_bytes(p.nt) + kNwCtrlBytes + dense_narrow_recv_bytes(p.nt, p.split);
   static std::atomic<unsigned long long> done{0};
-  const int rc = allow_smem(op, dense_narrow_kernel<T, EPI>, kNwSmemTarget, done);
+  const int rc = allow_smem(op, dense_narrow_kernel<T, EPI, WIDE>, dense_narrow_smem(true), done);
   if (rc != TAB_OK) return rc;
-  return launch_cluster(op, dense_narrow_kernel<T, EPI>, tiles * p.split, kNwThreads, smem, p.split, p.dependent != 0, mw, mx, p, st);
+  return launch_cluster(op, dense_narrow_kernel<T, EPI, WIDE>, p.row_tiles * p.col_tiles * p.split, dense_narrow_threads(WIDE), smem, p.split,
+                        p.dependent != 0, mw, mx, p, st);
 }
 
 template <int EPI>
-static int launch_narrow_epi(const char* op, int dtype, const DenseOperand& x, const DenseOperand& w, DenseParams& p, cudaStream_t st) {
+static int launch_narrow_epi(const char* op, int dtype, const DenseOperand& x, const DenseOperand& w, DenseParams& p, const NarrowPlan& plan,
+                             cudaStream_t st) {
   p.num_kb = (int)((x.depth + kDnBlockK - 1) / kDnBlockK);
-  p.nt = 16;
-  while (p.nt < p.M) p.nt *= 2;
-  const int tiles = EPI == kEpiGlu ? (p.N + 63) / 64 : (p.N + 127) / 128;
-  // CTAs per tile: as many as fill the SMs, two of them on some.  Measured over weights that come from HBM (us): one row, 56 tiles
-  // of K = 2048: 10.4 / 9.3 / 9.7 / 11.4 with 2 / 3 / 4 / 5 CTAs; 32 tiles of K = 7168: 15.6 / 14.8 / 14.4 / 14.2 with 3 / 4 / 5 / 6;
-  // from 64 rows on the parts to exchange weigh more: 128 rows, 56 tiles: 15.7 / 17.2 with 2 / 3; 32 tiles: 21.2 / 24.0 with 4 / 5.
-  p.split = (p.nt <= 32 ? 176 : 132) / tiles;
-  if (p.split > kNwMaxSplit) p.split = kNwMaxSplit;
-  if (p.split > p.num_kb / 2) p.split = p.num_kb / 2;
-  if (p.split < 1) p.split = 1;
-  p.stages = (kNwSmemTarget - 1024 - kNwCtrlBytes) / dense_narrow_stage_bytes(p.nt);
+  p.nt = plan.nt;
+  p.split = plan.split;
+  p.row_tiles = plan.row_tiles;
+  p.col_tiles = plan.col_tiles;
+  const bool wide = plan.nt > 64;
+  const int recv = dense_narrow_recv_bytes(p.nt, p.split);
+  const bool alone = wide || plan.row_tiles * plan.col_tiles * plan.split <= kClusterRoom[plan.split];
+  p.stages = (dense_narrow_smem(alone) - 1024 - kNwCtrlBytes - recv) / dense_narrow_stage_bytes(p.nt);
   if (p.stages > kNwMaxStages) p.stages = kNwMaxStages;
   p.a_mn = w.mn;
-  p.b_mn = 0;
-  p.idesc = ptx::idesc_f16(128, p.nt, dtype == TAB_BF16 ? 1 : 0, w.mn, 0);
+  p.b_mn = x.mn;
+  p.idesc = ptx::idesc_f16(128, p.nt, dtype == TAB_BF16 ? 1 : 0, w.mn, x.mn);
   p.wait_cycles = dense_wait_cycles();
   CUtensorMap mw, mx;
   int rc = make_map(op, w, 64, &mw);
-  if (rc == TAB_OK) rc = make_map(op, x, p.nt, &mx);
+  if (rc == TAB_OK) rc = make_map(op, x, x.mn ? 64 : p.nt, &mx);
   if (rc != TAB_OK) return rc;
-  return dtype == TAB_BF16 ? launch_narrow_t<__nv_bfloat16, EPI>(op, mw, mx, p, tiles, st)
-                           : launch_narrow_t<__half, EPI>(op, mw, mx, p, tiles, st);
+  if (dtype == TAB_BF16)
+    return wide ? launch_narrow_t<__nv_bfloat16, EPI, true>(op, mw, mx, p, st) : launch_narrow_t<__nv_bfloat16, EPI, false>(op, mw, mx, p, st);
+  return wide ? launch_narrow_t<__half, EPI, true>(op, mw, mx, p, st) : launch_narrow_t<__half, EPI, false>(op, mw, mx, p, st);
 }
-static_assert(kNwMaxTokens * 128 * 4 <= 3 * dense_narrow_stage_bytes(kNwMaxTokens), "the parts of a tile overlay the ring");
-static_assert(1024 + 3 * dense_narrow_stage_bytes(kNwMaxTokens) + kNwCtrlBytes <= kNwSmemTarget, "three stages at the widest tile");
+constexpr bool narrow_fits(int nt, int split, int stages) {     // that many stages, and the parts of a tile overlay them
+  return 1024 + stages * dense_narrow_stage_bytes(nt) + kNwCtrlBytes + dense_narrow_recv_bytes(nt, split) <= dense_narrow_smem(nt > 64) &&
+         nt * 512 <= stages * dense_narrow_stage_bytes(nt);
+}
+static_assert(narrow_fits(16, kNwMaxSplit, 5) && narrow_fits(32, kNwMaxSplit, 4) && narrow_fits(64, kNwMaxSplit, 3) &&
+              narrow_fits(128, kNwMaxSplit, 4) && narrow_fits(256, 1, 4), "shared memory of the narrow kernel");
+
+// Which kernel: the one with the lower estimate.
+template <int EPI>
+static int launch_dense(const char* op, int dtype, const DenseOperand& a, const DenseOperand& b, DenseParams& p, cudaStream_t st) {
+  const int num_kb = (int)((a.depth + kDnBlockK - 1) / kDnBlockK);
+  const NarrowPlan plan = narrow_plan(p.M, p.N, num_kb, EPI, a.mn != 0);
+  if (plan.nt != 0 && plan.cost <= pair_cost(p.M, p.N, num_kb, EPI, dense_sms() / 2)) return launch_narrow_epi<EPI>(op, dtype, a, b, p, plan, st);
+  return launch_pair_epi<EPI>(op, dtype, a, b, p, st);
+}
 
 // ---- checks ----
 static int check_dense(const char* op, int dtype, int64_t M, int64_t N, int64_t K, int act) {
@@ -262,8 +326,7 @@ static int gated_matmul(const char* op, const DenseOperand& x, const DenseOperan
   p.keep_scale = keep_scale;
   p.keep_ld = (int)keep_ld;
   p.keep_up = (int)(keep_q ? up64(I) : I);
-  if (use_narrow(M, x)) return launch_narrow_epi<kEpiGlu>(op, dtype, x, w, p, st);
-  return launch_pair_epi<kEpiGlu>(op, dtype, x, w, p, st);
+  return launch_dense<kEpiGlu>(op, dtype, x, w, p, st);
 }
 
 static int linear_matmul(const char* op, const DenseOperand& a, const DenseOperand& b, int dtype, int64_t M, int64_t N, const void* bias,
@@ -281,8 +344,7 @@ static int linear_matmul(const char* op, const DenseOperand& a, const DenseOpera
   p.keep_scale = keep_scale;
   p.keep_ld = (int)keep_ld;
   p.dependent = dependent;
-  if (use_narrow(M, a)) return launch_narrow_epi<kEpiLinear>(op, dtype, a, b, p, st);
-  return launch_pair_epi<kEpiLinear>(op, dtype, a, b, p, st);
+  return launch_dense<kEpiLinear>(op, dtype, a, b, p, st);
 }
 
 }  // namespace tab
@@ -337,7 +399,7 @@ extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* w
   p.keep_scale = const_cast<float*>(keep_scale);
   p.keep_ld = (int)keep_ld;
   p.keep_up = (int)(keep_q ? up64(I) : I);
-  return launch_pair_epi<kEpiGluGrad>(op, dtype, oa, ow, p, as_stream(stream));
+  return launch_dense<kEpiGluGrad>(op, dtype, oa, ow, p, as_stream(stream));
 }
 
 extern "C" int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes) {

@@ -1,12 +1,19 @@
-// Dense 16-bit GEMM for few rows (decode): out[m, n] = sum_k x[m, k] W[k, n] with at most 128 rows, weights streamed once.
+// Dense 16-bit GEMM for few rows or few tiles: out[m, n] = sum_k x[m, k] W[k, n] in tiles of 128 output features x NT rows, one CTA
+// or one cluster to a tile.
 //
-// What bounds it: the bytes of W.  The weights are the stationary 128-row operand of tcgen05.mma (128 output features; for the
-// gated form 64 gate features and the matching 64 up features), the rows of x its narrow N operand (16 .. 128 columns), so
-// no MMA work is padded beyond 16 rows.  One tile of 128 features holds far too little work for an SM when N is a few
-// thousand: a cluster of `split` CTAs shares a tile, each taking a part of the contraction.  The parts meet in distributed
-// shared memory: every CTA leaves its fp32 accumulators in its own shared memory, and after a cluster barrier each CTA adds
-// up, in the order of the contraction, the groups of 64 features that are its to finish, and runs the epilogue on them.  No
-// workspace, no atomics, the same bits every time.  Two CTAs share an SM, each with a ring of about 100 KB.
+// The features are the stationary 128-row operand of tcgen05.mma (for the gated form 64 gate features and the matching 64 up
+// features), the rows of x its narrow N operand (NT = 16 .. 256 columns): a decode batch pads no MMA work beyond 16 rows, and the
+// weights stream from HBM once.  What bounds it: the bytes of W for a handful of rows, the operand bytes from L2 (NT = 128: 32 KB per
+// 256 tensor cycles) where there are many; the pair kernel needs half of those, but only 74 tiles of its 256 x 256 fill the GPU.
+//
+// One tile holds too little work for an SM when there are few: a cluster of `split` CTAs shares it, each taking a part of the
+// contraction.  The parts meet in distributed shared memory: every CTA copies the rows of its fp32 accumulators to the CTAs that
+// finish them (one bulk copy each, counted on a barrier of the receiver), which add them in the order of the contraction and
+// run the epilogue.  No workspace, no atomics, the same bits every time.  Cluster barriers are only arrived at early and
+// waited for late; reading the parts remotely between two full barriers cost some 2 us more per launch.
+//
+// A launch of this kernel is over in 5 to 15 us, so its start counts: the producer sets up its barriers and asks for the first
+// weights before the CTA's threads have met and tensor memory is allocated.
 //
 // A launch marked `dependent` (the second projection of a feed-forward block) may start while the kernel before it still
 // runs: it fills its ring with weights first and waits for that kernel only before it touches x.
@@ -16,34 +23,33 @@
 
 namespace tab {
 
-constexpr int kNwThreads = 192;               // producer warp, MMA warp, 4 warps that empty tensor memory; all of them add up
-constexpr int kNwMaxTokens = 128;
-constexpr int kNwMaxStages = 8;
+constexpr int kNwMaxTokens = 256;
+constexpr int kNwMaxStages = 12;
 constexpr int kNwCtrlBytes = 256;
-constexpr int kNwSmemTarget = 113 * 1024;     // two CTAs per SM
 constexpr int kNwMaxSplit = 8;
 
+// Up to 64 rows two CTAs may share an SM, each with a ring of about 110 KB: the one streams weights while the other is in its
+// prologue or epilogue.  A CTA that has its SM to itself (wider tiles, or no more CTAs than SMs) takes all of the shared memory:
+// a block of the contraction then takes some 550 cycles with five stages of 20 KB in flight, less with eleven.
+__host__ __device__ constexpr int dense_narrow_threads(bool wide) { return wide ? 320 : 192; }
+__host__ __device__ constexpr int dense_narrow_smem(bool alone) { return alone ? kDnSmemLimit : 113 * 1024; }
 __host__ __device__ constexpr int dense_narrow_stage_bytes(int nt) { return kDnOperandBytes + nt * 128; }
+// where a CTA of a cluster receives the parts of the rows that it finishes: rows x 128 fp32 of a tile in all, up to one more
+// group of 64 or 128 from each of the CTAs where the rows do not divide evenly
+__host__ __device__ constexpr int dense_narrow_recv_bytes(int nt, int split) { return split > 1 ? (nt + split) * 512 : 0; }
 
-// 8 consecutive features of one token, summed over the cluster in rank order
-__device__ __forceinline__ void sum_parts8(uint32_t part_addr, int token, int feature, int split, float (&v)[8]) {
-  const uint32_t off = part_addr + static_cast<uint32_t>(token * 128 + feature) * 4u;
-  float4 a[kNwMaxSplit], b[kNwMaxSplit];
-#pragma unroll
-  for (int r = 0; r < kNwMaxSplit; ++r)
-    if (r < split) {
-      const uint32_t at = ptx::mapa(off, static_cast<uint32_t>(r));
-      a[r] = ptx::ld_cluster_f4(at);
-      b[r] = ptx::ld_cluster_f4(at + 16);
-    }
-  v[0] = a[0].x; v[1] = a[0].y; v[2] = a[0].z; v[3] = a[0].w;
-  v[4] = b[0].x; v[5] = b[0].y; v[6] = b[0].z; v[7] = b[0].w;
-#pragma unroll
-  for (int r = 1; r < kNwMaxSplit; ++r)
-    if (r < split) {
-      v[0] += a[r].x; v[1] += a[r].y; v[2] += a[r].z; v[3] += a[r].w;
-      v[4] += b[r].x; v[5] += b[r].y; v[6] += b[r].z; v[7] += b[r].w;
-    }
+// 8 consecutive fp32 values at `src` of the first part, summed over the parts in order
+__device__ __forceinline__ void sum_parts8(const float* src, int part_floats, int parts, float (&v)[8]) {
+  float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+#pragma unroll 1
+  for (int r = 1; r < parts; ++r) {
+    src += part_floats;
+    const float4 c = *reinterpret_cast<const float4*>(src), d = *reinterpret_cast<const float4*>(src + 4);
+    a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+    b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+  }
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
 template <typename T>
@@ -77,67 +83,111 @@ __device__ __forceinline__ void keep8(const DenseParams& p, const float (&v)[8],
   }
 }
 
-template <typename T, int EPI>
-__global__ void __launch_bounds__(kNwThreads, 2)
+// 8 kept values of a row
+template <typename T>
+__device__ __forceinline__ void kept8(const DenseParams& p, int64_t row, int col, float (&v)[8]) {
+  if (p.keep_q != nullptr) {
+    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p.keep_q + row * p.keep_ld + col));
+    const float s = __ldg(p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int8_t>(j < 4 ? q.x >> (8 * j) : q.y >> (8 * j - 32))) * s;
+  } else {
+    Elem<T>::load8(static_cast<const T*>(p.keep) + row * p.keep_ld + col, v);
+  }
+}
+
+template <typename T, int EPI, bool WIDE>
+__global__ void __launch_bounds__(dense_narrow_threads(WIDE), WIDE ? 1 : 2)
 dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const DenseParams p) {
+  constexpr int kThreads = dense_narrow_threads(WIDE);
+  constexpr int kTmemCols = WIDE ? 256 : 64;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = ptx::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
   const uint32_t tiles_addr = ptx::smem_u32(smem);
   const int stage_bytes = dense_narrow_stage_bytes(p.nt);
   uint8_t* ctrl = smem + p.stages * stage_bytes;
+  float* recv = reinterpret_cast<float*>(ctrl + kNwCtrlBytes);         // parts of this CTA's groups, one after another
   const uint32_t bar0 = ptx::smem_u32(ctrl);
   auto bar_full = [&](int s) { return bar0 + 8u * s; };
   auto bar_empty = [&](int s) { return bar0 + 8u * (kNwMaxStages + s); };
   const uint32_t bar_tfull = bar0 + 8u * (2 * kNwMaxStages);
-  static_assert(8 * (2 * kNwMaxStages + 1) <= 224, "barriers overflow the control block");
+  const uint32_t bar_recv = bar_tfull + 8u;
+  static_assert(8 * (2 * kNwMaxStages + 2) <= 224 && 2 * kNwMaxStages + 2 <= 32, "barriers: one per lane, ahead of the control words");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(ctrl + 224);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  float* part = reinterpret_cast<float*>(smem);          // [tokens][128], over the stages once the MMAs are done
+  float* part = reinterpret_cast<float*>(smem);          // [rows][128], over the stages once the MMAs are done
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(ptx::cluster_ctarank());
-  const int tile = blockIdx.x / p.split;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * p.num_kb / p.split);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * p.num_kb / p.split);
+  const int split = p.split;
+  const int rank = split > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const int tile = blockIdx.x / split;
+  const int ft = tile / p.row_tiles;                     // CTAs that follow one another read the same features
+  const int row0 = (tile - ft * p.row_tiles) * p.nt;
+  const int rows = min(p.nt, p.M - row0);
+  const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * p.num_kb / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * p.num_kb / split);
   const int n_kb = kb1 - kb0;                            // >= 1: the host keeps split <= num_kb
+  const int head = min(p.stages, n_kb);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      ptx::mbar_init(bar_full(s), 1);
-      ptx::mbar_init(bar_empty(s), 1);
+  // groups of 64 output features of one row; CTA r finishes groups [r G / split, (r + 1) G / split)
+  constexpr int kGroups = EPI == kEpiGlu ? 1 : 2;        // per row
+  constexpr int kGroupFloats = 128 / kGroups;            // accumulators of a group (gate and up together)
+  const int groups = rows * kGroups;
+  auto group_begin = [&](int r) { return r * groups / split; };
+
+  const int f0 = EPI == kEpiGlu ? ft * 64 : ft * 128;
+  const int f1 = EPI == kEpiGlu ? p.N + f0 : f0 + 64;
+  auto load_w = [&](int s, int kb) {                     // by the elected lane of the producer warp
+    const uint32_t st = tiles_addr + s * stage_bytes;
+    const int k = kb * kDnBlockK;
+    ptx::mbar_expect_tx(bar_full(s), static_cast<uint32_t>(stage_bytes));
+    ptx::tma_load_2d(st, &tm_w, bar_full(s), p.a_mn ? f0 : k, p.a_mn ? k : f0);
+    ptx::tma_load_2d(st + kDnBoxBytes, &tm_w, bar_full(s), p.a_mn ? f1 : k, p.a_mn ? k : f1);
+  };
+  auto load_x = [&](int s, int kb) {
+    const uint32_t st = tiles_addr + s * stage_bytes + kDnOperandBytes;
+    if (p.b_mn) {                                        // 64 rows per box
+      for (int r = 0; r < p.nt; r += 64) ptx::tma_load_2d(st + r * 128, &tm_x, bar_full(s), row0 + r, kb * kDnBlockK);
+    } else {
+      ptx::tma_load_2d(st, &tm_x, bar_full(s), kb * kDnBlockK, row0);
     }
-    ptx::mbar_init(bar_tfull, 1);
-    *s_abort = 0;
+  };
+
+  if (warp == 0) {
+    if (lane < 2 * kNwMaxStages + 2) ptx::mbar_init(bar0 + 8u * lane, 1);
+    if (lane == 0) *s_abort = 0;
     ptx::fence_barrier_init();
-    ptx::prefetch_tensormap(&tm_w);
-    ptx::prefetch_tensormap(&tm_x);
+    __syncwarp();
+    if (ptx::elect_one()) {
+      const int mine = group_begin(rank + 1) - group_begin(rank);
+      if (split > 1 && mine > 0) ptx::mbar_expect_tx(bar_recv, static_cast<uint32_t>(mine * split * kGroupFloats * 4));
+      for (int i = 0; i < min(head, 2); ++i) load_w(i, kb0 + i);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    ptx::tmem_alloc<kTmemCols>(ptx::smem_u32(s_tmem));
   }
-  if (warp == 1) ptx::tmem_alloc<kNwMaxTokens>(ptx::smem_u32(s_tmem));
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
+  if (split > 1) ptx::cluster_arrive();                  // this CTA runs and its barriers exist
   const uint32_t tmem_base = *s_tmem;
   ptx::launch_dependents();
 
   if (warp == 0) {
-    const int f0 = EPI == kEpiGlu ? tile * 64 : tile * 128;
-    const int f1 = EPI == kEpiGlu ? p.N + f0 : f0 + 64;
-    auto load_w = [&](int s, int kb) {                   // by the elected lane
-      const uint32_t st = tiles_addr + s * stage_bytes;
-      const int k = kb * kDnBlockK;
-      ptx::mbar_expect_tx(bar_full(s), static_cast<uint32_t>(stage_bytes));
-      ptx::tma_load_2d(st, &tm_w, bar_full(s), p.a_mn ? f0 : k, p.a_mn ? k : f0);
-      ptx::tma_load_2d(st + kDnBoxBytes, &tm_w, bar_full(s), p.a_mn ? f1 : k, p.a_mn ? k : f1);
-    };
-    auto load_x = [&](int s, int kb) {
-      ptx::tma_load_2d(tiles_addr + s * stage_bytes + kDnOperandBytes, &tm_x, bar_full(s), kb * kDnBlockK, 0);
-    };
-    const int head = min(p.stages, n_kb);
     if (ptx::elect_one()) {
-      for (int i = 0; i < head; ++i) load_w(i, kb0 + i);
-      ptx::dependency_wait();
-      for (int i = 0; i < head; ++i) load_x(i, kb0 + i);
+      if (!p.dependent) {                                // nothing to wait for: the first blocks' rows before the later weights
+        for (int i = 0; i < min(head, 2); ++i) load_x(i, kb0 + i);
+        for (int i = 2; i < head; ++i) {
+          load_w(i, kb0 + i);
+          load_x(i, kb0 + i);
+        }
+      } else {
+        for (int i = 2; i < head; ++i) load_w(i, kb0 + i);
+        ptx::dependency_wait();
+        for (int i = 0; i < head; ++i) load_x(i, kb0 + i);
+      }
     }
     __syncwarp();
     int stage = 0;
@@ -155,17 +205,17 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const uint32_t a_step = p.a_mn ? 128u : 2u;
+    const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;
     for (int i = 0; i < n_kb; ++i) {
       ok = __all_sync(0xffffffffu, dense_wait(bar_full(stage), phase, s_abort, 42, p.wait_cycles));
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t st = tiles_addr + stage * stage_bytes;
       const uint64_t a = p.a_mn ? ptx::smem_desc_mn128(st, kDnBoxBytes) : ptx::smem_desc_k128(st);
-      const uint64_t b = ptx::smem_desc_k128(st + kDnOperandBytes);
+      const uint64_t b = p.b_mn ? ptx::smem_desc_mn128(st + kDnOperandBytes, kDnBoxBytes) : ptx::smem_desc_k128(st + kDnOperandBytes);
       if (ptx::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kDnBlockK / 16; ++k) ptx::mma_f16(tmem_base, a + k * a_step, b + k * 2, p.idesc, (i | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < kDnBlockK / 16; ++k) ptx::mma_f16(tmem_base, a + k * a_step, b + k * b_step, p.idesc, (i | k) != 0 ? 1u : 0u);
         ptx::mma_commit(bar_empty(stage));
       }
       __syncwarp();
@@ -184,72 +234,126 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     __syncwarp();
     if (__all_sync(0xffffffffu, got)) {
       ptx::tc_fence_after();
-      const int quarter = warp & 3;
+      const int quarter = warp & 3, group = (warp - 2) >> 2;       // warps of one lane quarter take the 16-row steps in turn
       const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = 0; c < p.M; c += 16) {
-        int v[16];
+      for (int c = group * 16; c < rows; c += (kThreads / 32 - 2) / 4 * 16) {
+        float v[16];
         __syncwarp();
-        ptx::tmem_ld16(t0 + c, v);
+        ptx::tmem_ld16f(t0 + c, v);
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (c + j < p.M) part[(c + j) * 128 + quarter * 32 + lane] = __int_as_float(v[j]);
+          if (c + j < rows) part[(c + j) * 128 + quarter * 32 + lane] = v[j];
       }
     }
     ptx::tc_fence_before();
+    if (split > 1) ptx::fence_async_shared();            // the copies below read what this thread wrote
   }
   __syncthreads();
-  ptx::cluster_sync_all();            // every CTA's part is in place
 
-  // ---- add up and finish: groups of 64 output features of one token, 8 lanes x 8 features each ----
-  constexpr int kGroupsPerToken = EPI == kEpiGlu ? 1 : 2;
-  const int groups = p.M * kGroupsPerToken;
-  const int g_begin = static_cast<int>(static_cast<int64_t>(rank) * groups / p.split);
-  const int g_end = static_cast<int>(static_cast<int64_t>(rank + 1) * groups / p.split);
-  const uint32_t part_addr = tiles_addr;
-  for (int g0 = g_begin; g0 < g_end; g0 += kNwThreads / 8) {
+  // ---- the parts go to the CTAs that finish their rows ----
+  const int g_begin = group_begin(rank), g_end = group_begin(rank + 1);
+  const int part_floats = split > 1 ? (g_end - g_begin) * kGroupFloats : 0;
+  const float* sums = part;                              // first of this CTA's groups in the first part
+  if (split > 1) {
+    ptx::cluster_wait();                                 // every CTA of the cluster runs
+    if (warp == 0 && lane < split) {
+      const int b = group_begin(lane), n = group_begin(lane + 1) - b;
+      if (n > 0)
+        ptx::copy_to_cluster(ptx::mapa(ptx::smem_u32(recv) + static_cast<uint32_t>(rank * n * kGroupFloats * 4), static_cast<uint32_t>(lane)),
+                             tiles_addr + static_cast<uint32_t>(b * kGroupFloats * 4), static_cast<uint32_t>(n * kGroupFloats * 4),
+                             ptx::mapa(bar_recv, static_cast<uint32_t>(lane)));
+    }
+    __syncwarp();
+    if (part_floats > 0) dense_wait(bar_recv, 0, s_abort, 44, p.wait_cycles);
+    sums = recv;
+    __syncthreads();
+    ptx::cluster_arrive();                               // what was sent here has arrived: the senders may leave
+  }
+
+  // ---- add up and finish: 8 lanes x 8 features to a group ----
+  const bool has_bias = p.bias != nullptr, has_res = p.residual != nullptr, keeps = p.keep != nullptr || p.keep_q != nullptr;
+  const int act = p.act;
+  const int64_t ld = p.N;
+  const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual);
+  T* out = static_cast<T*>(p.out);
+  const int lane8 = (threadIdx.x & 7) * 8;
+#pragma unroll 2
+  for (int g0 = g_begin; g0 < g_end; g0 += kThreads / 8) {
     const int g = g0 + static_cast<int>(threadIdx.x >> 3);
     const bool mine = g < g_end;
-    const int token = mine ? g / kGroupsPerToken : 0;
-    const int in_tile = (mine ? g % kGroupsPerToken : 0) * 64 + (threadIdx.x & 7) * 8;
-    const int col = tile * (EPI == kEpiGlu ? 64 : 128) + in_tile;
+    const int64_t row = row0 + (mine ? g / kGroups : 0);
+    const int col = ft * (EPI == kEpiGlu ? 64 : 128) + (mine ? g % kGroups : 0) * 64 + lane8;
     const bool in = mine && col < p.N;
-    const bool live = mine && (col & ~63) < p.N;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (in) {
-      sum_parts8(part_addr, token, in_tile, p.split, v);
-      if (p.bias != nullptr) add8(v, static_cast<const T*>(p.bias) + col);
-    }
-    keep8<T>(p, v, token, col, in, live);
-    if constexpr (EPI == kEpiGlu) {
-      float u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float* src = sums + (mine ? g - g_begin : 0) * kGroupFloats + lane8;
+    float v[8];
+    if constexpr (EPI == kEpiGluGrad) {
       if (in) {
-        sum_parts8(part_addr, token, 64 + in_tile, p.split, u);
-        if (p.bias != nullptr) add8(u, static_cast<const T*>(p.bias) + p.N + col);
-      }
-      keep8<T>(p, u, token, p.keep_up + col, in, live);
-      with_act(p.act, [&](auto tag) {
+        float gate[8], up[8];
+        kept8<T>(p, row, col, gate);
+        kept8<T>(p, row, p.keep_up + col, up);
+        sum_parts8(src, part_floats, split, v);
+        // h = a u, d(gate) = dh u a', d(up) = dh a; gate, up and v are overwritten in turn
+        with_act(act, [&](auto tag) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]) * u[i];
-      });
-    } else if (p.act != TAB_ACT_NONE) {
-      with_act(p.act, [&](auto tag) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]);
-      });
-    }
-    if (in) {
-      const int64_t at = static_cast<int64_t>(token) * p.N + col;
-      if constexpr (EPI == kEpiLinear) {
-        if (p.residual != nullptr) add8(v, static_cast<const T*>(p.residual) + at);
+          for (int i = 0; i < 8; ++i) {
+            float a, d;
+            act_both<decltype(tag)::value>(gate[i], a, d);
+            const float h = a * up[i];
+            gate[i] = v[i] * up[i] * d;
+            up[i] = v[i] * a;
+            v[i] = h;
+          }
+        });
+        T* dz = static_cast<T*>(p.dgate) + row * 2 * ld + col;
+        Elem<T>::store8(dz, gate);
+        Elem<T>::store8(dz + p.N, up);
+        Elem<T>::store8(out + row * ld + col, v);
       }
-      Elem<T>::store8(static_cast<T*>(p.out) + at, v);
+    } else {
+      float u[8], r[8];
+      if (in) {
+        const int64_t at = row * ld + col;
+        if (EPI == kEpiLinear && has_res) Elem<T>::load8(res + at, r);
+        sum_parts8(src, part_floats, split, v);
+        if (has_bias) add8(v, bias + col);
+        if constexpr (EPI == kEpiGlu) {
+          sum_parts8(src + 64, part_floats, split, u);
+          if (has_bias) add8(u, bias + p.N + col);
+        }
+      }
+      if (keeps) {
+        const bool live = mine && (col & ~63) < p.N;
+        keep8<T>(p, v, row, col, in, live);
+        if constexpr (EPI == kEpiGlu) keep8<T>(p, u, row, p.keep_up + col, in, live);
+      }
+      if (in) {
+        if constexpr (EPI == kEpiGlu) {
+          with_act(act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]) * u[i];
+          });
+        } else if (act != TAB_ACT_NONE) {
+          with_act(act, [&](auto tag) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]);
+          });
+        }
+        if (EPI == kEpiLinear && has_res) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += r[i];
+        }
+        Elem<T>::store8(out + row * ld + col, v);
+      }
     }
   }
-  ptx::cluster_sync_all();            // no CTA leaves while another still reads its part
+  if (split > 1) {
+    __syncwarp();
+    ptx::cluster_wait();              // what this CTA sent has arrived
+  }
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc<kNwMaxTokens>(tmem_base);
+    ptx::tmem_dealloc<kTmemCols>(tmem_base);
   }
 }
 
