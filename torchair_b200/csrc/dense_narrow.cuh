@@ -175,51 +175,62 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   const uint32_t tmem_base = *s_tmem;
   ptx::launch_dependents();
 
-  if (warp == 0) {
+  // Two producer warps (the second is one that has nothing to do before the epilogue) take the blocks in turn: one alone needs
+  // some 400 cycles for a block's wait and copies, more than the bytes do.
+  if (warp == 0 || warp == 2) {
+    const int odd = warp >> 1;
     if (ptx::elect_one()) {
-      if (!p.dependent) {                                // nothing to wait for: the first blocks' rows before the later weights
-        for (int i = 0; i < min(head, 2); ++i) load_x(i, kb0 + i);
-        for (int i = 2; i < head; ++i) {
-          load_w(i, kb0 + i);
-          load_x(i, kb0 + i);
-        }
-      } else {
-        for (int i = 2; i < head; ++i) load_w(i, kb0 + i);
+      if (!p.dependent && odd < head) load_x(odd, kb0 + odd);
+      for (int i = 2 + odd; i < head; i += 2) {
+        load_w(i, kb0 + i);
+        if (!p.dependent) load_x(i, kb0 + i);
+      }
+      if (p.dependent) {
         ptx::dependency_wait();
-        for (int i = 0; i < head; ++i) load_x(i, kb0 + i);
+        for (int i = odd; i < head; i += 2) load_x(i, kb0 + i);
       }
     }
     __syncwarp();
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int i = head; i < n_kb; ++i) {
-      if (!__all_sync(0xffffffffu, dense_wait(bar_empty(stage), phase, s_abort, 41, p.wait_cycles))) break;
-      if (ptx::elect_one()) {
-        load_w(stage, kb0 + i);
-        load_x(stage, kb0 + i);
+    int i = odd, stage = odd;
+    uint32_t phase = 1;                                  // of the first use; later ones wait for the MMAs of the use before
+    while (stage >= p.stages) stage -= p.stages;
+    for (; i < n_kb; i += 2) {
+      if (i >= head) {
+        if (!__all_sync(0xffffffffu, dense_wait(bar_empty(stage), phase, s_abort, 41, p.wait_cycles))) break;
+        if (ptx::elect_one()) {
+          load_w(stage, kb0 + i);
+          load_x(stage, kb0 + i);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      stage += 2;
+      if (stage >= p.stages) { stage -= p.stages; phase ^= 1u; }
     }
+  }
+  if (warp == 0) {
+    // nothing until the parts are exchanged
   } else if (warp == 1) {
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u;
+    const uint32_t a_step = p.a_mn ? 128u : 2u, b_step = p.b_mn ? 128u : 2u, idesc = p.idesc;
+    const uint64_t a_first = p.a_mn ? ptx::smem_desc_mn128(tiles_addr, kDnBoxBytes) : ptx::smem_desc_k128(tiles_addr);
+    const uint64_t b_first = p.b_mn ? ptx::smem_desc_mn128(tiles_addr + kDnOperandBytes, kDnBoxBytes) : ptx::smem_desc_k128(tiles_addr + kDnOperandBytes);
+    const uint32_t stage_step = static_cast<uint32_t>(stage_bytes) >> 4;
+    uint32_t off = 0;
     for (int i = 0; i < n_kb; ++i) {
       ok = __all_sync(0xffffffffu, dense_wait(bar_full(stage), phase, s_abort, 42, p.wait_cycles));
       if (!ok) break;
       ptx::tc_fence_after();
-      const uint32_t st = tiles_addr + stage * stage_bytes;
-      const uint64_t a = p.a_mn ? ptx::smem_desc_mn128(st, kDnBoxBytes) : ptx::smem_desc_k128(st);
-      const uint64_t b = p.b_mn ? ptx::smem_desc_mn128(st + kDnOperandBytes, kDnBoxBytes) : ptx::smem_desc_k128(st + kDnOperandBytes);
       if (ptx::elect_one()) {
+        const uint64_t a = a_first + off, b = b_first + off;
 #pragma unroll
-        for (int k = 0; k < kDnBlockK / 16; ++k) ptx::mma_f16(tmem_base, a + k * a_step, b + k * b_step, p.idesc, (i | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < kDnBlockK / 16; ++k) ptx::mma_f16(tmem_base, a + k * a_step, b + k * b_step, idesc, (i | k) != 0 ? 1u : 0u);
         ptx::mma_commit(bar_empty(stage));
       }
       __syncwarp();
-      if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      off += stage_step;
+      if (++stage == p.stages) { stage = 0; phase ^= 1u; off = 0; }
     }
     // also after a wait that gave up: the barrier then says that no MMA is in flight any more
     if (ptx::elect_one()) ptx::mma_commit(bar_tfull);
