@@ -736,7 +736,7 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     one, n, odd = ctypes.c_void_p(256), ctypes.c_void_p(None), ctypes.c_void_p(260)
     mat = lambda **kw: [kw.get("a", one), kw.get("lda", 64), 0, kw.get("b", one), kw.get("ldb", 64), 0, kw.get("dtype", 15), kw.get("M", 4),  # noqa: E731
                         kw.get("N", 64), kw.get("K", 64), kw.get("bias", n), n, kw.get("act", 0), kw.get("keep", n), kw.get("keep_q", n),
-                        kw.get("keep_scale", n), kw.get("keep_ld", 0), kw.get("out", one), n]
+                        kw.get("keep_scale", n), kw.get("keep_ld", 0), kw.get("out", one), 0, n]
     for kw, match in ((dict(a=n), "null"), (dict(dtype=6), "dtype"), (dict(N=60), "multiple of 8"), (dict(lda=63), "multiple of 8"),
                       (dict(lda=56), "shorter"), (dict(ldb=32), "shorter"), (dict(act=9), "activation"), (dict(K=0), "K=0"),
                       (dict(M=-1), "M=-1"), (dict(out=n), "null output"), (dict(a=odd), "aligned"), (dict(bias=odd), "aligned"),

@@ -148,7 +148,8 @@ static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMa
     p.tile_begin = 0;
     p.tile_end = (int)whole;
     p.split = 1;
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes<EPI>, 2, false, ma, mb, p, st);
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes<EPI>, 2, p.beside != 0, ma,
+                        mb, p, st);
     if (rc != TAB_OK) return rc;
   }
   if (rest > 0) {
@@ -157,7 +158,8 @@ static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMa
     p.tile_end = (int)tiles;
     p.split = split;
     // both launches read the same operands and write different tiles: the second may fill SMs that the first has left
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes<EPI>, 2 * split, whole > 0, ma, mb, p, st);
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes<EPI>, 2 * split, whole > 0 || p.beside != 0, ma, mb,
+                        p, st);
   }
   return rc;
 }
@@ -241,7 +243,7 @@ static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensor
   const int rc = allow_smem(op, dense_narrow_kernel<T, EPI, WIDE>, dense_narrow_smem(true), done);
   if (rc != TAB_OK) return rc;
   return launch_cluster(op, dense_narrow_kernel<T, EPI, WIDE>, p.row_tiles * p.col_tiles * p.split, dense_narrow_threads(WIDE), smem, p.split,
-                        p.dependent != 0, mw, mx, p, st);
+                        p.dependent != 0 || p.beside != 0, mw, mx, p, st);
 }
 
 template <int EPI>
@@ -331,7 +333,7 @@ static int gated_matmul(const char* op, const DenseOperand& x, const DenseOperan
 
 static int linear_matmul(const char* op, const DenseOperand& a, const DenseOperand& b, int dtype, int64_t M, int64_t N, const void* bias,
                          const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* out, int dependent,
-                         cudaStream_t st) {
+                         int beside, cudaStream_t st) {
   DenseParams p = {};
   p.M = (int)M;
   p.N = (int)N;
@@ -344,6 +346,7 @@ static int linear_matmul(const char* op, const DenseOperand& a, const DenseOpera
   p.keep_scale = keep_scale;
   p.keep_ld = (int)keep_ld;
   p.dependent = dependent;
+  p.beside = beside;
   return launch_dense<kEpiLinear>(op, dtype, a, b, p, st);
 }
 
@@ -353,7 +356,7 @@ using namespace tab;
 
 extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M, int64_t N,
                                 int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q, float* keep_scale,
-                                int64_t keep_ld, void* out, tab_stream_t stream) {
+                                int64_t keep_ld, void* out, int beside_previous, tab_stream_t stream) {
   const char* op = "dense_matmul";
   int rc = check_dense(op, dtype, M, N, K, act);
   if (rc != TAB_OK || M == 0) return rc;
@@ -361,7 +364,8 @@ extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void
   if ((rc = check_operand(op, "a", oa)) != TAB_OK || (rc = check_operand(op, "b", ob)) != TAB_OK) return rc;
   if ((rc = check_epilogue_ptrs(op, bias, residual, out)) != TAB_OK) return rc;
   if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, keep_q ? up64(N) : N)) != TAB_OK) return rc;
-  return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0, as_stream(stream));
+  return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0,
+                       beside_previous ? 1 : 0, as_stream(stream));
 }
 
 extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
@@ -429,7 +433,7 @@ extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t
   rc = gated_matmul(op, ox, o1, dtype, M, I, bias1, act, keep, keep_q, keep_scale, keep_ld, workspace, st);
   if (rc != TAB_OK) return rc;
   const DenseOperand oh = {workspace, I, M, I, 0};
-  return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, st);
+  return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, 0, st);
 }
 
 extern "C" int tab_dense_status_reset(tab_stream_t stream) {

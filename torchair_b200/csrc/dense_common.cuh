@@ -47,6 +47,7 @@ struct DenseParams {
   int split;             // CTAs (dense_pair.cuh: pairs) of a cluster that share one tile's contraction
   int stages, nt;        // dense_narrow.cuh: shared-memory stages, token columns of a tile
   int dependent;         // launched as dependent of the kernel that writes the token operand
+  int beside;            // may run beside the launch before it
   long long wait_cycles;
 };
 

@@ -366,6 +366,8 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     ptx::tc_fence_after();
     ptx::tmem_dealloc<kTmemCols>(tmem_base);
   }
+  // a launch that was allowed to start under the one before it ends only after that one has
+  if (threadIdx.x == 0) ptx::dependency_wait();
 }
 
 }  // namespace tab

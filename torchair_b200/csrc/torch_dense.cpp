@@ -187,23 +187,23 @@ struct Kept {
 
 // act(a b^T + bias) + residual: a [m, k], b [n, k] as operands
 void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int64_t m, int64_t n, int64_t k, const Tensor& out,
-            const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept()) {
+            const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept(), bool beside = false) {
   c.flush();
   ok(tab_dense_matmul(a, lda, a_mn, b, ldb, b_mn, c.dtype, m, n, k, ptr(bias), ptr(residual), act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
-                      out.data_ptr(), c.stream),
+                      out.data_ptr(), beside, c.stream),
      "tab_dense_matmul");
 }
 
 // x^T dz [k, n] (both row-major), in the memory order of the weight `like`
-Tensor weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_t n, const Tensor& like) {
+Tensor weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_t n, const Tensor& like, bool beside) {
   const int64_t m = x.t.size(0);
   if (col_major(like)) {
     Tensor out = c.empty({n, k});
-    matmul(c, dz.ptr(), dz.ld, 1, x.ptr(), x.ld, 1, n, k, m, out);
+    matmul(c, dz.ptr(), dz.ld, 1, x.ptr(), x.ld, 1, n, k, m, out, Tensor(), Tensor(), 0, Kept(), beside);
     return out.t();
   }
   Tensor out = c.empty({k, n});
-  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out);
+  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out, Tensor(), Tensor(), 0, Kept(), beside);
   return out;
 }
 
@@ -389,24 +389,27 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
   }
-  if (want[2]) dw2 = cut(c, weight_grad(c, hidden, dy, inner8, h8, weight2), inner, h);
+  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8);
+  if (want[3]) act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
+  if (want[4]) act_grad(c, dy, h8, 0, Kept(), false, true, db2);
+  // The products that are left depend on nothing but what is ordered before them: each may start in the SMs that the last turn of
+  // the one before leaves idle.  Everything they touch stays allocated until all of them are launched.
+  bool beside = false;
+  if (want[2]) {
+    dw2 = weight_grad(c, hidden, dy, inner8, h8, weight2, beside);
+    beside = true;
+  }
   if (want[0]) {
-    Tensor out = c.empty({m, h8});
-    matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h8, 2 * inner8, out);
-    dx = cut(c, out, m, h).view(grad_.sizes());
+    dx = c.empty({m, h8});
+    matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h8, 2 * inner8, dx, Tensor(), Tensor(), 0, Kept(), beside);
+    beside = true;
   }
-  if (want[1]) {
-    if (x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8);
-    dw1 = cut_halves(c, weight_grad(c, xm, dz, h8, 2 * inner8, weight1), h, inner);
-  }
-  if (want[3]) {
-    act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
-    db1 = cut_halves(c, db1, 1, inner).view({2 * inner});
-  }
-  if (want[4]) {
-    act_grad(c, dy, h8, 0, Kept(), false, true, db2);
-    db2 = cut(c, db2, 1, h).view({h});
-  }
+  if (want[1]) dw1 = weight_grad(c, xm, dz, h8, 2 * inner8, weight1, beside);
+  if (want[0]) dx = cut(c, dx, m, h).view(grad_.sizes());
+  if (want[1]) dw1 = cut_halves(c, dw1, h, inner);
+  if (want[2]) dw2 = cut(c, dw2, inner, h);
+  if (want[3]) db1 = cut_halves(c, db1, 1, inner).view({2 * inner});
+  if (want[4]) db2 = cut(c, db2, 1, h).view({h});
   c.flush();
   return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
 }
@@ -520,15 +523,14 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
     if (want[0]) w = matrix_of(c, weight, k8, n8);
     if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, k}), k8);
     const Mat dz = act_grad(c, rows_of(c, grad_.reshape({m, n}), n8), n8, act, kept, want[0] || want[1], want[2], db);
+    if (want[1] && x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8);
     if (want[0]) {
-      Tensor out = c.empty({m, k8});
-      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k8, n8, out);
-      dx = cut(c, out, m, k).view(x_sizes);
+      dx = c.empty({m, k8});
+      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k8, n8, dx);
     }
-    if (want[1]) {
-      if (x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8);
-      dw = cut(c, weight_grad(c, xm, dz, k8, n8, weight), k, n);
-    }
+    if (want[1]) dw = weight_grad(c, xm, dz, k8, n8, weight, want[0]);     // beside the one before: see npu_gated_ffn_backward
+    if (want[0]) dx = cut(c, dx, m, k).view(x_sizes);
+    if (want[1]) dw = cut(c, dw, k, n);
     if (want[2]) db = cut(c, db, 1, n).view({n});
     c.flush();
   }
