@@ -97,7 +97,46 @@ __device__ __forceinline__ RowQuant make_block_quant(float amax, bool finite) {
     rq.inv = 0.f;
     rq.exact = false;
   }
-  return rq;                         // quant8 stores zeros where !(scale > 0): NaN included
+  return rq;                         // quant8 gives zeros where !(scale > 0): NaN included
+}
+
+// Two fp32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// quant8 (the correctly rounded quotient, rounded half to even, in the low bytes) on pairs of values.
+__device__ __forceinline__ uint2 block_quant8(const float (&v)[8], const RowQuant& rq) {
+  if (rq.exact || !(rq.scale > 0.f)) return quant8(v, rq);
+  const uint64_t inv = f32x2(rq.inv, rq.inv), minus_scale = f32x2(-rq.scale, -rq.scale), magic = f32x2(kRoundMagic, kRoundMagic);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t x = f32x2(v[2 * i], v[2 * i + 1]);
+    const uint64_t q0 = mul_f32x2(x, inv);
+    const uint64_t q1 = fma_f32x2(fma_f32x2(q0, minus_scale, x), inv, q0);
+    const uint64_t r = add_f32x2(q1, magic);
+    w[2 * i] = static_cast<uint32_t>(r);
+    w[2 * i + 1] = static_cast<uint32_t>(r >> 32);
+  }
+  return make_uint2(pack4_words(w[0], w[1], w[2], w[3]), pack4_words(w[4], w[5], w[6], w[7]));
 }
 
 // ---- packing -------------------------------------------------------------------------------------------------------------

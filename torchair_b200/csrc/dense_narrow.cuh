@@ -74,7 +74,7 @@ __device__ __forceinline__ void keep8(const DenseParams& p, const float (&v)[8],
     for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (live) {
       const RowQuant rq = make_block_quant(__uint_as_float(m), m < 0x7f800000u);
-      const uint2 q = in ? quant8(v, rq) : make_uint2(0u, 0u);
+      const uint2 q = in ? block_quant8(v, rq) : make_uint2(0u, 0u);
       *reinterpret_cast<uint2*>(p.keep_q + row * p.keep_ld + col) = q;
       if ((threadIdx.x & 7) == 0) p.keep_scale[row * (p.keep_ld / kKeepBlock) + col / kKeepBlock] = rq.scale;
     }

@@ -165,7 +165,7 @@ __device__ __forceinline__ void store_q16(const float (&v)[16], const RowQuant& 
       float t[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = v[8 * k + i];
-      o[k] = quant8(t, rq);
+      o[k] = block_quant8(t, rq);
     }
   }
   *reinterpret_cast<uint4*>(q) = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
