@@ -654,6 +654,31 @@ def test_compiled_by_the_backend(dev):
         assert torch.equal(compiled(nx), model(nx))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("fused", [True, False])
+def test_moe_layer_with_a_shared_expert(dev, fused):
+    """The layer's shared expert is npu_gated_ffn handed to the combine; without one nothing changes."""
+    from oracle import moe_oracle as O
+    from torchair_b200.layer import moe_layer
+    cfg = O.CONFIGS["cfg0"]
+    w = O.make_weights(cfg, seed=3)
+    x, ids, wt = (t.to(dev) for t in O.make_tokens(cfg, seed=3))
+    args = (x, ids, wt, w.w1.to(dev), w.s1.to(dev), w.w2.to(dev), w.s2.to(dev))
+    g = gen(2)
+    h = x.shape[1]
+    s1, s2 = weight(g, h, 512, True, x.dtype), weight(g, 256, h, True, x.dtype)
+    plain = moe_layer(*args, fused=fused)
+    got = moe_layer(*args, fused=fused, shared_w1=s1, shared_w2=s2)
+    shared = npu.npu_gated_ffn(x, s1, s2)
+    check(shared, *ref_ffn(x, s1, s2, None, None, None, "silu"), "shared expert")
+    # the routed sum was rounded once in `plain`, and is not in `got`: both roundings apart
+    off = (got.double() - plain.double() - shared.double()).abs()
+    assert (off <= U(x.dtype) * (plain.double().abs() + got.double().abs()) + 2.0 ** -20).all()
+    with pytest.raises(RuntimeError, match="both shared_w1 and shared_w2"):
+        moe_layer(*args, fused=fused, shared_w1=s1)
+    assert torch.equal(plain.cpu(), O.moe_layer([x.cpu()], [ids.cpu()], [wt.cpu()], w, [])[0])
+
+
 # ---- refusals (CPU) ------------------------------------------------------------------------------------------------------
 def _meta(*shape, dtype=torch.bfloat16):
     return torch.empty(*shape, dtype=dtype, device="meta")

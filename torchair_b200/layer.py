@@ -9,11 +9,12 @@ from __future__ import annotations
 
 import torch
 
-from . import ops  # noqa: F401  (registers torch.ops.npu.*)
+from . import dense, ops  # noqa: F401  (register torch.ops.npu.*)
 
 
 def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "", ep_world_size: int = 1,
-              ep_rank_id: int = 0, moe_expert_num: int = None, fused: bool = True, after_dispatch=None):
+              ep_rank_id: int = 0, moe_expert_num: int = None, fused: bool = True, after_dispatch=None, shared_w1=None,
+              shared_w2=None):
     """x [T, H] bf16; expert_ids int32 [T, K]; expert_scales fp32 [T, K]; w1 int8 [E_l, H, 2I]; s1 fp32 [E_l, 2I];
     w2 int8 [E_l, I, H]; s2 fp32 [E_l, H] (this rank's experts).  Returns [T, H] bf16.
 
@@ -24,7 +25,12 @@ def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "
     after_dispatch: optional callable without arguments, called once the dispatch has been enqueued.  A caller that has
     work of its own to run beside the layer (transfers for the next step on other streams, say) forks it there: next to
     the expert GEMMs it disturbs the step less than next to the latency-bound exchange at the step's start.
+
+    shared_w1 [H, 2 I_s], shared_w2 [I_s, H] (both or neither, of x's dtype): a shared expert in 16 bits.  Every token passes
+    through it (npu_gated_ffn) and the combine adds its row before the one rounding of the result.
     """
+    if (shared_w1 is None) != (shared_w2 is None):
+        raise RuntimeError("moe_layer: a shared expert needs both shared_w1 and shared_w2")
     npu = torch.ops.npu
     R = ep_world_size
     E = moe_expert_num if moe_expert_num is not None else w1.shape[0] * R
@@ -35,6 +41,7 @@ def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "
         x, expert_ids, group_ep, R, ep_rank_id, E, quant_mode=2, expert_token_nums_type=1)
     if after_dispatch is not None:
         after_dispatch()
+    shared = None if shared_w1 is None else npu.npu_gated_ffn(x, shared_w1, shared_w2)
     if fused:
         hq, hs = npu.npu_grouped_matmul_swiglu_quant_v2(ex, [w1], [s1], xs, nums, group_list_type=1, tuning_config=tune)
     else:
@@ -46,8 +53,9 @@ def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "
         # down GEMM and combine in one step: over peer memory the GEMM's epilogue stores its rows into the senders'
         # return buffers (a compiled graph gets the same rewrite from the FX pass of the backend)
         return ops.fused_down_combine(hq, w2, s2, hs, nums, 1, expert_ids, expand_idx, ep_recv, expert_scales, group_ep, R,
-                                      ep_rank_id, E, out_dtype=x.dtype, expected_rows=tune[0])
+                                      ep_rank_id, E, shared_expert_x=shared, out_dtype=x.dtype, expected_rows=tune[0])
     y = npu.npu_grouped_matmul([hq], [w2], scale=[s2], per_token_scale=[hs], group_list=nums, split_item=2,
                                group_type=0, group_list_type=1, output_dtype=15 if x.dtype == torch.bfloat16 else 5,
                                tuning_config=tune)[0]
-    return npu.npu_moe_distribute_combine(y, expert_ids, expand_idx, ep_recv, expert_scales, group_ep, R, ep_rank_id, E)
+    return npu.npu_moe_distribute_combine(y, expert_ids, expand_idx, ep_recv, expert_scales, group_ep, R, ep_rank_id, E,
+                                          shared_expert_x=shared)
