@@ -228,6 +228,7 @@ struct TileEpilogue {
   int lane, row_base, ct, col_begin, col_end;
   bool rvalid;
   Ahead r0, r1;            // residual (kEpiLinear); kept gate and up (kEpiGluGrad)
+  uint32_t bias_pair;      // lane l: two bias values of this warp's columns (kEpiGlu: lanes 16.. those of the up values)
 
   __device__ __forceinline__ TileEpilogue(const DenseParams& p_, uint8_t* patch_, int lane_, int row_base_, int ct_, int begin, int end)
       : p(p_), patch(patch_), lane(lane_), row_base(row_base_), ct(ct_), col_begin(begin), col_end(end), rvalid(row_base_ + lane_ < p_.M) {}
@@ -245,9 +246,27 @@ struct TileEpilogue {
     }
   }
 
-  // before the wait for the accumulators
+  // Before the wait for the accumulators.  The bias of all of a warp's columns (64, or 32 pairs) fits one register per lane and is
+  // handed out by shuffles: asked for step by step, every step waited for L2.
   __device__ __forceinline__ void prefetch() {
-    if (row_base < p.M && col_begin < col_end) look_ahead(col_begin);
+    if (row_base >= p.M || col_begin >= col_end) return;
+    look_ahead(col_begin);
+    bias_pair = 0u;
+    if (EPI != kEpiGluGrad && p.bias != nullptr) {
+      const bool up = EPI == kEpiGlu && lane >= 16;
+      const int col = ct * (EPI == kEpiGlu ? 128 : 256) + col_begin + 2 * (up ? lane - 16 : lane);
+      if (col < p.N) bias_pair = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.bias) + (up ? p.N : 0) + col));
+    }
+  }
+  // v[0..15] += bias of the 16 columns from c on (first_lane: where the pair of col_begin is held)
+  __device__ __forceinline__ void add_bias(float (&v)[16], int c, int first_lane) const {
+    const int from = first_lane + ((c - col_begin) >> 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 b = unpack2<T>(__shfl_sync(0xffffffffu, bias_pair, from + i));
+      v[2 * i] += b.x;
+      v[2 * i + 1] += b.y;
+    }
   }
 
   __device__ __forceinline__ void run(DenseAcc& acc) {
@@ -290,12 +309,10 @@ struct TileEpilogue {
       if (keep8 && ((c & 63) == 0 || c == col_begin))
         rq = block_quant(acc, p.bias, c & ~63, col & ~63, p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock, (c & 63) == 0);
       float v[16];
-      Bias16<T> b;
-      if (has_bias) b.load(p.bias, col, p.N);
       if (has_res) r0.put(main_patch, lane);
       acc.fetch(c, v);                                   // (the warp meets in there)
       if (c + 16 >= col_end) acc.release(lane);
-      if (has_bias) b.add(v);
+      if (has_bias) add_bias(v, c, 0);
       if (keep8) {
         if (rvalid) store_q16(v, rq, p.keep_q + row * p.keep_ld + col, col, p.N);
       } else if (keep16) {
@@ -340,17 +357,12 @@ struct TileEpilogue {
         ru = block_quant(acc, has_bias ? bias_up : nullptr, block_at + 64, col & ~63, scale + p.keep_up / kKeepBlock, (c & 63) == 0);
       }
       float g[16], u[16];
-      Bias16<T> bg, bu;
-      if (has_bias) {
-        bg.load(p.bias, col, p.N);
-        bu.load(bias_up, col, p.N);
-      }
       acc.fetch(at, g);
       acc.fetch(at + 64, u);
       if (c + 16 >= col_end) acc.release(lane);
       if (has_bias) {
-        bg.add(g);
-        bu.add(u);
+        add_bias(g, c, 0);
+        add_bias(u, c, 16);
       }
       if (keep8) {
         if (rvalid) {
