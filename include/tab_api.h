@@ -450,8 +450,9 @@ TAB_API int tab_gmm_status_reset(tab_stream_t stream);
  * No counterpart on the reference's path (its shared experts are dense modules beside the routed ones); they serve
  * npu_gated_ffn, npu_linear_act and npu_checkpoint_weight_grad of this package.
  *
- * dtype 5 (fp16) or 15 (bf16) for every 16-bit tensor of a call; accumulators and epilogues are fp32.  All pointers 16-byte
- * aligned, leading dimensions and output features (N, H, I) multiples of 8; rows and the contraction are free.  An operand with `mn` = 0 is contiguous
+ * dtype 5 (fp16) or 15 (bf16) for every 16-bit tensor of a call; accumulators and epilogues are fp32.  Operands and kept values
+ * are 16-byte aligned with leading dimensions that are multiples of 8, and so is I; rows, contraction and output features N, H
+ * are free (out, residual and bias of N or H features may lie anywhere; whole 16-byte rows are faster).  An operand with `mn` = 0 is contiguous
  * along the contraction (element (i, k) at i * ld + k), with `mn` = 1 along its own index (k * ld + i).
  * keep / keep_q + keep_scale (all null: nothing is kept) receive the values before the activation for the backward pass,
  * 16-bit, or int8 with one fp32 scale per row and 64 values (keep_ld a multiple of 64, scales [M, keep_ld / 64]; see
@@ -467,7 +468,8 @@ TAB_API int tab_gmm_status_reset(tab_stream_t stream);
  * tab_gated_matmul_grad:  dh = the product of dy [M, K] with the operand weight (index i of I, contraction over K: the second
  *                         projection's [I, K] weight has mn = 0 here when its rows are contiguous);
  *                         from the kept gate g and up u: dz[M, 2 I] = [dh u act'(g) | dh act(g)] and h = act(g) u again
- * tab_gated_ffn:          y[M, H] = (act(z[:, :I]) * z[:, I:]) w2 + bias2[H] + residual, z = x w1 + bias1; h lives in the workspace */
+ * tab_gated_ffn:          y[M, H] = (act(z[:, :I]) * z[:, I:]) w2 + bias2[H] + residual, z = x w1 + bias1; h lives in the workspace;
+ *                         w2 has w2_rows <= I rows (the rest of I is padding, whose w1 columns and bias1 are zero) */
 TAB_API int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int dtype, int64_t M,
                              int64_t N, int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q,
                              float* keep_scale, int64_t keep_ld, void* out, int beside_previous,
@@ -480,7 +482,7 @@ TAB_API int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weig
                                   int64_t keep_ld, void* dz, void* h, tab_stream_t stream);
 TAB_API int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, size_t* bytes);
 TAB_API int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ldw1, int w1_mn, const void* w2, int64_t ldw2, int w2_mn,
-                          int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual,
+                          int64_t w2_rows, int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual,
                           int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* y, void* workspace,
                           size_t workspace_bytes, tab_stream_t stream);
 TAB_API int tab_dense_status(int* status_host, tab_stream_t stream);

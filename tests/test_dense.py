@@ -762,9 +762,9 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     mat = lambda **kw: [kw.get("a", one), kw.get("lda", 64), 0, kw.get("b", one), kw.get("ldb", 64), 0, kw.get("dtype", 15), kw.get("M", 4),  # noqa: E731
                         kw.get("N", 64), kw.get("K", 64), kw.get("bias", n), n, kw.get("act", 0), kw.get("keep", n), kw.get("keep_q", n),
                         kw.get("keep_scale", n), kw.get("keep_ld", 0), kw.get("out", one), 0, n]
-    for kw, match in ((dict(a=n), "null"), (dict(dtype=6), "dtype"), (dict(N=60), "multiple of 8"), (dict(lda=63), "multiple of 8"),
+    for kw, match in ((dict(a=n), "null"), (dict(dtype=6), "dtype"), (dict(lda=63), "multiple of 8"),
                       (dict(lda=56), "shorter"), (dict(ldb=32), "shorter"), (dict(act=9), "activation"), (dict(K=0), "K=0"),
-                      (dict(M=-1), "M=-1"), (dict(out=n), "null output"), (dict(a=odd), "aligned"), (dict(bias=odd), "aligned"),
+                      (dict(M=-1), "M=-1"), (dict(out=n), "null output"), (dict(a=odd), "aligned"), (dict(bias=ctypes.c_void_p(261)), "aligned"),
                       (dict(keep=one, keep_ld=32), "kept rows"), (dict(keep_q=one, keep_ld=64), "scales"),
                       (dict(keep=one, keep_q=one, keep_scale=one, keep_ld=64), "either"), (dict(keep_q=one, keep_scale=one, keep_ld=72), "multiple of 8"),
                       (dict(M=2 ** 40), "too large")):
@@ -782,7 +782,7 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     with pytest.raises(RuntimeError, match="null"):
         _lib.call("tab_act_grad", one, 64, 15, 4, 64, 4, n, n, n, 64, one, n, n)
     with pytest.raises(RuntimeError, match="256-byte"):
-        _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, n, 0, n)
+        _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 64, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, n, 0, n)
     with pytest.raises(RuntimeError, match="workspace"):
-        _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, one, 16, n)
+        _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 64, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, one, 16, n)
     assert _lib.workspace_bytes("tab_gated_ffn_workspace_bytes", 4, 64, 64) >= 4 * 64 * 2

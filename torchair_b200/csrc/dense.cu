@@ -292,10 +292,13 @@ static int check_dense(const char* op, int dtype, int64_t M, int64_t N, int64_t 
   if (M < 0 || N <= 0 || K <= 0) return fail(TAB_ERR_BAD_ARG, "%s: M=%lld N=%lld K=%lld", op, (long long)M, (long long)N, (long long)K);
   if (dtype != TAB_BF16 && dtype != TAB_F16) return fail(TAB_ERR_UNSUPPORTED, "%s: dtype %d (want 5 or 15)", op, dtype);
   if (act < TAB_ACT_NONE || act > TAB_ACT_SILU) return fail(TAB_ERR_BAD_ARG, "%s: activation %d", op, act);
-  if (N % 8 != 0) return fail(TAB_ERR_ALIGNMENT, "%s: %lld output features (must be a multiple of 8)", op, (long long)N);
   if (M > (1LL << 30) || N > (1LL << 24) || K > (1LL << 30)) return fail(TAB_ERR_UNSUPPORTED, "%s: dimension too large", op);
   if (((M + 255) / 256) * ((N + 127) / 128) > (1LL << 28)) return fail(TAB_ERR_UNSUPPORTED, "%s: too many tiles", op);
   return TAB_OK;
+}
+
+static int check_multiple(const char* op, const char* name, int64_t v) {
+  return v % 8 == 0 ? TAB_OK : fail(TAB_ERR_ALIGNMENT, "%s: %s=%lld (must be a multiple of 8)", op, name, (long long)v);
 }
 
 static int check_keep(const char* op, const void* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld, int64_t width) {
@@ -309,9 +312,12 @@ static int check_keep(const char* op, const void* keep, const int8_t* keep_q, co
 
 static int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 
-static int check_epilogue_ptrs(const char* op, const void* bias, const void* residual, const void* out) {
+static int check_epilogue_ptrs(const char* op, const void* bias, const void* residual, const void* out, bool whole = true) {
   if (!out) return fail(TAB_ERR_BAD_ARG, "%s: null output", op);
-  if (!aligned16(out) || !aligned16(bias) || !aligned16(residual)) return fail(TAB_ERR_ALIGNMENT, "%s: bias, residual and output must be 16-byte aligned", op);
+  if (whole && (!aligned16(out) || !aligned16(bias) || !aligned16(residual)))
+    return fail(TAB_ERR_ALIGNMENT, "%s: bias, residual and output must be 16-byte aligned", op);
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(residual)) & 1u) != 0)
+    return fail(TAB_ERR_ALIGNMENT, "%s: misaligned pointer", op);
   return TAB_OK;
 }
 
@@ -336,7 +342,8 @@ static int linear_matmul(const char* op, const DenseOperand& a, const DenseOpera
                          int beside, cudaStream_t st) {
   DenseParams p = {};
   p.M = (int)M;
-  p.N = (int)N;
+  p.N = (int)((N + 7) / 8 * 8);
+  p.n_out = (int)N;
   p.act = act;
   p.bias = bias;
   p.residual = residual;
@@ -347,6 +354,7 @@ static int linear_matmul(const char* op, const DenseOperand& a, const DenseOpera
   p.keep_ld = (int)keep_ld;
   p.dependent = dependent;
   p.beside = beside;
+  if (N % 8 != 0 || !aligned16(out) || !aligned16(bias) || !aligned16(residual)) return launch_dense<kEpiLinearAny>(op, dtype, a, b, p, st);
   return launch_dense<kEpiLinear>(op, dtype, a, b, p, st);
 }
 
@@ -362,8 +370,8 @@ extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void
   if (rc != TAB_OK || M == 0) return rc;
   const DenseOperand oa = {a, lda, M, K, a_mn ? 1 : 0}, ob = {b, ldb, N, K, b_mn ? 1 : 0};
   if ((rc = check_operand(op, "a", oa)) != TAB_OK || (rc = check_operand(op, "b", ob)) != TAB_OK) return rc;
-  if ((rc = check_epilogue_ptrs(op, bias, residual, out)) != TAB_OK) return rc;
-  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, keep_q ? up64(N) : N)) != TAB_OK) return rc;
+  if ((rc = check_epilogue_ptrs(op, bias, residual, out, false)) != TAB_OK) return rc;
+  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, keep_q ? up64(N) : (N + 7) / 8 * 8)) != TAB_OK) return rc;
   return linear_matmul(op, oa, ob, dtype, M, N, bias, residual, act, keep, keep_q, keep_scale, keep_ld, out, 0,
                        beside_previous ? 1 : 0, as_stream(stream));
 }
@@ -373,6 +381,7 @@ extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, 
                                 tab_stream_t stream) {
   const char* op = "gated_matmul";
   int rc = check_dense(op, dtype, M, I, K, act);
+  if (rc == TAB_OK) rc = check_multiple(op, "I", I);
   if (rc != TAB_OK || M == 0) return rc;
   const DenseOperand ox = {x, ldx, M, K, 0}, ow = {weight, ldw, 2 * I, K, w_mn ? 1 : 0};
   if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
@@ -386,6 +395,7 @@ extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* w
                                      void* dz, void* h, tab_stream_t stream) {
   const char* op = "gated_matmul_grad";
   int rc = check_dense(op, dtype, M, I, K, act);
+  if (rc == TAB_OK) rc = check_multiple(op, "I", I);
   if (rc != TAB_OK || M == 0) return rc;
   const DenseOperand oa = {dy, lddy, M, K, 0}, ow = {weight, ldw, I, K, w_mn ? 1 : 0};
   if ((rc = check_operand(op, "dy", oa)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
@@ -413,17 +423,20 @@ extern "C" int tab_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I, si
 }
 
 extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ldw1, int w1_mn, const void* w2, int64_t ldw2, int w2_mn,
-                             int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual, int act,
+                             int64_t w2_rows, int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual, int act,
                              void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* y, void* workspace,
                              size_t workspace_bytes, tab_stream_t stream) {
   const char* op = "gated_ffn";
   int rc = check_dense(op, dtype, M, I, H, act);
   if (rc == TAB_OK) rc = check_dense(op, dtype, M, H, I, act);
+  if (rc == TAB_OK) rc = check_multiple(op, "I", I);
   if (rc != TAB_OK || M == 0) return rc;
-  const DenseOperand ox = {x, ldx, M, H, 0}, o1 = {w1, ldw1, 2 * I, H, w1_mn ? 1 : 0}, o2 = {w2, ldw2, H, I, w2_mn ? 1 : 0};
+  if (w2_rows > I || w2_rows <= 0) return fail(TAB_ERR_BAD_ARG, "%s: the second weight has %lld rows for I=%lld", op, (long long)w2_rows, (long long)I);
+  const DenseOperand ox = {x, ldx, M, H, 0}, o1 = {w1, ldw1, 2 * I, H, w1_mn ? 1 : 0}, o2 = {w2, ldw2, H, w2_rows, w2_mn ? 1 : 0};
   if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight1", o1)) != TAB_OK || (rc = check_operand(op, "weight2", o2)) != TAB_OK)
     return rc;
-  if ((rc = check_epilogue_ptrs(op, bias1, residual, y)) != TAB_OK || (rc = check_epilogue_ptrs(op, bias2, nullptr, y)) != TAB_OK) return rc;
+  if ((rc = check_epilogue_ptrs(op, bias2, residual, y, false)) != TAB_OK) return rc;
+  if (!aligned16(bias1)) return fail(TAB_ERR_ALIGNMENT, "%s: bias1 must be 16-byte aligned", op);
   if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
   size_t need = 0;
   tab_gated_ffn_workspace_bytes(M, H, I, &need);

@@ -22,12 +22,16 @@ constexpr long long kDnCyclesPerMs = 2000000LL;
 enum DenseEpilogue {
   kEpiLinear = 0,   // out = act(acc + bias) + residual, optionally keeping acc + bias for the backward pass
   kEpiGlu = 1,      // out = act(gate) * up, optionally keeping gate and up
-  kEpiGluGrad = 2   // acc = d(act(gate) * up): writes d(gate), d(up) and act(gate) * up from the kept gate and up
+  kEpiGluGrad = 2,  // acc = d(act(gate) * up): writes d(gate), d(up) and act(gate) * up from the kept gate and up
+  kEpiLinearAny = 3 // kEpiLinear whose bias, residual and out are accessed element by element: rows of any length, anywhere.  A kind
+                    // of its own: the checks for it inside the loops of kEpiLinear cost 10 % of a 4096 x 4096 x 1024 product
 };
+__host__ __device__ constexpr bool epi_linear(int epi) { return epi == kEpiLinear || epi == kEpiLinearAny; }
 
 struct DenseParams {
   int M;             // rows of the product
-  int N;             // columns of the product (kEpiGlu, kEpiGluGrad: inner features I); a multiple of 8
+  int N;             // columns of the product (kEpiGlu, kEpiGluGrad: inner features I), rounded up to a multiple of 8
+  int n_out;         // columns of bias, residual and out of kEpiLinearAny
   int num_kb;        // blocks of 64 along the contraction
   int row_tiles, col_tiles;
   int tile_begin, tile_end;   // tiles of this launch (dense_pair.cuh)

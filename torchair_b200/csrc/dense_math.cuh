@@ -152,6 +152,12 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// 8 values of a row of n that may begin and end anywhere, columns >= n as zero
+template <typename T>
+__device__ __forceinline__ void load8_any(const T* row, int col, int n, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = col + i < n ? Elem<T>::to_f32(row[col + i]) : 0.f;
+}
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <>

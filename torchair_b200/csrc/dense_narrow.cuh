@@ -265,7 +265,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   // ---- the parts go to the CTAs that finish their rows ----
   const int g_begin = group_begin(rank), g_end = group_begin(rank + 1);
   const int part_floats = split > 1 ? (g_end - g_begin) * kGroupFloats : 0;
-  const float* sums = part;                              // first of this CTA's groups in the first part
+  float* sums = part + g_begin * kGroupFloats;           // this CTA's groups in the first part
   if (split > 1) {
     ptx::cluster_wait();                                 // every CTA of the cluster runs
     if (warp == 0 && lane < split) {
@@ -285,7 +285,9 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   // ---- add up and finish: 8 lanes x 8 features to a group ----
   const bool has_bias = p.bias != nullptr, has_res = p.residual != nullptr, keeps = p.keep != nullptr || p.keep_q != nullptr;
   const int act = p.act;
-  const int64_t ld = p.N;
+  constexpr bool ragged = EPI == kEpiLinearAny;
+  const int n_out = ragged ? p.n_out : p.N;
+  const int64_t ld = n_out;
   const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual);
   T* out = static_cast<T*>(p.out);
   const int lane8 = (threadIdx.x & 7) * 8;
@@ -296,7 +298,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     const int64_t row = row0 + (mine ? g / kGroups : 0);
     const int col = ft * (EPI == kEpiGlu ? 64 : 128) + (mine ? g % kGroups : 0) * 64 + lane8;
     const bool in = mine && col < p.N;
-    const float* src = sums + (mine ? g - g_begin : 0) * kGroupFloats + lane8;
+    float* src = sums + (mine ? g - g_begin : 0) * kGroupFloats + lane8;
     float v[8];
     if constexpr (EPI == kEpiGluGrad) {
       if (in) {
@@ -325,9 +327,20 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       float u[8], r[8];
       if (in) {
         const int64_t at = row * ld + col;
-        if (EPI == kEpiLinear && has_res) Elem<T>::load8(res + at, r);
+        if (epi_linear(EPI) && has_res) {
+          if (ragged) load8_any(res + row * ld, col, n_out, r); else Elem<T>::load8(res + at, r);
+        }
         sum_parts8(src, part_floats, split, v);
-        if (has_bias) add8(v, bias + col);
+        if (has_bias) {
+          if (ragged) {
+            float b[8];
+            load8_any(bias, col, n_out, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += b[i];
+          } else {
+            add8(v, bias + col);
+          }
+        }
         if constexpr (EPI == kEpiGlu) {
           sum_parts8(src + 64, part_floats, split, u);
           if (has_bias) add8(u, bias + p.N + col);
@@ -350,12 +363,21 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
             for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]);
           });
         }
-        if (EPI == kEpiLinear && has_res) {
+        if (epi_linear(EPI) && has_res) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += r[i];
         }
-        Elem<T>::store8(out + row * ld + col, v);
+        // rows that begin anywhere leave through shared memory (over the sums just read), so that lanes run along them
+        if (ragged) Elem<T>::store8(reinterpret_cast<T*>(src), v); else Elem<T>::store8(out + row * ld + col, v);
       }
+    }
+  }
+  if (ragged) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < (g_end - g_begin) * 64; e += kThreads) {
+      const int g = g_begin + (e >> 6), c = e & 63;
+      const int col = ft * 128 + (g % kGroups) * 64 + c;
+      if (col < n_out) out[(row0 + g / kGroups) * ld + col] = reinterpret_cast<const T*>(sums + (e & ~63) + (c & ~7))[c & 7];
     }
   }
   if (split > 1) {

@@ -64,7 +64,8 @@ __device__ __forceinline__ void dense_tile_coord(int t, int row_tiles, int col_t
 // a chain of latencies, and with half the warps a tile's plain epilogue took 6400 cycles, its silu 11300, against 8300 for the
 // main loop at K = 1024.  16-bit values pass between registers and row-major memory through patches of 32 rows x 16 columns, so
 // that global accesses are 16 bytes per lane, two lanes to a row's 32-byte sector.  Rows >= M and columns >= N are left alone
-// (loads give zeros); N is a multiple of 8, no 16-byte piece is ever cut.
+// (loads give zeros); N is a multiple of 8, no 16-byte piece is ever cut.  (kEpiLinearAny moves
+// results, residuals and biases element by element instead.)
 __device__ __forceinline__ uint32_t patch_at(int row, int piece) { return static_cast<uint32_t>(row * 32 + ((piece ^ ((row >> 2) & 1)) << 4)); }
 
 template <typename T>
@@ -107,6 +108,25 @@ __device__ __forceinline__ void patch_store(const uint8_t* patch, int lane, T* b
   }
 }
 
+// The same for rows that begin anywhere: element by element, 16 lanes to a row.
+template <typename T>
+__device__ __forceinline__ void patch_store_any(const uint8_t* patch, int lane, T* base, int64_t ld, int row_base, int rows_end, int col, int cols) {
+  const int c = lane & 15;
+  if (col + c >= cols) return;
+#pragma unroll 4
+  for (int r = lane >> 4; r < 32; r += 2)
+    if (row_base + r < rows_end)
+      base[static_cast<int64_t>(row_base + r) * ld + col + c] = *reinterpret_cast<const T*>(patch + patch_at(r, c >> 3) + (c & 7) * 2);
+}
+template <typename T>
+__device__ __forceinline__ void patch_load_any(uint8_t* patch, int lane, const T* base, int64_t ld, int row_base, int rows_end, int col, int cols) {
+  const int c = lane & 15;
+#pragma unroll 4
+  for (int r = lane >> 4; r < 32; r += 2)
+    *reinterpret_cast<T*>(patch + patch_at(r, c >> 3) + (c & 7) * 2) =
+        col + c < cols && row_base + r < rows_end ? base[static_cast<int64_t>(row_base + r) * ld + col + c] : Elem<T>::from_f32(0.f);
+}
+
 // memory -> registers, as the patch will be filled from them
 struct Ahead {
   uint4 x[2];
@@ -130,11 +150,18 @@ struct Ahead {
 template <typename T>
 struct Bias16 {
   uint4 x[2];
-  __device__ __forceinline__ void load(const void* bias, int col, int cols) {
+  __device__ __forceinline__ void load(const void* bias, int col, int cols, bool ragged) {
+    const T* b = static_cast<const T*>(bias);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       x[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (bias != nullptr && col + 8 * k < cols) x[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(bias) + col + 8 * k));
+      if (ragged) {
+        float v[8];
+        load8_any(b, col + 8 * k, cols, v);
+        x[k] = pack8<T>(v);
+      } else if (col + 8 * k < cols) {
+        x[k] = __ldg(reinterpret_cast<const uint4*>(b + col + 8 * k));
+      }
     }
   }
   __device__ __forceinline__ void add(float (&v)[16]) const {
@@ -255,7 +282,11 @@ struct TileEpilogue {
     if (EPI != kEpiGluGrad && p.bias != nullptr) {
       const bool up = EPI == kEpiGlu && lane >= 16;
       const int col = ct * (EPI == kEpiGlu ? 128 : 256) + col_begin + 2 * (up ? lane - 16 : lane);
-      if (col < p.N) bias_pair = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.bias) + (up ? p.N : 0) + col));
+      const T* b = static_cast<const T*>(p.bias) + (up ? p.N : 0);
+      if (EPI == kEpiLinearAny)
+        bias_pair = pack2<T>(col < p.n_out ? Elem<T>::to_f32(b[col]) : 0.f, col + 1 < p.n_out ? Elem<T>::to_f32(b[col + 1]) : 0.f);
+      else if (col < p.N)
+        bias_pair = __ldg(reinterpret_cast<const uint32_t*>(b + col));
     }
   }
   // v[0..15] += bias of the 16 columns from c on (first_lane: where the pair of col_begin is held)
@@ -271,7 +302,7 @@ struct TileEpilogue {
 
   __device__ __forceinline__ void run(DenseAcc& acc) {
     if (row_base < p.M && col_begin < col_end) {
-      if constexpr (EPI == kEpiLinear) linear(acc);
+      if constexpr (epi_linear(EPI)) linear(acc);
       if constexpr (EPI == kEpiGlu) glu(acc);
       if constexpr (EPI == kEpiGluGrad) glu_grad(acc);
     }
@@ -286,7 +317,7 @@ struct TileEpilogue {
     for (int h = 0; h < 64; h += 16) {
       float v[16];
       Bias16<T> b;
-      if (bias != nullptr) b.load(bias, col + h, p.N);
+      if (bias != nullptr) b.load(bias, col + h, EPI == kEpiLinearAny ? p.n_out : p.N, EPI == kEpiLinearAny);
       acc.fetch(at + h, v);
       if (bias != nullptr) b.add(v);
       m = max(m, amax_bits16(v, col + h, p.N));
@@ -300,6 +331,7 @@ struct TileEpilogue {
     const int64_t row = row_base + lane;
     const bool has_bias = p.bias != nullptr, has_res = p.residual != nullptr, keep8 = p.keep_q != nullptr, keep16 = !keep8 && p.keep != nullptr;
     const int act = p.act;
+    constexpr bool ragged = EPI == kEpiLinearAny;
     uint8_t *main_patch = patch, *side_patch = patch + kDpPatch;
     RowQuant rq;
 #pragma unroll 1
@@ -309,7 +341,10 @@ struct TileEpilogue {
       if (keep8 && ((c & 63) == 0 || c == col_begin))
         rq = block_quant(acc, p.bias, c & ~63, col & ~63, p.keep_scale + row * (p.keep_ld / kKeepBlock) + col / kKeepBlock, (c & 63) == 0);
       float v[16];
-      if (has_res) r0.put(main_patch, lane);
+      if (has_res) {
+        if (ragged) patch_load_any<T>(main_patch, lane, static_cast<const T*>(p.residual), p.n_out, row_base, p.M, col, p.n_out);
+        else r0.put(main_patch, lane);
+      }
       acc.fetch(c, v);                                   // (the warp meets in there)
       if (c + 16 >= col_end) acc.release(lane);
       if (has_bias) add_bias(v, c, 0);
@@ -333,7 +368,8 @@ struct TileEpilogue {
       patch_put<T>(main_patch, lane, v);
       __syncwarp();
       if (keep16) patch_store<T>(side_patch, lane, static_cast<T*>(p.keep), p.keep_ld, row_base, p.M, col, p.N);
-      patch_store<T>(main_patch, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
+      if (ragged) patch_store_any<T>(main_patch, lane, static_cast<T*>(p.out), p.n_out, row_base, p.M, col, p.n_out);
+      else patch_store<T>(main_patch, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
       __syncwarp();
     }
   }

@@ -100,76 +100,101 @@ struct Mat {
   int mn_by_cols() const { return row_major ? 1 : 0; }
 };
 
-// t [m, n] row-major with `cols` >= n columns (a multiple of 8): itself where its memory allows that, else a zero-padded copy
-Mat rows_of(const Call& c, const Tensor& t, int64_t cols) {
-  if (t.size(1) == cols && t.stride(1) == 1 && aligned(t)) {
-    if (t.size(0) <= 1) return {t, cols, true};
-    if (t.stride(0) % 8 == 0 && t.stride(0) >= cols) return {t, t.stride(0), true};
+// t [m, n] row-major: itself where its memory allows that, else a copy with rows of `pitch` >= n elements (a multiple of 8), zero
+// behind n
+Mat rows_of(const Call& c, const Tensor& t, int64_t pitch) {
+  const int64_t n = t.size(1);
+  if ((t.stride(1) == 1 || n == 1) && aligned(t)) {
+    if (t.size(0) <= 1) return {t, pitch, true};
+    if (t.stride(0) % 8 == 0 && t.stride(0) >= n) return {t, t.stride(0), true};
   }
-  Tensor out = c.empty({t.size(0), cols});
+  Tensor out = c.empty({t.size(0), pitch});
   copy_2d(c, t, out);
-  return {out, cols, true};
+  return {out, pitch, true};
+}
+
+// the same with zeros behind the n columns, whatever lies there in t's memory
+Mat padded_rows(const Call& c, const Tensor& t, int64_t pitch) {
+  Tensor out = c.empty({t.size(0), pitch});
+  copy_2d(c, t, out);
+  return {out, pitch, true};
 }
 
 bool col_major(const Tensor& t) { return t.stride(0) == 1 && t.stride(1) != 1; }
 
-// a weight [r, c], padded to [rows, cols] if need be; keeps the order in memory that the weight (and so its gradient) has
-Mat matrix_of(const Call& c, const Tensor& t, int64_t rows, int64_t cols) {
-  if (t.size(0) == rows && t.size(1) == cols && aligned(t)) {
+// a weight [r, c], copied if need be; keeps the order in memory that the weight (and so its gradient) has
+Mat matrix_of(const Call& c, const Tensor& t) {
+  const int64_t rows = t.size(0), cols = t.size(1);
+  if (aligned(t)) {
     if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= cols) return {t, t.stride(0), true};
     if (t.stride(0) == 1 && t.stride(1) % 8 == 0 && t.stride(1) >= rows) return {t, t.stride(1), false};
   }
-  if (col_major(t)) {
-    Tensor out = c.empty({cols, rows}).t();
-    copy_2d(c, t, out);
-    return {out, rows, false};
-  }
-  Tensor out = c.empty({rows, cols});
+  const bool cm = col_major(t);
+  const int64_t pitch = up(cm ? rows : cols, 8);
+  Tensor out = cm ? c.empty({cols, pitch}).t() : c.empty({rows, pitch});
   copy_2d(c, t, out);
-  return {out, cols, true};
+  return {out, pitch, !cm};
 }
 
 // weight1 [H, 2 I] with either half padded to `half` columns when I is not a multiple of 8
-Mat halves_of(const Call& c, const Tensor& t, int64_t rows, int64_t half) {
-  const int64_t inner = t.size(1) / 2;
-  if (inner == half) return matrix_of(c, t, rows, 2 * half);
+Mat halves_of(const Call& c, const Tensor& t, int64_t half) {
+  const int64_t rows = t.size(0), inner = t.size(1) / 2;
+  if (inner == half) return matrix_of(c, t);
   const bool cm = col_major(t);
-  Tensor out = cm ? c.empty({2 * half, rows}).t() : c.empty({rows, 2 * half});
+  const int64_t pitch = cm ? up(rows, 8) : 2 * half;
+  Tensor out = cm ? c.empty({2 * half, pitch}).t() : c.empty({rows, pitch});
   copy_2d(c, t.narrow(1, 0, inner), out.narrow(1, 0, half));
   copy_2d(c, t.narrow(1, inner, inner), out.narrow(1, half, half));
-  return {out, cm ? rows : 2 * half, !cm};
+  return {out, pitch, !cm};
 }
 
-// t [m, n] as [m, cols] without gaps between rows, 16-byte aligned
-Tensor dense_rows(const Call& c, const Tensor& t, int64_t cols) {
-  if (t.size(1) == cols && t.is_contiguous() && aligned(t)) return t;
-  Tensor out = c.empty({t.size(0), cols});
+// weight2 [I, H] with zero rows behind I
+Tensor padded_weight2(const Call& c, const Tensor& t, int64_t rows) {
+  const int64_t cols = t.size(1);
+  Tensor out = col_major(t) ? c.empty({cols, rows}).t() : c.empty({rows, up(cols, 8)}).narrow(1, 0, cols);
   copy_2d(c, t, out);
   return out;
 }
 
-// a bias of n (padded) values; halves: either half padded on its own
-Tensor vector_of(const Call& c, const OptTensor& t, int64_t n, bool halves = false) {
-  if (!t.has_value()) return Tensor();
-  if (t->size(0) == n && t->stride(0) == 1 && aligned(*t)) return *t;
-  if (halves) return halves_of(c, t->unsqueeze(0), 1, n / 2).t;
-  return dense_rows(c, t->unsqueeze(0), n);
-}
-
-// the unpadded corner of a padded result, without gaps, in the same order
-Tensor cut(const Call& c, const Tensor& t, int64_t rows, int64_t cols) {
-  if (t.size(0) == rows && t.size(1) == cols) return t;
-  if (col_major(t)) return cut(c, t.t(), cols, rows).t();
-  Tensor out = c.empty({rows, cols});
-  copy_2d(c, t.narrow(0, 0, rows).narrow(1, 0, cols), out);
+// t [m, n] without gaps between rows, 16-byte aligned where that makes its rows whole pieces
+Tensor dense_rows(const Call& c, const Tensor& t) {
+  if (t.is_contiguous() && (aligned(t) || t.size(1) % 8 != 0)) return t;
+  Tensor out = c.empty({t.size(0), t.size(1)});
+  copy_2d(c, t, out);
   return out;
 }
-Tensor cut_halves(const Call& c, const Tensor& t, int64_t rows, int64_t inner) {
-  const int64_t half = t.size(1) / 2;
-  if (t.size(0) == rows && half == inner) return t;
+
+// a bias without gaps
+Tensor vector_of(const Call& c, const OptTensor& t) {
+  if (!t.has_value()) return Tensor();
+  return dense_rows(c, t->unsqueeze(0));
+}
+// bias1 [2 I], either half padded to `half` values, 16-byte aligned
+Tensor halves_vector(const Call& c, const OptTensor& t, int64_t half) {
+  if (!t.has_value()) return Tensor();
+  if (t->size(0) == 2 * half) {
+    if (t->stride(0) == 1 && aligned(*t)) return *t;
+    Tensor out = c.empty({1, 2 * half});
+    copy_2d(c, t->unsqueeze(0), out);
+    return out;
+  }
+  return halves_of(c, t->unsqueeze(0), half).t;
+}
+
+// the first n values of a padded row of sums
+Tensor cut_row(const Call& c, const Tensor& t, int64_t n) {
+  if (t.size(1) == n) return t.view({n});
+  Tensor out = c.empty({1, n});
+  copy_2d(c, t.narrow(1, 0, n), out);
+  return out.view({n});
+}
+// [rows, 2 I8] -> [rows, 2 I], in the same order
+Tensor cut_halves(const Call& c, const Tensor& t, int64_t inner) {
+  const int64_t rows = t.size(0), half = t.size(1) / 2;
+  if (half == inner) return t;
   Tensor out = col_major(t) ? c.empty({2 * inner, rows}).t() : c.empty({rows, 2 * inner});
-  copy_2d(c, t.narrow(0, 0, rows).narrow(1, 0, inner), out.narrow(1, 0, inner));
-  copy_2d(c, t.narrow(0, 0, rows).narrow(1, half, inner), out.narrow(1, inner, inner));
+  copy_2d(c, t.narrow(1, 0, inner), out.narrow(1, 0, inner));
+  copy_2d(c, t.narrow(1, half, inner), out.narrow(1, inner, inner));
   return out;
 }
 
@@ -245,13 +270,14 @@ void keep_x(const Call& c, const Tensor& x, Kept& kept) {
   quantise(c.stream, xr, x.size(0), x.size(1), xr.stride(0), kept.x_q, kept.x_scale);
 }
 
-// int8 [m, k] with its scales (no gaps) -> 16 bits [m, cols], zero-padded
-Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale, int64_t cols) {
-  Tensor y = c.empty({q.size(0), cols});
+// int8 [m, k] with its scales (no gaps) -> 16 bits, rows of a multiple of 8 values, zero behind k
+Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale) {
+  const int64_t pitch = up(q.size(1), 8);
+  Tensor y = c.empty({q.size(0), pitch});
   ok(tab_checkpoint_dequant(static_cast<const int8_t*>(q.data_ptr()), q.size(1), static_cast<const float*>(scale.data_ptr()), scale.size(1), q.size(0),
-                            q.size(1), y.data_ptr(), c.dtype, cols, cols, c.stream),
+                            q.size(1), y.data_ptr(), c.dtype, pitch, pitch, c.stream),
      "tab_checkpoint_dequant");
-  return {y, cols, true};
+  return {y, pitch, true};
 }
 
 using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
@@ -291,24 +317,21 @@ FfnSizes ffn_check(const Tensor& x, const Tensor& w1, const Tensor& w2, const Op
 
 Tensor ffn_forward(const Call& c, const FfnSizes& s, const Tensor& x, const Tensor& weight1, const Tensor& weight2, const OptTensor& bias1,
                    const OptTensor& bias2, const OptTensor& residual, const Kept& kept) {
-  const int64_t h8 = up(s.h, 8), inner8 = up(s.inner, 8);
-  Tensor y = h8 == s.h ? c.empty(x.sizes()) : c.empty({s.m, h8});
+  const int64_t inner8 = up(s.inner, 8);
+  Tensor y = c.empty(x.sizes());
   if (s.m > 0) {
-    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.h}), h8);
-    const Mat w1 = halves_of(c, weight1, h8, inner8), w2 = matrix_of(c, weight2, inner8, h8);
-    const Tensor b1 = vector_of(c, bias1, 2 * inner8, s.inner != inner8), b2 = vector_of(c, bias2, h8);
-    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.h}), h8) : Tensor();
+    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.h}), up(s.h, 8));
+    const Mat w1 = halves_of(c, weight1, inner8), w2 = matrix_of(c, weight2);
+    const Tensor b1 = halves_vector(c, bias1, inner8), b2 = vector_of(c, bias2);
+    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.h})) : Tensor();
     size_t bytes = 0;
-    ok(tab_gated_ffn_workspace_bytes(s.m, h8, inner8, &bytes), "tab_gated_ffn_workspace_bytes");
+    ok(tab_gated_ffn_workspace_bytes(s.m, s.h, inner8, &bytes), "tab_gated_ffn_workspace_bytes");
     const Tensor ws = c.workspace(bytes);
     c.flush();
-  ok(tab_gated_ffn(xm.ptr(), xm.ld, w1.ptr(), w1.ld, w1.mn_by_cols(), w2.ptr(), w2.ld, w2.mn_by_cols(), c.dtype, s.m, h8, inner8, ptr(b1), ptr(b2),
-                     ptr(r), s.act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), y.data_ptr(), ws.data_ptr(), ws.numel(), c.stream),
+    ok(tab_gated_ffn(xm.ptr(), xm.ld, w1.ptr(), w1.ld, w1.mn_by_cols(), w2.ptr(), w2.ld, w2.mn_by_cols(), s.inner, c.dtype, s.m, s.h, inner8, ptr(b1),
+                     ptr(b2), ptr(r), s.act, kept.p16(), kept.p8(), kept.ps(), kept.ld(), y.data_ptr(), ws.data_ptr(), ws.numel(), c.stream),
        "tab_gated_ffn");
   }
-  if (h8 == s.h) return y;
-  y = cut(c, y, s.m, s.h).view(x.sizes());
-  c.flush();
   return y;
 }
 
@@ -372,44 +395,42 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     if (want[4]) db2 = at::zeros({h}, c.opt);
     return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
   }
-  const Mat dy = rows_of(c, grad_.reshape({m, h}), h8);
+  // column sums read whole pieces of 8: a gradient whose rows are not is copied for them with zeros behind h
+  const Mat dy = want[4] && h8 != h ? padded_rows(c, grad_.reshape({m, h}), h8) : rows_of(c, grad_.reshape({m, h}), h8);
   Mat w1, xm;
-  if (want[0]) w1 = halves_of(c, weight1, h8, inner8);
+  if (want[0]) w1 = halves_of(c, weight1, inner8);
   if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, h}), h8);
   Kept kept;
   kept.values = kept_values;
   kept.scale = kept_scale;
   Mat dz{Tensor(), 2 * inner8, true}, hidden{Tensor(), inner8, true};
   if (want[0] || want[1] || want[2] || want[3]) {
-    const Mat w2 = matrix_of(c, weight2, inner8, h8);
+    const Mat w2 = matrix_of(c, inner == inner8 ? weight2 : padded_weight2(c, weight2, inner8));
     dz.t = c.empty({m, 2 * inner8});
     hidden.t = c.empty({m, inner8});
     c.flush();
-  ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h8, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
+    ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
   }
-  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), h8);
+  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}));
   if (want[3]) act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
   if (want[4]) act_grad(c, dy, h8, 0, Kept(), false, true, db2);
   // The products that are left depend on nothing but what is ordered before them: each may start in the SMs that the last turn of
   // the one before leaves idle.  Everything they touch stays allocated until all of them are launched.
   bool beside = false;
   if (want[2]) {
-    dw2 = weight_grad(c, hidden, dy, inner8, h8, weight2, beside);
+    dw2 = weight_grad(c, hidden, dy, inner, h, weight2, beside);
     beside = true;
   }
   if (want[0]) {
-    dx = c.empty({m, h8});
-    matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h8, 2 * inner8, dx, Tensor(), Tensor(), 0, Kept(), beside);
+    dx = c.empty(grad_.sizes());
+    matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h, 2 * inner8, dx, Tensor(), Tensor(), 0, Kept(), beside);
     beside = true;
   }
-  if (want[1]) dw1 = weight_grad(c, xm, dz, h8, 2 * inner8, weight1, beside);
-  if (want[0]) dx = cut(c, dx, m, h).view(grad_.sizes());
-  if (want[1]) dw1 = cut_halves(c, dw1, h, inner);
-  if (want[2]) dw2 = cut(c, dw2, inner, h);
-  if (want[3]) db1 = cut_halves(c, db1, 1, inner).view({2 * inner});
-  if (want[4]) db2 = cut(c, db2, 1, h).view({h});
+  if (want[1]) dw1 = cut_halves(c, weight_grad(c, xm, dz, h, 2 * inner8, weight1, beside), inner);
+  if (want[3]) db1 = cut_halves(c, db1, inner).reshape({2 * inner});
+  if (want[4]) db2 = cut_row(c, db2, h);
   c.flush();
   return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
 }
@@ -443,18 +464,14 @@ LinearSizes linear_check(const Tensor& x, const Tensor& w, const OptTensor& b, c
 
 Tensor linear_forward(const Call& c, const LinearSizes& s, at::IntArrayRef out_sizes, const Tensor& x, const Tensor& weight, const OptTensor& bias,
                       const OptTensor& residual, const Kept& kept) {
-  const int64_t k8 = up(s.k, 8), n8 = up(s.n, 8);
-  Tensor y = n8 == s.n ? c.empty(out_sizes) : c.empty({s.m, n8});
+  Tensor y = c.empty(out_sizes);
   if (s.m > 0) {
-    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.k}), k8);
-    const Mat w = matrix_of(c, weight, k8, n8);
-    const Tensor b = vector_of(c, bias, n8);
-    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.n}), n8) : Tensor();
-    matmul(c, xm.ptr(), xm.ld, 0, w.ptr(), w.ld, w.mn_by_cols(), s.m, n8, k8, y, b, r, s.act, kept);
+    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.k}), up(s.k, 8));
+    const Mat w = matrix_of(c, weight);
+    const Tensor b = vector_of(c, bias);
+    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.n})) : Tensor();
+    matmul(c, xm.ptr(), xm.ld, 0, w.ptr(), w.ld, w.mn_by_cols(), s.m, s.n, s.k, y, b, r, s.act, kept);
   }
-  if (n8 == s.n) return y;
-  y = cut(c, y, s.m, s.n).view(out_sizes);
-  c.flush();
   return y;
 }
 
@@ -493,7 +510,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
   TORCH_CHECK(weight.dim() == 2 && grad_.dim() >= 1 && grad_.size(-1) == weight.size(1) && weight.size(0) > 0 && weight.size(1) > 0, op, ": grad ",
               grad_.sizes(), " and weight ", weight.sizes(), " do not fit [..., N] and [K, N]");
   same(op, grad_, "weight", weight);
-  const int64_t k = weight.size(0), n = weight.size(1), m = grad_.numel() / n, k8 = up(k, 8), n8 = up(n, 8);
+  const int64_t k = weight.size(0), n = weight.size(1), m = grad_.numel() / n, n8 = up(n, 8);
   const bool int8 = kept_values.scalar_type() == at::kChar, x8 = x_.scalar_type() == at::kChar;
   const int64_t width = up(n, int8 ? kBlock : 8);
   TORCH_CHECK(act == TAB_ACT_NONE ||
@@ -520,18 +537,18 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
       kept.scale = kept_scale;
     }
     Mat w, xm;
-    if (want[0]) w = matrix_of(c, weight, k8, n8);
-    if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, k}), k8);
-    const Mat dz = act_grad(c, rows_of(c, grad_.reshape({m, n}), n8), n8, act, kept, want[0] || want[1], want[2], db);
-    if (want[1] && x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}), k8);
+    if (want[0]) w = matrix_of(c, weight);
+    if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, k}), up(k, 8));
+    // the elementwise kernel reads whole pieces of 8
+    const Mat dy = n8 != n && (act || want[2]) ? padded_rows(c, grad_.reshape({m, n}), n8) : rows_of(c, grad_.reshape({m, n}), n8);
+    const Mat dz = act_grad(c, dy, n8, act, kept, want[0] || want[1], want[2], db);
+    if (want[1] && x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}));
     if (want[0]) {
-      dx = c.empty({m, k8});
-      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k8, n8, dx);
+      dx = c.empty(x_sizes);
+      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k, n, dx);
     }
-    if (want[1]) dw = weight_grad(c, xm, dz, k8, n8, weight, want[0]);     // beside the one before: see npu_gated_ffn_backward
-    if (want[0]) dx = cut(c, dx, m, k).view(x_sizes);
-    if (want[1]) dw = cut(c, dw, k, n);
-    if (want[2]) db = cut(c, db, 1, n).view({n});
+    if (want[1]) dw = weight_grad(c, xm, dz, k, n, weight, want[0]);       // beside the one before: see npu_gated_ffn_backward
+    if (want[2]) db = cut_row(c, db, n);
     c.flush();
   }
   auto result = [&](const Tensor& t) { return t.defined() ? t : c.empty({0}); };
@@ -593,16 +610,14 @@ Tensor ck_weight_grad_cuda(const Tensor& q_, const Tensor& scale_, const Tensor&
   for (int64_t i = 0; fits && i + 1 < q_.dim(); ++i) fits = q_.size(i) == grad_.size(i);
   TORCH_CHECK(fits, op, ": q ", q_.sizes(), " and grad ", grad_.sizes(), " must be [..., K] and [..., N] of the same rows");
   TORCH_CHECK(grad_.device() == q_.device(), op, ": grad is on ", grad_.device(), ", q is on ", q_.device());
-  const int64_t k = q_.size(-1), n = grad_.size(-1), m = q_.numel() / k, k8 = up(k, 8), n8 = up(n, 8);
+  const int64_t k = q_.size(-1), n = grad_.size(-1), m = q_.numel() / k;
   const c10::cuda::CUDAGuard guard(grad_.device());
   const Call c(grad_, dtype);
   if (m == 0) return at::zeros({k, n}, c.opt);
   const Tensor q = q_.contiguous().view({m, k}), scale = scale_.contiguous().view({m, -1});
-  const Mat x = dequantise(c, q, scale, k8), dz = rows_of(c, grad_.reshape({m, n}), n8);
-  Tensor out = c.empty({k8, n8});
-  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k8, n8, m, out);
-  out = cut(c, out, k, n);
-  c.flush();
+  const Mat x = dequantise(c, q, scale), dz = rows_of(c, grad_.reshape({m, n}), up(n, 8));
+  Tensor out = c.empty({k, n});
+  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out);
   return out;
 }
 
