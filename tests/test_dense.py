@@ -149,7 +149,15 @@ LINEAR = [  # rows, in, out, transposed weight, act, bias, residual
     (1000, 72, 3000, True, "none", False, False),
     (2049, 512, 4096, False, "silu", True, True),
     (5000, 4096, 1032, True, "relu", False, False),
+    # a few tiles in a last turn that share their contraction (81 = 74 + 7 and 100 = 74 + 26 tiles of 256 x 256)
+    (2300, 4160, 2104, False, "gelu", True, True),
+    (2560, 4096, 2560, True, "none", False, False),
+    # clusters that share narrow tiles, up to eight to one
+    (128, 8192, 1000, True, "silu", True, False),
+    (70, 2048, 136, False, "none", False, True),
+    (20, 8192, 128, True, "gelu_tanh", True, True),
     # sizes that are multiples of nothing
+    (2301, 4161, 2101, True, "relu", True, True),
     (1, 1, 1, False, "none", True, True),
     (3, 7, 13, True, "silu", True, False),
     (777, 1003, 1501, False, "relu", True, False),
@@ -183,6 +191,8 @@ FFN = [  # rows, hidden, inner, transposed weights, act, biases, residual
     (129, 264, 136, True, "silu", True, True),
     (300, 1024, 520, False, "gelu", False, False),
     (2500, 768, 1024, True, "silu", True, True),
+    (2300, 4160, 1104, False, "silu", True, True),       # 81 tiles of gate and up: the last 7 share their contraction
+    (90, 4096, 200, True, "gelu", False, True),
     (5, 33, 17, False, "silu", True, True),
     (200, 100, 129, True, "gelu_tanh", True, True),
 ]
@@ -636,6 +646,91 @@ def test_only_the_wanted_gradients_and_no_second_order(dev):
     with torch.no_grad():
         assert not npu.npu_gated_ffn(x, w1, w2).requires_grad
     assert not npu.npu_gated_ffn(x.detach(), w1.detach(), w2.detach()).requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(700, 256, 200), (3001, 512, 352), (77, 100, 33), (5, 64, 48)], ids=str)
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+def test_each_gradient_alone_equals_all_at_once(dev, case, int8):
+    """The products of a backward pass overlap on the GPU; asked for one by one they cannot."""
+    m, h, inner = case
+    g = gen(m)
+    x, dy = make(g, m, h), make(g, m, h)
+    w1, w2 = weight(g, h, 2 * inner, False, x.dtype), weight(g, inner, h, True, x.dtype)
+    b1, b2 = make(g, 2 * inner), make(g, h)
+    _, kept, ks, xq, xs = npu.npu_gated_ffn_keep(x, w1, w2, bias1=b1, bias2=b2, checkpoint_int8=int8)
+    src = xq if int8 else x
+    for _ in range(3):
+        both = npu.npu_gated_ffn_backward(dy, src, xs, w1, w2, kept, ks, "silu", [True] * 5)
+        for i in range(5):
+            one = npu.npu_gated_ffn_backward(dy, src, xs, w1, w2, kept, ks, "silu", [i == j for j in range(5)])
+            assert torch.equal(one[i], both[i]) and all(t.numel() == 0 for j, t in enumerate(one) if j != i)
+    w = weight(g, h, inner, True, x.dtype)
+    _, kept, ks, xq, xs = npu.npu_linear_act_keep(x, w, activation="gelu", checkpoint_int8=int8)
+    src, dyl = (xq if int8 else x), make(g, m, inner)
+    both = npu.npu_linear_act_backward(dyl, src, xs, w, kept, ks, "gelu", [True] * 3)
+    for i in range(3):
+        one = npu.npu_linear_act_backward(dyl, src, xs, w, kept, ks, "gelu", [i == j for j in range(3)])
+        assert torch.equal(one[i], both[i])
+
+
+@pytest.mark.gpu
+def test_gradients_of_some_inputs_only(dev):
+    g = gen(14)
+    t = {"x": make(g, 30, 64), "weight1": make(g, 64, 96, scale=0.1), "weight2": make(g, 48, 64, scale=0.1), "bias1": make(g, 96),
+         "bias2": make(g, 64), "residual": make(g, 30, 64)}
+    dy = make(g, 30, 64)
+
+    def grads(names):
+        leaves = {k: v.detach().requires_grad_(k in names) for k, v in t.items()}
+        y = npu.npu_gated_ffn(leaves["x"], leaves["weight1"], leaves["weight2"], **{k: leaves[k] for k in ("bias1", "bias2", "residual")})
+        return dict(zip(names, torch.autograd.grad(y, [leaves[k] for k in names], dy)))
+
+    full = grads(list(t))
+    for names in (["bias1"], ["bias2"], ["residual"], ["x", "bias2"], ["weight2", "residual"], ["weight1"]):
+        for k, v in grads(names).items():
+            assert torch.equal(v, full[k]), (names, k)
+    # a tensor that is an input twice gets both gradients
+    x = t["x"].detach().requires_grad_()
+    y = npu.npu_gated_ffn(x, t["weight1"], t["weight2"], bias1=t["bias1"], bias2=t["bias2"], residual=x)
+    dx, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(dx, (full["x"] + full["residual"]))
+
+
+@pytest.mark.gpu
+def test_outputs_that_lie_anywhere(dev):
+    """The C entry with out, residual and bias one element past a 16-byte boundary, and what lies around out left alone."""
+    import ctypes
+    g = gen(15)
+    for m in (20, 300):
+        x, w = make(g, m, 64), make(g, 64, 136, scale=0.1)
+        b, r = make(g, 137)[1:], make(g, m * 136 + 1)[1:]
+        flat = torch.full((m * 136 + 9,), 7.0, dtype=x.dtype, device=dev)
+        out = flat[1:1 + m * 136]
+        none = ctypes.c_void_p(None)
+        _lib.call("tab_dense_matmul", x.data_ptr(), 64, 0, w.data_ptr(), 136, 1, 15, m, 136, 64, b.data_ptr(), r.data_ptr(), 4, none, none, none, 0,
+                  out.data_ptr(), 0, torch.cuda.current_stream(dev).cuda_stream)
+        want = npu.npu_linear_act(x, w, bias=b, residual=r.view(m, 136), activation="silu")
+        assert torch.equal(out.view(m, 136), want) and flat[0] == 7 and (flat[1 + m * 136:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+def test_traced_forward_and_backward(dev, int8):
+    """The operators under AOT autograd: the same bits as eager, forward and gradients."""
+    ins = _step_inputs(30)
+    want = _train_step(*ins, int8)
+
+    def model(x, w1, w2, w):
+        h = npu.npu_gated_ffn(x, w1, w2, residual=x, checkpoint_int8=int8)
+        return npu.npu_linear_act(h, w, activation="gelu", checkpoint_int8=int8)
+
+    compiled = torch.compile(model, backend="aot_eager", fullgraph=True, dynamic=False)
+    y = compiled(*ins[:4])
+    got = (y.detach(),) + torch.autograd.grad(y, ins[:4], ins[4])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.inference_mode():
+        assert torch.equal(model(*[t.detach() for t in ins[:4]]), want[0])
 
 
 @pytest.mark.gpu
