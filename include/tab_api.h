@@ -464,7 +464,6 @@ TAB_API int tab_gmm_status_reset(tab_stream_t stream);
  *                         partly filled turn leaves SMs idle).  The caller vouches that nothing this product reads or writes is
  *                         written by, and nothing it writes read by, the launches since the last ordinary one, memory that was freed
  *                         and handed out again in between included.  A later ordinary launch waits for both, as ever.
- * tab_gated_matmul:       h[M, I] = act(z[:, :I]) * z[:, I:], z = x weight + bias[2 I], weight [K, 2 I]
  * tab_gated_matmul_grad:  dh = the product of dy [M, K] with the operand weight (index i of I, contraction over K: the second
  *                         projection's [I, K] weight has mn = 0 here when its rows are contiguous);
  *                         from the kept gate g and up u: dz[M, 2 I] = [dh u act'(g) | dh act(g)] and h = act(g) u again
@@ -474,9 +473,6 @@ TAB_API int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void* b
                              int64_t N, int64_t K, const void* bias, const void* residual, int act, void* keep, int8_t* keep_q,
                              float* keep_scale, int64_t keep_ld, void* out, int beside_previous,
                              tab_stream_t stream);
-TAB_API int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
-                             int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld,
-                             void* h, tab_stream_t stream);
 TAB_API int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M,
                                   int64_t I, int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale,
                                   int64_t keep_ld, void* dz, void* h, tab_stream_t stream);

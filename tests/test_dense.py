@@ -497,6 +497,57 @@ def test_nan_and_infinity_stay_in_their_rows(dev, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inner", [33, 40])
+@pytest.mark.parametrize("m", [5, 300])
+def test_padding_of_the_inner_features_adds_nothing_to_infinities(dev, m, inner):
+    """Weights and values are positive, so a row that holds an infinity has infinities and no NaN in its results and gradients,
+    whether or not the inner features are padded to a multiple of 8.  (The gradient of up * relu(gate) at gate = up = inf is
+    dh * up * 1 and dh * gate.)"""
+    g = gen(inner + m)
+    x, dy = make(g, m, 48).abs() + 0.125, make(g, m, 48).abs() + 0.125
+    w1, w2 = make(g, 48, 2 * inner).abs() + 0.125, make(g, inner, 48).abs() + 0.125
+    x[2, 3] = math.inf
+    dy[3, 5] = math.inf
+    leaf = x.clone().requires_grad_()
+    y = npu.npu_gated_ffn(leaf, w1, w2, activation="relu")
+    dx, = torch.autograd.grad(y, leaf, dy)
+    inf = torch.zeros(m, dtype=torch.bool, device=dev)
+    inf[2] = True
+    assert torch.equal(torch.isposinf(y), inf[:, None].expand_as(y)) and not torch.isnan(y).any()
+    inf[3] = True
+    assert torch.equal(torch.isposinf(dx), inf[:, None].expand_as(dx)) and not torch.isnan(dx).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ACTS)
+def test_gradient_at_nan_is_nan(dev, act):
+    """as in the formulas: also of relu, where neither branch holds at NaN"""
+    x = torch.ones(4, 8, dtype=torch.bfloat16, device=dev)
+    x[1, 0] = math.nan
+    w = torch.ones(8, 16, dtype=torch.bfloat16, device=dev)
+    leaf = x.requires_grad_()
+    dx, = torch.autograd.grad(npu.npu_linear_act(leaf, w, activation=act), leaf, torch.ones(4, 16, dtype=torch.bfloat16, device=dev))
+    nan = torch.tensor([False, act != "none", False, False], device=dev)
+    assert torch.equal(torch.isnan(dx), nan[:, None].expand_as(dx))
+
+
+@pytest.mark.gpu
+def test_gradients_have_the_strides_that_the_meta_implementation_gives(dev):
+    meta = lambda t: t if not isinstance(t, torch.Tensor) else torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="meta")
+    g = gen(16)
+    for m in (0, 3):
+        for transposed in (False, True):
+            for h, inner in ((16, 24), (9, 5), (1, 1)):
+                w1, w2 = weight(g, h, 2 * inner, transposed, torch.float16), weight(g, inner, h, transposed, torch.float16)
+                x = make(g, m, h, dtype=torch.float16)
+                y, kept, ks, xq, xs = npu.npu_gated_ffn_keep(x, w1, w2)
+                for op, args in ((npu.npu_gated_ffn_backward, (y, x, xs, w1, w2, kept, ks, "silu", [True] * 5)),
+                                 (npu.npu_linear_act_backward, (make(g, m, 2 * inner, dtype=torch.float16), x, xs, w1, kept, ks, "none", [True] * 3))):
+                    for real, want in zip(op(*args), op(*[meta(a) for a in args])):
+                        assert real.shape == want.shape and real.stride() == want.stride() and real.dtype == want.dtype
+
+
+@pytest.mark.gpu
 def test_rows_of_a_batch_do_not_depend_on_each_other(dev):
     """The same row at another place of a batch of the same size gives the same bits; other rows do not touch it."""
     g = gen(8)

@@ -1,5 +1,5 @@
 // Host side of the dense 16-bit GEMMs: argument checks, tensor maps, the choice between the narrow and the pair kernel and
-// how many CTAs share a tile, and the C entry points tab_dense_matmul, tab_gated_matmul, tab_gated_matmul_grad, tab_gated_ffn.
+// how many CTAs share a tile, and the C entry points tab_dense_matmul, tab_gated_matmul_grad, tab_gated_ffn.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -376,20 +376,6 @@ extern "C" int tab_dense_matmul(const void* a, int64_t lda, int a_mn, const void
                        beside_previous ? 1 : 0, as_stream(stream));
 }
 
-extern "C" int tab_gated_matmul(const void* x, int64_t ldx, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
-                                int64_t K, const void* bias, int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* h,
-                                tab_stream_t stream) {
-  const char* op = "gated_matmul";
-  int rc = check_dense(op, dtype, M, I, K, act);
-  if (rc == TAB_OK) rc = check_multiple(op, "I", I);
-  if (rc != TAB_OK || M == 0) return rc;
-  const DenseOperand ox = {x, ldx, M, K, 0}, ow = {weight, ldw, 2 * I, K, w_mn ? 1 : 0};
-  if ((rc = check_operand(op, "x", ox)) != TAB_OK || (rc = check_operand(op, "weight", ow)) != TAB_OK) return rc;
-  if ((rc = check_epilogue_ptrs(op, bias, nullptr, h)) != TAB_OK) return rc;
-  if ((rc = check_keep(op, keep, keep_q, keep_scale, keep_ld, 2 * (keep_q ? up64(I) : I))) != TAB_OK) return rc;
-  return gated_matmul(op, ox, ow, dtype, M, I, bias, act, keep, keep_q, keep_scale, keep_ld, h, as_stream(stream));
-}
-
 extern "C" int tab_gated_matmul_grad(const void* dy, int64_t lddy, const void* weight, int64_t ldw, int w_mn, int dtype, int64_t M, int64_t I,
                                      int64_t K, int act, const void* keep, const int8_t* keep_q, const float* keep_scale, int64_t keep_ld,
                                      void* dz, void* h, tab_stream_t stream) {
@@ -445,7 +431,8 @@ extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t
   cudaStream_t st = as_stream(stream);
   rc = gated_matmul(op, ox, o1, dtype, M, I, bias1, act, keep, keep_q, keep_scale, keep_ld, workspace, st);
   if (rc != TAB_OK) return rc;
-  const DenseOperand oh = {workspace, I, M, I, 0};
+  // the hidden columns behind w2_rows meet no row of w2 and are not read: a row of infinities leaves NaN there
+  const DenseOperand oh = {workspace, I, M, w2_rows, 0};
   return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, 0, st);
 }
 

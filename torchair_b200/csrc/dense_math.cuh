@@ -48,7 +48,7 @@ template <int ACT>
 __device__ __forceinline__ void act_both(float z, float& a, float& d) {
   if constexpr (ACT == TAB_ACT_RELU) {
     a = z < 0.f ? 0.f : z;
-    d = z > 0.f ? 1.f : 0.f;
+    d = z <= 0.f ? 0.f : z > 0.f ? 1.f : z;                          // in the derivative too
   } else if constexpr (ACT == TAB_ACT_SILU) {
     const float s = sigmoid_f(z);
     a = z * s;

@@ -64,8 +64,8 @@ __device__ __forceinline__ void dense_tile_coord(int t, int row_tiles, int col_t
 // a chain of latencies, and with half the warps a tile's plain epilogue took 6400 cycles, its silu 11300, against 8300 for the
 // main loop at K = 1024.  16-bit values pass between registers and row-major memory through patches of 32 rows x 16 columns, so
 // that global accesses are 16 bytes per lane, two lanes to a row's 32-byte sector.  Rows >= M and columns >= N are left alone
-// (loads give zeros); N is a multiple of 8, no 16-byte piece is ever cut.  (kEpiLinearAny moves
-// results, residuals and biases element by element instead.)
+// (loads give zeros); N is a multiple of 8, no 16-byte piece is ever cut.  (kEpiLinearAny moves results, residuals and biases
+// element by element instead.)
 __device__ __forceinline__ uint32_t patch_at(int row, int piece) { return static_cast<uint32_t>(row * 32 + ((piece ^ ((row >> 2) & 1)) << 4)); }
 
 template <typename T>
@@ -246,8 +246,13 @@ struct DenseAcc {
   }
 };
 
-// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 16).  What it reads from global memory (residual, kept values) is asked for before the
-// accumulators are waited for, then one step ahead.
+// Epilogue of one warp: 32 rows (row_base ..) x the output columns [col_begin, col_end) of the tile (multiples of 16).  What it
+// reads from global memory (residual, kept values) is asked for before the accumulators are waited for, then one step ahead.
+//
+// Rounding.  The kept values of kEpiGlu and kEpiLinear, the hidden rows of kEpiGlu and the three results of kEpiGluGrad go to HBM
+// in the operands' 16 bits: the next product takes 16-bit operands anyway, and the values that only the backward pass reads would
+// cost twice the bytes in fp32 (3001 x 2 x 1408 of them: 17 MB more per direction) for an error that stays below that of the
+// operands' own rounding.  The activation and the products of the epilogue see the fp32 accumulator, not its rounded copy.
 template <typename T, int EPI>
 struct TileEpilogue {
   const DenseParams& p;
@@ -623,7 +628,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       }
     }
   } else {
-    // ---------------- epilogue: warps 2..9, thread = row, two warps share the columns of a row ----------------
+    // ---------------- epilogue: warps 2..17, thread = row, four warps share the columns of a row ----------------
     const int quarter = warp & 3;
     const int share = (warp - 2) >> 2;
     int buf = 0;

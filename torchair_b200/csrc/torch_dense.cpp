@@ -213,6 +213,7 @@ struct Kept {
 // act(a b^T + bias) + residual: a [m, k], b [n, k] as operands
 void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, int64_t ldb, int b_mn, int64_t m, int64_t n, int64_t k, const Tensor& out,
             const Tensor& bias = Tensor(), const Tensor& residual = Tensor(), int act = 0, const Kept& kept = Kept(), bool beside = false) {
+  beside = beside && c.pending == 0;           // a product does not run beside the copy that it reads
   c.flush();
   ok(tab_dense_matmul(a, lda, a_mn, b, ldb, b_mn, c.dtype, m, n, k, ptr(bias), ptr(residual), act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                       out.data_ptr(), beside, c.stream),
@@ -230,6 +231,11 @@ Tensor weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_
   Tensor out = c.empty({k, n});
   matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out, Tensor(), Tensor(), 0, Kept(), beside);
   return out;
+}
+
+// the same without rows to sum over
+Tensor zero_grad(const Call& c, const Tensor& like) {
+  return col_major(like) ? at::zeros({like.size(1), like.size(0)}, c.opt).t() : at::zeros({like.size(0), like.size(1)}, c.opt);
 }
 
 // dz = grad act'(kept) (grad itself without an activation) and, if wanted, its column sums
@@ -389,8 +395,8 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
   };
   if (m == 0) {
     if (want[0]) dx = at::zeros(grad_.sizes(), c.opt);
-    if (want[1]) dw1 = at::zeros({h, 2 * inner}, c.opt);
-    if (want[2]) dw2 = at::zeros({inner, h}, c.opt);
+    if (want[1]) dw1 = zero_grad(c, weight1);
+    if (want[2]) dw2 = zero_grad(c, weight2);
     if (want[3]) db1 = at::zeros({2 * inner}, c.opt);
     if (want[4]) db2 = at::zeros({h}, c.opt);
     return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
@@ -412,6 +418,12 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
+    if (want[0] && inner != inner8) {      // the product for dx runs over the columns behind I too: infinities leave NaN there
+      const Tensor nothing = dz.t.narrow(1, 0, 0);
+      copy_2d(c, nothing, dz.t.narrow(1, inner, inner8 - inner));
+      copy_2d(c, nothing, dz.t.narrow(1, inner8 + inner, inner8 - inner));
+      c.flush();
+    }
   }
   if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}));
   if (want[3]) act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
@@ -528,7 +540,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
   Tensor dx, dw, db;
   if (m == 0) {
     if (want[0]) dx = at::zeros(x_sizes, c.opt);
-    if (want[1]) dw = at::zeros({k, n}, c.opt);
+    if (want[1]) dw = zero_grad(c, weight);
     if (want[2]) db = at::zeros({n}, c.opt);
   } else {
     Kept kept;

@@ -116,10 +116,21 @@ def _ffn_keep_meta(x, weight1, weight2, *, bias1=None, bias2=None, residual=None
     return (torch.empty(x.shape, dtype=x.dtype, device=x.device),) + _kept_meta(x, m, width, width // KEEP_BLOCK, checkpoint_int8)
 
 
+def _grad_meta(grad, shape, want):
+    """An empty gradient: of a weight in the order in memory that the weight has, of anything else contiguous."""
+    if not want:
+        shape = (0,)
+    elif isinstance(shape, torch.Tensor):
+        if shape.stride(0) == 1 and shape.stride(1) != 1:
+            return torch.empty(shape.shape[::-1], dtype=grad.dtype, device=grad.device).t()
+        shape = shape.shape
+    return torch.empty(shape, dtype=grad.dtype, device=grad.device)
+
+
 def _ffn_backward_meta(grad, x, x_scale, weight1, weight2, kept, kept_scale, activation, output_mask):
     _act_code("npu_gated_ffn_backward", activation)
-    shapes = (grad.shape, weight1.shape, weight2.shape, (weight1.shape[1],), (weight2.shape[1],))
-    return tuple(torch.empty(s if want else (0,), dtype=grad.dtype, device=grad.device) for s, want in zip(shapes, output_mask))
+    shapes = (grad.shape, weight1, weight2, (weight1.shape[1],), (weight2.shape[1],))
+    return tuple(_grad_meta(grad, s, want) for s, want in zip(shapes, output_mask))
 
 
 def _linear_check(op, x, weight, bias, residual, activation):
@@ -151,8 +162,8 @@ def _linear_keep_meta(x, weight, *, bias=None, residual=None, activation="none",
 
 def _linear_backward_meta(grad, x, x_scale, weight, kept, kept_scale, activation, output_mask):
     _act_code("npu_linear_act_backward", activation)
-    shapes = (grad.shape[:-1] + (weight.shape[0],), weight.shape, (weight.shape[1],))
-    return tuple(torch.empty(s if want else (0,), dtype=grad.dtype, device=grad.device) for s, want in zip(shapes, output_mask))
+    shapes = (grad.shape[:-1] + (weight.shape[0],), weight, (weight.shape[1],))
+    return tuple(_grad_meta(grad, s, want) for s, want in zip(shapes, output_mask))
 
 
 def _ck_quant_meta(x):
