@@ -632,6 +632,75 @@ def test_a_run_of_them_on_other_streams_and_in_graphs(dev, m, int8):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 40, 200, 2000])
+def test_every_operand_written_by_the_call_before(dev, m):
+    """Launches overlap the end of the one before; what that one writes (x, weight, bias, residual, an 8-bit checkpoint, a gradient)
+    or still reads must be waited for.  The same calls with the GPU idle before each give the same bits."""
+    g = gen(m)
+    h = 512
+    x, w, v = make(g, m, h), make(g, h, h, scale=h ** -0.5), make(g, h, h, scale=h ** -0.5)
+
+    def chain(wait):
+        def call(f, *args, **kwargs):
+            if wait:
+                torch.cuda.synchronize()
+            return f(*args, **kwargs)
+
+        out = []
+        for _ in range(4):
+            weight2 = call(npu.npu_linear_act, w, v)                                   # written here, used as a weight
+            y = call(npu.npu_linear_act, x, weight2, activation="relu")
+            y = call(npu.npu_linear_act, x, w, residual=y)                             # as the residual
+            weight1 = call(npu.npu_linear_act, v, torch.cat((w, v), 1))
+            y = call(npu.npu_gated_ffn, y, weight1, weight2)
+            b = call(npu.npu_linear_act, y[:1], w)[0]
+            y = call(npu.npu_linear_act, y, w.t(), bias=b)                             # as the bias
+            q, s = call(npu.npu_checkpoint_quant, y)
+            d = call(npu.npu_checkpoint_weight_grad, q, s, x)
+            y = call(npu.npu_checkpoint_dequant, *call(npu.npu_checkpoint_quant, call(npu.npu_linear_act, y, d)))
+            leaf = y.detach().requires_grad_()
+            z = call(npu.npu_gated_ffn, leaf, weight1, weight2, checkpoint_int8=True)
+            dx, = torch.autograd.grad(z, leaf, call(npu.npu_linear_act, x, weight2))
+            out += [y, d, z.detach(), dx]
+            del weight1, weight2, b, q, s, z, leaf                                     # their memory goes to the next calls
+        torch.cuda.synchronize()
+        return out
+
+    want = chain(True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+
+
+@pytest.mark.gpu
+def test_a_graph_whose_branches_meet(dev):
+    """Captured calls after a fork and a join: launches with several predecessors."""
+    g = gen(17)
+    x, w = make(g, 24, 256), make(g, 256, 256, scale=1 / 16)
+
+    def work(side):
+        a = npu.npu_linear_act(x, w, activation="silu")
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = npu.npu_linear_act(a, w, activation="gelu")
+        c = npu.npu_gated_ffn(a, torch.cat((w, w), 1), w)
+        here.wait_stream(side)
+        return npu.npu_linear_act(c, w, residual=b)
+
+    side = torch.cuda.Stream()
+    want = work(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(side)
+    for _ in range(20):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(dev):
     """Calls that overlap on two streams share nothing."""
     a, b = _step_inputs(700, seed=1), _step_inputs(90, seed=2)

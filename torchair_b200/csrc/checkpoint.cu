@@ -6,8 +6,30 @@
 // flight, loads first, the values in their raw form until they are quantised.  When rows are whole numbers of blocks and lie
 // back to back, the matrix is one long row and no division is left in the loop.
 #include "dense_math.cuh"
+#include "ptx_sm100.cuh"
 
 namespace tab {
+
+// Every kernel here is launched so that it may begin while the launch before it on the stream still runs, and waits for that one's end
+// first of all; the launch after it may then begin in the same way.
+__device__ __forceinline__ void after_previous() {
+  ptx::dependency_wait();
+  ptx::launch_dependents();
+}
+
+template <typename... Params, typename... Args>
+static void launch(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);      // errors are picked up by check_launch
+}
 
 constexpr int kCkThreads = 256;
 constexpr int kCkUnroll = 4;
@@ -53,6 +75,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kCkThreads, VEC ? kCkQuantCtas : 2) checkpoint_quant_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
                                                                                          int64_t cols, int8_t* __restrict__ q, int64_t ldq,
                                                                                          float* __restrict__ scale, int64_t lds) {
+  after_previous();
   const int lane = threadIdx.x & 31;
   const int64_t blocks = (cols + 63) / 64;
   const int64_t chunks = (blocks + kCkChunk - 1) / kCkChunk;
@@ -107,6 +130,7 @@ __global__ void __launch_bounds__(kCkThreads, VEC ? kCkQuantCtas : 2) checkpoint
 template <typename T>
 __global__ void __launch_bounds__(kCkThreads, kCkQuantCtas) checkpoint_quant_flat_kernel(const T* __restrict__ x, int blocks, int8_t* __restrict__ q,
                                                                               float* __restrict__ scale) {
+  after_previous();
   const int lane = threadIdx.x & 31;
   const int sub = lane >> 3, part = lane & 7;
   const int step = gridDim.x * (kCkThreads / 32) * kCkChunk;
@@ -154,6 +178,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
                                                                         int64_t lds, int64_t rows, int64_t cols, T* __restrict__ y,
                                                                         int64_t ldy, int64_t pad_cols) {
+  after_previous();
   const int lane = threadIdx.x & 31;
   const int64_t blocks = (pad_cols + 63) / 64;
   const int64_t chunks = (blocks + kCkChunk - 1) / kCkChunk;
@@ -239,6 +264,7 @@ __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(cons
                                                               const T* __restrict__ keep, const int8_t* __restrict__ keep_q,
                                                               const float* __restrict__ keep_scale, int64_t keep_ld, T* __restrict__ dz,
                                                               float* __restrict__ sums) {
+  after_previous();
   __shared__ float red[kAgRows][kAgCols + 4];
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kAgCols + cl * 8;
@@ -294,6 +320,7 @@ __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(cons
 
 template <typename T>
 __global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ sums, int64_t splits, int64_t N, T* __restrict__ out) {
+  after_previous();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (c >= N) return;
   float s = 0.f;
@@ -318,6 +345,7 @@ struct CopyList {
 };
 
 __global__ void __launch_bounds__(256) copy_2d_kernel(const __grid_constant__ CopyList list) {
+  after_previous();
   __shared__ __align__(16) uint16_t tile[64][72];
   for (int t = blockIdx.x; t < list.tiles; t += gridDim.x) {
     int k = 0;
@@ -370,7 +398,7 @@ template <typename T, bool VEC>
 static void launch_quant(const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale, int64_t lds, cudaStream_t st) {
   const int64_t chunks = ((cols + 63) / 64 + kCkChunk - 1) / kCkChunk;
   const int grid = grid_for((rows * chunks + kCkThreads / 32 - 1) / (kCkThreads / 32), VEC ? kCkQuantCtas : 2);
-  checkpoint_quant_kernel<T, VEC><<<grid, kCkThreads, 0, st>>>(static_cast<const T*>(x), ldx, rows, cols, q, ldq, scale, lds);
+  launch(checkpoint_quant_kernel<T, VEC>, grid, kCkThreads, st, static_cast<const T*>(x), ldx, rows, cols, q, ldq, scale, lds);
 }
 
 template <typename T, bool VEC>
@@ -378,7 +406,7 @@ static void launch_dequant(const int8_t* q, int64_t ldq, const float* scale, int
                            int64_t pad_cols, cudaStream_t st) {
   const int64_t chunks = ((pad_cols + 63) / 64 + kCkChunk - 1) / kCkChunk;
   const int grid = grid_for((rows * chunks + kCkThreads / 32 - 1) / (kCkThreads / 32), 8);
-  checkpoint_dequant_kernel<T, VEC><<<grid, kCkThreads, 0, st>>>(q, ldq, scale, lds, rows, cols, static_cast<T*>(y), ldy, pad_cols);
+  launch(checkpoint_dequant_kernel<T, VEC>, grid, kCkThreads, st, q, ldq, scale, lds, rows, cols, static_cast<T*>(y), ldy, pad_cols);
 }
 
 // slices of the rows: as many as keep all CTAs resident at once, at least 64 rows each
@@ -418,8 +446,8 @@ extern "C" int tab_checkpoint_quant(const void* x, int dtype, int64_t ldx, int64
   if (vec && rows == 1 && cols % 64 == 0 && cols / 64 < (1LL << 30) && dtype != TAB_F32) {
     const int n = (int)(cols / 64);
     const int grid = grid_for((n + kCkChunk * (kCkThreads / 32) - 1) / (kCkChunk * (kCkThreads / 32)), kCkQuantCtas);
-    if (dtype == TAB_BF16) checkpoint_quant_flat_kernel<<<grid, kCkThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(x), n, q, scale);
-    else checkpoint_quant_flat_kernel<<<grid, kCkThreads, 0, st>>>(static_cast<const __half*>(x), n, q, scale);
+    if (dtype == TAB_BF16) launch(checkpoint_quant_flat_kernel<__nv_bfloat16>, grid, kCkThreads, st, static_cast<const __nv_bfloat16*>(x), n, q, scale);
+    else launch(checkpoint_quant_flat_kernel<__half>, grid, kCkThreads, st, static_cast<const __half*>(x), n, q, scale);
     return check_launch(op);
   }
 #define TAB_CQ(T) vec ? launch_quant<T, true>(x, ldx, rows, cols, q, ldq, scale, lds, st) : launch_quant<T, false>(x, ldx, rows, cols, q, ldq, scale, lds, st)
@@ -479,7 +507,7 @@ extern "C" int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, 
   const dim3 grid((unsigned)((N + kAgCols - 1) / kAgCols), (unsigned)act_grad_splits(M, N));
   cudaStream_t st = as_stream(stream);
 #define TAB_AG(T, K8) \
-  act_grad_kernel<T, K8><<<grid, kAgThreads, 0, st>>>(static_cast<const T*>(dy), lddy, M, N, act, static_cast<const T*>(keep), keep_q, keep_scale, \
+  launch(act_grad_kernel<T, K8>, grid, kAgThreads, st, static_cast<const T*>(dy), lddy, M, N, act, static_cast<const T*>(keep), keep_q, keep_scale, \
                                                       keep_ld, static_cast<T*>(dz), column_sums)
   if (dtype == TAB_BF16) {
     if (keep_q) TAB_AG(__nv_bfloat16, true); else TAB_AG(__nv_bfloat16, false);
@@ -496,8 +524,8 @@ extern "C" int tab_column_sums(const float* column_sums, int64_t splits, int64_t
   if (dtype != TAB_BF16 && dtype != TAB_F16) return fail(TAB_ERR_UNSUPPORTED, "%s: dtype %d (want 5 or 15)", op, dtype);
   if (!column_sums || !out) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
   const unsigned grid = (unsigned)((N + 255) / 256);
-  if (dtype == TAB_BF16) column_sums_kernel<<<grid, 256, 0, as_stream(stream)>>>(column_sums, splits, N, static_cast<__nv_bfloat16*>(out));
-  else column_sums_kernel<<<grid, 256, 0, as_stream(stream)>>>(column_sums, splits, N, static_cast<__half*>(out));
+  if (dtype == TAB_BF16) launch(column_sums_kernel<__nv_bfloat16>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__nv_bfloat16*>(out));
+  else launch(column_sums_kernel<__half>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__half*>(out));
   return check_launch(op);
 }
 
@@ -532,6 +560,6 @@ extern "C" int tab_copy_2d(const tab_copy* copies, int count, tab_stream_t strea
   }
   if (tiles == 0) return TAB_OK;
   list.tiles = (int)tiles;
-  copy_2d_kernel<<<grid_for(tiles, 8), 256, 0, as_stream(stream)>>>(list);
+  launch(copy_2d_kernel, grid_for(tiles, 8), 256, as_stream(stream), list);
   return check_launch(op);
 }

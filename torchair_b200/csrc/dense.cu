@@ -100,7 +100,7 @@ static int allow_smem(const char* op, F* kernel, int bytes, std::atomic<unsigned
 }
 
 template <typename F>
-static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int smem, int cluster, bool under_previous, const CUtensorMap& ma,
+static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int smem, int cluster, const CUtensorMap& ma,
                           const CUtensorMap& mb, const DenseParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
@@ -115,7 +115,7 @@ static int launch_cluster(const char* op, F* kernel, int ctas, int threads, int 
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = under_previous ? 2 : 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -148,8 +148,7 @@ static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMa
     p.tile_begin = 0;
     p.tile_end = (int)whole;
     p.split = 1;
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes<EPI>, 2, p.beside != 0, ma,
-                        mb, p, st);
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, false>, 2 * (int)(whole < pairs ? whole : pairs), kDpThreads, kDpSmemBytes<EPI>, 2, ma, mb, p, st);
     if (rc != TAB_OK) return rc;
   }
   if (rest > 0) {
@@ -157,9 +156,8 @@ static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMa
     p.tile_begin = (int)whole;
     p.tile_end = (int)tiles;
     p.split = split;
-    // both launches read the same operands and write different tiles: the second may fill SMs that the first has left
-    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes<EPI>, 2 * split, whole > 0 || p.beside != 0, ma, mb,
-                        p, st);
+    if (whole > 0) p.beside = 1;      // both launches read the same operands and write different tiles: the second may fill SMs that the first has left
+    rc = launch_cluster(op, dense_pair_kernel<T, EPI, true>, 2 * split * (int)rest, kDpThreads, kDpSmemBytes<EPI>, 2 * split, ma, mb, p, st);
   }
   return rc;
 }
@@ -243,7 +241,7 @@ static int launch_narrow_t(const char* op, const CUtensorMap& mw, const CUtensor
   const int rc = allow_smem(op, dense_narrow_kernel<T, EPI, WIDE>, dense_narrow_smem(true), done);
   if (rc != TAB_OK) return rc;
   return launch_cluster(op, dense_narrow_kernel<T, EPI, WIDE>, p.row_tiles * p.col_tiles * p.split, dense_narrow_threads(WIDE), smem, p.split,
-                        p.dependent != 0 || p.beside != 0, mw, mx, p, st);
+                        mw, mx, p, st);
 }
 
 template <int EPI>

@@ -50,8 +50,11 @@ struct DenseParams {
   void* dgate;           // kEpiGluGrad: d(gate) in columns [0, N), d(up) in [N, 2 N) of rows of 2 N values
   int split;             // CTAs (dense_pair.cuh: pairs) of a cluster that share one tile's contraction
   int stages, nt;        // dense_narrow.cuh: shared-memory stages, token columns of a tile
-  int dependent;         // launched as dependent of the kernel that writes the token operand
-  int beside;            // may run beside the launch before it
+  // Every launch of these kernels may begin while the one before it on the stream still runs: it sets up its barriers and tensor
+  // memory, then waits for that one to end before it touches global memory, and only then lets the next launch begin.  (linear
+  // layers one after the other, 8 x 2048 -> 7168: 11.0 -> 9.6 us.)  Two kinds wait later:
+  int dependent;         // the launch before writes the token operand and nothing else of this one: weights are loaded ahead of the wait
+  int beside;            // nothing of this one is written or read by the launch before: waits only before it ends
   long long wait_cycles;
 };
 

@@ -15,8 +15,8 @@
 // A launch of this kernel is over in 5 to 15 us, so its start counts: the producer sets up its barriers and asks for the first
 // weights before the CTA's threads have met and tensor memory is allocated.
 //
-// A launch marked `dependent` (the second projection of a feed-forward block) may start while the kernel before it still
-// runs: it fills its ring with weights first and waits for that kernel only before it touches x.
+// A launch marked `dependent` (the second projection of a feed-forward block) fills its ring with weights before it waits for
+// the kernel that writes x.
 #pragma once
 
 #include "dense_common.cuh"
@@ -160,6 +160,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     ptx::fence_barrier_init();
     __syncwarp();
     if (ptx::elect_one()) {
+      if (!p.beside && !p.dependent) ptx::dependency_wait();
       const int mine = group_begin(rank + 1) - group_begin(rank);
       if (split > 1 && mine > 0) ptx::mbar_expect_tx(bar_recv, static_cast<uint32_t>(mine * split * kGroupFloats * 4));
       for (int i = 0; i < min(head, 2); ++i) load_w(i, kb0 + i);
@@ -173,7 +174,10 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   ptx::tc_fence_after();
   if (split > 1) ptx::cluster_arrive();                  // this CTA runs and its barriers exist
   const uint32_t tmem_base = *s_tmem;
-  ptx::launch_dependents();
+  if (!p.dependent) {
+    if (!p.beside) ptx::dependency_wait();
+    ptx::launch_dependents();
+  }
 
   // Two producer warps (the second is one that has nothing to do before the epilogue) take the blocks in turn: one alone needs
   // some 400 cycles for a block's wait and copies, more than the bytes do.
@@ -187,6 +191,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
       if (p.dependent) {
         ptx::dependency_wait();
+        ptx::launch_dependents();
         for (int i = odd; i < head; i += 2) load_x(i, kb0 + i);
       }
     }

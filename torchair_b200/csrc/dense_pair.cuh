@@ -553,6 +553,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   ptx::cluster_sync_all();          // both CTAs' barriers exist before anything signals across the pair
   ptx::tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  if (!p.beside) ptx::dependency_wait();
   ptx::launch_dependents();
 
   if (warp == 0) {
