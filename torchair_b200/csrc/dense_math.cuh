@@ -5,66 +5,160 @@
 
 namespace tab {
 
-// ---- activations ---------------------------------------------------------------------------------------------------------
-// fp32 throughout.  silu and the tanh form of GELU are both z * sigmoid(u): 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)), which
-// needs no cancelling sum for very negative z.
+// Two fp32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 from_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t splat(float a) { return f32x2(a, a); }
 
-__device__ __forceinline__ float sigmoid_f(float u) { return __fdividef(1.0f, 1.0f + __expf(-u)); }
+// ---- activations ---------------------------------------------------------------------------------------------------------
+// fp32 throughout, on pairs of values: the exponential and the reciprocal are the hardware's (2 and 1 units in the last place), all
+// else is two values to an instruction.  What they cost is instructions: 8192 x 7168 values of the GELU derivative from and to HBM
+// took 73 us one by one, 60 so (bytes: 54).  silu and the tanh form of GELU are both z * sigmoid(u): 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v)),
+// which needs no cancelling sum for very negative z.
+__device__ __forceinline__ uint64_t exp2_f32x2(uint64_t v) {
+  float2 f = from_f32x2(v);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+  return f32x2(f.x, f.y);
+}
+__device__ __forceinline__ uint64_t rcp_f32x2(uint64_t v) {
+  float2 f = from_f32x2(v);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+  return f32x2(f.x, f.y);
+}
 
 constexpr float kGeluC = 0.7978845608028654f;      // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 constexpr float kInvSqrt2 = 0.7071067811865476f;
 constexpr float kInvSqrt2Pi = 0.3989422804014327f;
 
+// 1 / (1 + 2^u)
+__device__ __forceinline__ uint64_t logistic2(uint64_t u) { return rcp_f32x2(add_f32x2(exp2_f32x2(u), splat(1.f))); }
+
 // Normal distribution function c = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), by Abramowitz and Stegun 7.1.26: with
 // x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2) within 1.5e-7.  The exponential serves
 // the derivative as well; erff takes about twice the instructions and a branch.
-__device__ __forceinline__ void normal_cdf(float z, float& c, float& e) {
-  const float t = __fdividef(1.0f, __fmaf_rn(0.3275911f * kInvSqrt2, fabsf(z), 1.0f));
-  e = __expf(-0.5f * z * z);
-  float q = __fmaf_rn(1.061405429f, t, -1.453152027f);
-  q = __fmaf_rn(q, t, 1.421413741f);
-  q = __fmaf_rn(q, t, -0.284496736f);
-  q = __fmaf_rn(q, t, 0.254829592f);
-  const float tail = 0.5f * q * t * e;             // the side away from zero
-  c = z < 0.f ? tail : 1.0f - tail;
+__device__ __forceinline__ void normal_cdf(uint64_t z, uint64_t& c, uint64_t& e) {
+  const float2 f = from_f32x2(z);
+  const uint64_t t = rcp_f32x2(fma_f32x2(f32x2(fabsf(f.x), fabsf(f.y)), splat(0.3275911f * kInvSqrt2), splat(1.f)));
+  e = exp2_f32x2(mul_f32x2(mul_f32x2(z, z), splat(-0.5f * kLog2e)));
+  uint64_t q = fma_f32x2(t, splat(0.5f * 1.061405429f), splat(0.5f * -1.453152027f));
+  q = fma_f32x2(q, t, splat(0.5f * 1.421413741f));
+  q = fma_f32x2(q, t, splat(0.5f * -0.284496736f));
+  q = fma_f32x2(q, t, splat(0.5f * 0.254829592f));
+  const uint64_t tail = mul_f32x2(mul_f32x2(q, t), e);             // the side away from zero
+  const float2 near = from_f32x2(fma_f32x2(tail, splat(-1.f), splat(1.f))), far = from_f32x2(tail);
+  c = f32x2(f.x < 0.f ? far.x : near.x, f.y < 0.f ? far.y : near.y);
 }
 
+// a = act(z), d = act'(z); what a caller does not use is not computed
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (ACT == TAB_ACT_RELU) return z < 0.f ? 0.f : z;     // NaN stays NaN
-  if constexpr (ACT == TAB_ACT_SILU) return z * sigmoid_f(z);
-  if constexpr (ACT == TAB_ACT_GELU) {
-    float c, e;
-    normal_cdf(z, c, e);
-    return z * c;
-  }
-  if constexpr (ACT == TAB_ACT_GELU_TANH) return z * sigmoid_f(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
-  return z;
-}
-
-// value and derivative
-template <int ACT>
-__device__ __forceinline__ void act_both(float z, float& a, float& d) {
+__device__ __forceinline__ void act_pair(uint64_t z, uint64_t& a, uint64_t& d) {
+  const uint64_t one = splat(1.f), minus = splat(-1.f);
   if constexpr (ACT == TAB_ACT_RELU) {
-    a = z < 0.f ? 0.f : z;
-    d = z <= 0.f ? 0.f : z > 0.f ? 1.f : z;                          // in the derivative too
+    const float2 f = from_f32x2(z);
+    a = f32x2(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);       // NaN stays NaN, in the derivative too
+    d = f32x2(f.x <= 0.f ? 0.f : f.x > 0.f ? 1.f : f.x, f.y <= 0.f ? 0.f : f.y > 0.f ? 1.f : f.y);
   } else if constexpr (ACT == TAB_ACT_SILU) {
-    const float s = sigmoid_f(z);
-    a = z * s;
-    d = s * (1.0f + z * (1.0f - s));
+    const uint64_t s = logistic2(mul_f32x2(z, splat(-kLog2e)));
+    a = mul_f32x2(z, s);
+    d = mul_f32x2(s, fma_f32x2(z, fma_f32x2(s, minus, one), one));                 // s (1 + z (1 - s))
   } else if constexpr (ACT == TAB_ACT_GELU) {
-    float c, e;
+    uint64_t c, e;
     normal_cdf(z, c, e);
-    a = z * c;
-    d = c + z * kInvSqrt2Pi * e;
+    a = mul_f32x2(z, c);
+    d = fma_f32x2(mul_f32x2(z, splat(kInvSqrt2Pi)), e, c);
   } else if constexpr (ACT == TAB_ACT_GELU_TANH) {
-    const float s = sigmoid_f(2.0f * kGeluC * z * (1.0f + kGeluA * z * z));
-    a = z * s;
-    d = s + z * s * (1.0f - s) * (2.0f * kGeluC * (1.0f + 3.0f * kGeluA * z * z));
+    const uint64_t zz = mul_f32x2(z, z);
+    const uint64_t s = logistic2(mul_f32x2(z, fma_f32x2(zz, splat(-2.f * kLog2e * kGeluC * kGeluA), splat(-2.f * kLog2e * kGeluC))));
+    a = mul_f32x2(z, s);
+    // s + z s (1 - s) 2 C (1 + 3 A z^2)
+    d = fma_f32x2(mul_f32x2(a, fma_f32x2(s, minus, one)), fma_f32x2(zz, splat(6.f * kGeluC * kGeluA), splat(2.f * kGeluC)), s);
   } else {
     a = z;
-    d = 1.f;
+    d = one;
+  }
+}
+
+// v[i] = act(v[i])
+template <int ACT, int N>
+__device__ __forceinline__ void act_values(float (&v)[N]) {
+  if constexpr (ACT == TAB_ACT_NONE) return;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    uint64_t a, d;
+    act_pair<ACT>(f32x2(v[i], v[i + 1]), a, d);
+    const float2 f = from_f32x2(a);
+    v[i] = f.x;
+    v[i + 1] = f.y;
+  }
+}
+
+// g[i] = act(g[i]) u[i]
+template <int ACT, int N>
+__device__ __forceinline__ void act_gate(float (&g)[N], const float (&u)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    uint64_t a, d;
+    act_pair<ACT>(f32x2(g[i], g[i + 1]), a, d);
+    const float2 f = from_f32x2(mul_f32x2(a, f32x2(u[i], u[i + 1])));
+    g[i] = f.x;
+    g[i + 1] = f.y;
+  }
+}
+
+// the same backwards: g, u, dh = gate, up values and d(act(gate) up) become d(gate) = dh u act'(gate), d(up) = dh act(gate) and act(gate) u
+template <int ACT, int N>
+__device__ __forceinline__ void act_gate_grad(float (&g)[N], float (&u)[N], float (&dh)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t up = f32x2(u[i], u[i + 1]), grad = f32x2(dh[i], dh[i + 1]);
+    uint64_t a, d;
+    act_pair<ACT>(f32x2(g[i], g[i + 1]), a, d);
+    const float2 dg = from_f32x2(mul_f32x2(mul_f32x2(grad, up), d)), du = from_f32x2(mul_f32x2(grad, a)), h = from_f32x2(mul_f32x2(a, up));
+    g[i] = dg.x;
+    g[i + 1] = dg.y;
+    u[i] = du.x;
+    u[i + 1] = du.y;
+    dh[i] = h.x;
+    dh[i + 1] = h.y;
+  }
+}
+
+// g[i] *= act'(z[i])
+template <int ACT, int N>
+__device__ __forceinline__ void act_slope(float (&g)[N], const float (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    uint64_t a, d;
+    act_pair<ACT>(f32x2(z[i], z[i + 1]), a, d);
+    const float2 f = from_f32x2(mul_f32x2(f32x2(g[i], g[i + 1]), d));
+    g[i] = f.x;
+    g[i + 1] = f.y;
   }
 }
 
@@ -98,28 +192,6 @@ __device__ __forceinline__ RowQuant make_block_quant(float amax, bool finite) {
     rq.exact = false;
   }
   return rq;                         // quant8 gives zeros where !(scale > 0): NaN included
-}
-
-// Two fp32 operations in one instruction, each rounded as the single one is.
-__device__ __forceinline__ uint64_t f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // quant8 (the correctly rounded quotient, rounded half to even, in the low bytes) on pairs of values.

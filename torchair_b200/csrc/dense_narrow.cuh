@@ -311,18 +311,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         kept8<T>(p, row, col, gate);
         kept8<T>(p, row, p.keep_up + col, up);
         sum_parts8(src, part_floats, split, v);
-        // h = a u, d(gate) = dh u a', d(up) = dh a; gate, up and v are overwritten in turn
-        with_act(act, [&](auto tag) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float a, d;
-            act_both<decltype(tag)::value>(gate[i], a, d);
-            const float h = a * up[i];
-            gate[i] = v[i] * up[i] * d;
-            up[i] = v[i] * a;
-            v[i] = h;
-          }
-        });
+        with_act(act, [&](auto tag) { act_gate_grad<decltype(tag)::value>(gate, up, v); });
         T* dz = static_cast<T*>(p.dgate) + row * 2 * ld + col;
         Elem<T>::store8(dz, gate);
         Elem<T>::store8(dz + p.N, up);
@@ -358,15 +347,9 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
       if (in) {
         if constexpr (EPI == kEpiGlu) {
-          with_act(act, [&](auto tag) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]) * u[i];
-          });
+          with_act(act, [&](auto tag) { act_gate<decltype(tag)::value>(v, u); });
         } else if (act != TAB_ACT_NONE) {
-          with_act(act, [&](auto tag) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = act_value<decltype(tag)::value>(v[i]);
-          });
+          with_act(act, [&](auto tag) { act_values<decltype(tag)::value>(v); });
         }
         if (epi_linear(EPI) && has_res) {
 #pragma unroll

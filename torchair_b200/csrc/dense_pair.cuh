@@ -359,10 +359,7 @@ struct TileEpilogue {
         patch_put<T>(side_patch, lane, v);
       }
       if (act != TAB_ACT_NONE)
-        with_act(act, [&](auto tag) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
-        });
+        with_act(act, [&](auto tag) { act_values<decltype(tag)::value>(v); });
       if (has_res) {
         float r[16];
         patch_get<T>(main_patch, lane, r);
@@ -419,10 +416,7 @@ struct TileEpilogue {
         patch_store<T>(pu, lane, static_cast<T*>(p.keep) + p.keep_up, p.keep_ld, row_base, p.M, col, p.N);
         __syncwarp();
       }
-      with_act(p.act, [&](auto tag) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) g[j] = act_value<decltype(tag)::value>(g[j]) * u[j];
-      });
+      with_act(p.act, [&](auto tag) { act_gate<decltype(tag)::value>(g, u); });
       patch_put<T>(pg, lane, g);
       __syncwarp();
       patch_store<T>(pg, lane, static_cast<T*>(p.out), p.N, row_base, p.M, col, p.N);
@@ -463,18 +457,7 @@ struct TileEpilogue {
         if (c + 16 < col_end) look_ahead(c + 16);
       }
       if (c + 16 >= col_end) acc.release(lane);
-      // h = a u, d(gate) = dh u a', d(up) = dh a; g, u and dh are overwritten in turn
-      with_act(p.act, [&](auto tag) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          float a, d;
-          act_both<decltype(tag)::value>(g[j], a, d);
-          const float h = a * u[j];
-          g[j] = dh[j] * u[j] * d;
-          u[j] = dh[j] * a;
-          dh[j] = h;
-        }
-      });
+      with_act(p.act, [&](auto tag) { act_gate_grad<decltype(tag)::value>(g, u, dh); });
       patch_put<T>(pg, lane, g);
       patch_put<T>(pu, lane, u);
       patch_put<T>(ph, lane, dh);
