@@ -501,6 +501,10 @@ TAB_API int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float* sc
 TAB_API int tab_act_grad_splits(int64_t M, int64_t N, size_t* splits);
 TAB_API int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, int64_t N, int act, const void* keep, const int8_t* keep_q,
                          const float* keep_scale, int64_t keep_ld, void* dz, float* column_sums, tab_stream_t stream);
+/* tab_two_column_sums: the column sums of a [M, Na] and, unless Nb is 0, of b [M, Nb] into out_a and out_b; `sums` has room for `splits`
+ *   rows of Na + Nb values (tab_act_grad_splits of all columns that a caller may want sums of: the order of the additions depends on it) */
+TAB_API int tab_two_column_sums(const void* a, int64_t lda, int64_t Na, const void* b, int64_t ldb, int64_t Nb, int dtype, int64_t M, float* sums,
+                                int64_t splits, void* out_a, void* out_b, tab_stream_t stream);
 TAB_API int tab_column_sums(const float* column_sums, int64_t splits, int64_t N, void* out, int dtype, tab_stream_t stream);
 typedef struct tab_copy {
   const void* src; /* device; strides and sizes in elements */

@@ -996,6 +996,12 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
         _lib.call("tab_act_grad", one, 64, 15, 4, 64, 0, n, n, n, 0, n, n, n)
     with pytest.raises(RuntimeError, match="null"):
         _lib.call("tab_act_grad", one, 64, 15, 4, 64, 4, n, n, n, 64, one, n, n)
+    sums = lambda **kw: [one, kw.get("lda", 64), kw.get("Na", 64), kw.get("b", one), 64, kw.get("Nb", 64), kw.get("dtype", 5), 4, one,  # noqa: E731
+                         kw.get("splits", 1), one, kw.get("out_b", one), n]
+    for kw, match in ((dict(b=n), "null"), (dict(out_b=n), "null"), (dict(lda=56), "shorter"), (dict(Na=60), "multiples of 8"), (dict(Na=0), "Na=0"),
+                      (dict(dtype=6), "dtype"), (dict(splits=0), "splits=0"), (dict(splits=1 << 16), "splits=65536")):
+        with pytest.raises(RuntimeError, match=match):
+            _lib.call("tab_two_column_sums", *sums(**kw))
     with pytest.raises(RuntimeError, match="256-byte"):
         _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 64, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, n, 0, n)
     with pytest.raises(RuntimeError, match="workspace"):

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const in
   }
 }
 
-// dz = dy act'(z) and partial column sums of dz.  A CTA owns 128 columns (16 lanes x 8) and a slice of the rows; 16 rows per
+// dz = dy act'(z) and partial column sums of dz (and of a second matrix: a block's two bias gradients in one launch).  A CTA owns 128 columns (16 lanes x 8) and a slice of the rows; 16 rows per
 // step, so a warp reads two rows' 256-byte segments.  The next step's values are loaded before this step's are used.  Column sums
 // stay in registers over the slice and are added over the 16 row lanes once, in a fixed order.  The slices are chosen so that all
 // CTAs are resident at once: with 1.4 turns of CTAs and no load ahead, 8192 x 7168 with GELU took 171 us, now 60 (its bytes: 54).
@@ -263,11 +263,21 @@ template <typename T, bool KEEP8>
 __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(const T* __restrict__ dy, int64_t lddy, int64_t M, int64_t N, int act,
                                                               const T* __restrict__ keep, const int8_t* __restrict__ keep_q,
                                                               const float* __restrict__ keep_scale, int64_t keep_ld, T* __restrict__ dz,
-                                                              float* __restrict__ sums) {
+                                                              float* __restrict__ sums, const T* __restrict__ more, int64_t ld_more, int64_t n_more) {
   after_previous();
   __shared__ float red[kAgRows][kAgCols + 4];
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kAgCols + cl * 8;
+  // CTAs behind those of dy take the columns of `more`, whose sums follow those of dy in a row of `sums`
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kAgCols, width = N + n_more;
+  const int64_t own = (N + kAgCols - 1) / kAgCols * kAgCols, behind = N;
+  const bool is_more = first >= own;
+  const int64_t begin = is_more ? first - own : first;
+  if (is_more) {
+    dy = more;
+    lddy = ld_more;
+    N = n_more;
+  }
+  const int64_t col = begin + cl * 8;
   const int64_t r_begin = M * blockIdx.y / gridDim.y, r_end = M * (blockIdx.y + 1) / gridDim.y;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (col < N && r_begin + rl < r_end) {
@@ -303,25 +313,26 @@ __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(cons
   for (int j = 0; j < 8; ++j) red[rl][cl * 8 + j] = acc[j];
   __syncthreads();
   if (threadIdx.x < kAgCols) {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * kAgCols + threadIdx.x;
+    const int64_t c = begin + threadIdx.x;
     if (c < N) {
       float s = 0.f;
 #pragma unroll
       for (int r = 0; r < kAgRows; ++r) s += red[r][threadIdx.x];
-      sums[static_cast<int64_t>(blockIdx.y) * N + c] = s;
+      sums[blockIdx.y * width + (is_more ? behind : 0) + c] = s;
     }
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ sums, int64_t splits, int64_t N, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ sums, int64_t splits, int64_t N, T* __restrict__ out,
+                                                          int64_t n_out, T* __restrict__ out_more) {
   after_previous();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (c >= N) return;
   float s = 0.f;
 #pragma unroll 8
   for (int64_t i = 0; i < splits; ++i) s += sums[i * N + c];
-  out[c] = Elem<T>::from_f32(s);
+  (c < n_out ? out + c : out_more + (c - n_out))[0] = Elem<T>::from_f32(s);
 }
 
 // Up to kMaxCopies 16-bit copies between any strides in one launch, 64 x 64 tiles through shared memory so that both sides run
@@ -503,7 +514,7 @@ extern "C" int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, 
   cudaStream_t st = as_stream(stream);
 #define TAB_AG(T, K8) \
   launch(act_grad_kernel<T, K8>, grid, kAgThreads, st, static_cast<const T*>(dy), lddy, M, N, act, static_cast<const T*>(keep), keep_q, keep_scale, \
-                                                      keep_ld, static_cast<T*>(dz), column_sums)
+         keep_ld, static_cast<T*>(dz), column_sums, nullptr, 0, 0)
   if (dtype == TAB_BF16) {
     if (keep_q) TAB_AG(__nv_bfloat16, true); else TAB_AG(__nv_bfloat16, false);
   } else {
@@ -519,9 +530,35 @@ extern "C" int tab_column_sums(const float* column_sums, int64_t splits, int64_t
   if (dtype != TAB_BF16 && dtype != TAB_F16) return fail(TAB_ERR_UNSUPPORTED, "%s: dtype %d (want 5 or 15)", op, dtype);
   if (!column_sums || !out) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
   const unsigned grid = (unsigned)((N + 255) / 256);
-  if (dtype == TAB_BF16) launch(column_sums_kernel<__nv_bfloat16>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__nv_bfloat16*>(out));
-  else launch(column_sums_kernel<__half>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__half*>(out));
+  if (dtype == TAB_BF16) launch(column_sums_kernel<__nv_bfloat16>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__nv_bfloat16*>(out), N, nullptr);
+  else launch(column_sums_kernel<__half>, grid, 256, as_stream(stream), column_sums, splits, N, static_cast<__half*>(out), N, nullptr);
   return check_launch(op);
+}
+
+extern "C" int tab_two_column_sums(const void* a, int64_t lda, int64_t Na, const void* b, int64_t ldb, int64_t Nb, int dtype, int64_t M, float* sums,
+                                   int64_t splits, void* out_a, void* out_b, tab_stream_t stream) {
+  const char* op = "two_column_sums";
+  if (M < 0 || Na <= 0 || Nb < 0 || M > kMaxDim || Na > (1LL << 24) || Nb > (1LL << 24) || splits < 1 || splits > 65535)
+    return fail(TAB_ERR_BAD_ARG, "%s: M=%lld Na=%lld Nb=%lld splits=%lld", op, (long long)M, (long long)Na, (long long)Nb, (long long)splits);
+  if (dtype != TAB_BF16 && dtype != TAB_F16) return fail(TAB_ERR_UNSUPPORTED, "%s: dtype %d (want 5 or 15)", op, dtype);
+  if ((M > 0 && (!a || (Nb > 0 && !b))) || !sums || !out_a || (Nb > 0 && !out_b)) return fail(TAB_ERR_BAD_ARG, "%s: null pointer", op);
+  if (Na % 8 != 0 || Nb % 8 != 0 || lda % 8 != 0 || ldb % 8 != 0 || !aligned16(a) || !aligned16(b))
+    return fail(TAB_ERR_ALIGNMENT, "%s: widths and leading dimensions must be multiples of 8, pointers 16-byte aligned", op);
+  if (M > 1 && (lda < Na || ldb < Nb)) return fail(TAB_ERR_BAD_ARG, "%s: a leading dimension is shorter than a row", op);
+  const dim3 grid((unsigned)((Na + kAgCols - 1) / kAgCols + (Nb + kAgCols - 1) / kAgCols), (unsigned)splits);
+  const unsigned grid2 = (unsigned)((Na + Nb + 255) / 256);
+  cudaStream_t st = as_stream(stream);
+#define TAB_TS(T)                                                                                                                                  \
+  launch(act_grad_kernel<T, false>, grid, kAgThreads, st, static_cast<const T*>(a), lda, M, Na, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, nullptr, \
+         sums, static_cast<const T*>(b), ldb, Nb);                                                                                                 \
+  launch(column_sums_kernel<T>, grid2, 256, st, sums, splits, Na + Nb, static_cast<T*>(out_a), Na, static_cast<T*>(out_b))
+  if (dtype == TAB_BF16) {
+    TAB_TS(__nv_bfloat16);
+  } else {
+    TAB_TS(__half);
+  }
+#undef TAB_TS
+  return check_launch(op, 2);
 }
 
 extern "C" int tab_copy_2d(const tab_copy* copies, int count, tab_stream_t stream) {

@@ -426,8 +426,19 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     }
   }
   if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}));
-  if (want[3]) act_grad(c, dz, 2 * inner8, 0, Kept(), false, true, db1);
-  if (want[4]) act_grad(c, dy, h8, 0, Kept(), false, true, db2);
+  if (want[3] || want[4]) {                // in slices that do not depend on which of them are wanted, and so neither do their sums
+    const Mat &first = want[3] ? dz : dy, &second = want[3] && want[4] ? dy : Mat();
+    const int64_t n1 = want[3] ? 2 * inner8 : h8, n2 = want[3] && want[4] ? h8 : 0;
+    size_t splits = 0;
+    ok(tab_act_grad_splits(m, 2 * inner8 + h8, &splits), "tab_act_grad_splits");
+    const Tensor parts = c.empty({static_cast<int64_t>(splits), n1 + n2}, at::kFloat);
+    if (want[3]) db1 = c.empty({1, 2 * inner8});
+    if (want[4]) db2 = c.empty({1, h8});
+    c.flush();
+    ok(tab_two_column_sums(first.ptr(), first.ld, n1, n2 ? second.ptr() : nullptr, second.ld, n2, dtype, m, static_cast<float*>(parts.data_ptr()),
+                           static_cast<int64_t>(splits), want[3] ? db1.data_ptr() : db2.data_ptr(), n2 ? db2.data_ptr() : nullptr, c.stream),
+       "tab_two_column_sums");
+  }
   // The products that are left depend on nothing but what is ordered before them: each may start in the SMs that the last turn of
   // the one before leaves idle.  Everything they touch stays allocated until all of them are launched.
   bool beside = false;
