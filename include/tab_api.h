@@ -489,6 +489,7 @@ TAB_API int tab_dense_status_reset(tab_stream_t stream);
  * zeros: scale 0, q 0; a block with a value that is not finite: scale NaN, q 0, so that it comes back as NaN).
  * x [rows, cols] of dtype 5, 6 or 15 with ldx elements between rows; q int8 [rows, ldq]; scale fp32 [rows, lds], lds >= ceil(cols / 64).
  * tab_checkpoint_dequant: y = q * scale, rounded once to dtype 5, 6 or 15; columns [cols, pad_cols) of y become 0.
+ *   beside_previous: as for tab_dense_matmul
  * tab_act_grad: dz[M, N] = dy[M, N] act'(z), z kept in 16 bits (keep) or 8 (keep_q, keep_scale); dz null: nothing is stored (then act
  *   must be 0).  column_sums null, or fp32 [splits, N]: partial column sums of dz, one row per slice of the rows, summed by
  *   tab_column_sums into out[N] of `dtype` in slice order; the number of slices is tab_act_grad_splits(M, N).
@@ -497,14 +498,15 @@ TAB_API int tab_dense_status_reset(tab_stream_t stream);
 TAB_API int tab_checkpoint_quant(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int8_t* q, int64_t ldq, float* scale,
                                  int64_t lds, tab_stream_t stream);
 TAB_API int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t lds, int64_t rows, int64_t cols, void* y,
-                                   int dtype, int64_t ldy, int64_t pad_cols, tab_stream_t stream);
+                                   int dtype, int64_t ldy, int64_t pad_cols, int beside_previous, tab_stream_t stream);
 TAB_API int tab_act_grad_splits(int64_t M, int64_t N, size_t* splits);
 TAB_API int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, int64_t N, int act, const void* keep, const int8_t* keep_q,
                          const float* keep_scale, int64_t keep_ld, void* dz, float* column_sums, tab_stream_t stream);
 /* tab_two_column_sums: the column sums of a [M, Na] and, unless Nb is 0, of b [M, Nb] into out_a and out_b; `sums` has room for `splits`
- *   rows of Na + Nb values (tab_act_grad_splits of all columns that a caller may want sums of: the order of the additions depends on it) */
+ *   rows of Na + Nb values (tab_act_grad_splits of all columns that a caller may want sums of: the order of the additions depends on it);
+ *   beside_previous: as for tab_dense_matmul */
 TAB_API int tab_two_column_sums(const void* a, int64_t lda, int64_t Na, const void* b, int64_t ldb, int64_t Nb, int dtype, int64_t M, float* sums,
-                                int64_t splits, void* out_a, void* out_b, tab_stream_t stream);
+                                int64_t splits, void* out_a, void* out_b, int beside_previous, tab_stream_t stream);
 TAB_API int tab_column_sums(const float* column_sums, int64_t splits, int64_t N, void* out, int dtype, tab_stream_t stream);
 typedef struct tab_copy {
   const void* src; /* device; strides and sizes in elements */

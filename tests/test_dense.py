@@ -989,7 +989,7 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     with pytest.raises(RuntimeError, match="too short"):
         _lib.call("tab_checkpoint_quant", one, 15, 32, 4, 64, one, 64, one, 1, n)
     with pytest.raises(RuntimeError, match="too short"):
-        _lib.call("tab_checkpoint_dequant", one, 64, one, 0, 4, 64, one, 15, 64, 64, n)
+        _lib.call("tab_checkpoint_dequant", one, 64, one, 0, 4, 64, one, 15, 64, 64, 0, n)
     with pytest.raises(RuntimeError, match="dtype"):
         _lib.call("tab_checkpoint_quant", one, 1, 64, 4, 64, one, 64, one, 1, n)
     with pytest.raises(RuntimeError, match="nothing to compute"):
@@ -997,7 +997,7 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     with pytest.raises(RuntimeError, match="null"):
         _lib.call("tab_act_grad", one, 64, 15, 4, 64, 4, n, n, n, 64, one, n, n)
     sums = lambda **kw: [one, kw.get("lda", 64), kw.get("Na", 64), kw.get("b", one), 64, kw.get("Nb", 64), kw.get("dtype", 5), 4, one,  # noqa: E731
-                         kw.get("splits", 1), one, kw.get("out_b", one), n]
+                         kw.get("splits", 1), one, kw.get("out_b", one), 0, n]
     for kw, match in ((dict(b=n), "null"), (dict(out_b=n), "null"), (dict(lda=56), "shorter"), (dict(Na=60), "multiples of 8"), (dict(Na=0), "Na=0"),
                       (dict(dtype=6), "dtype"), (dict(splits=0), "splits=0"), (dict(splits=1 << 16), "splits=65536")):
         with pytest.raises(RuntimeError, match=match):

@@ -68,10 +68,10 @@ SIGNATURES = {
     "tab_dense_status": [POINTER(c_int), _P],
     "tab_dense_status_reset": [_P],
     "tab_checkpoint_quant": [_P, _I, _L, _L, _L, _P, _L, _P, _L, _P],
-    "tab_checkpoint_dequant": [_P, _L, _P, _L, _L, _L, _P, _I, _L, _L, _P],
+    "tab_checkpoint_dequant": [_P, _L, _P, _L, _L, _L, _P, _I, _L, _L, _I, _P],
     "tab_act_grad_splits": [_L, _L, POINTER(c_size_t)],
     "tab_act_grad": [_P, _L, _I, _L, _L, _I, _P, _P, _P, _L, _P, _P, _P],
-    "tab_two_column_sums": [_P, _L, _L, _P, _L, _L, _I, _L, _P, _L, _P, _P, _P],
+    "tab_two_column_sums": [_P, _L, _L, _P, _L, _L, _I, _L, _P, _L, _P, _P, _I, _P],
     "tab_column_sums": [_P, _L, _L, _P, _I, _P],
     "tab_copy_2d": [_P, _I, _P],
 }

@@ -11,10 +11,14 @@
 namespace tab {
 
 // Every kernel here is launched so that it may begin while the launch before it on the stream still runs, and waits for that one's end
-// first of all; the launch after it may then begin in the same way.
-__device__ __forceinline__ void after_previous() {
-  ptx::dependency_wait();
+// first of all; the launch after it may then begin in the same way.  One that runs beside the launch before it (`beside`: nothing of
+// either is written by the other) fills the SMs that the other's last turn leaves idle, and waits before it ends.
+__device__ __forceinline__ void after_previous(int beside = 0) {
+  if (!beside) ptx::dependency_wait();
   ptx::launch_dependents();
+}
+__device__ __forceinline__ void end_after_previous() {
+  if (threadIdx.x == 0) ptx::dependency_wait();
 }
 
 template <typename... Params, typename... Args>
@@ -177,8 +181,8 @@ __global__ void __launch_bounds__(kCkThreads, kCkQuantCtas) checkpoint_quant_fla
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const int8_t* __restrict__ q, int64_t ldq, const float* __restrict__ scale,
                                                                         int64_t lds, int64_t rows, int64_t cols, T* __restrict__ y,
-                                                                        int64_t ldy, int64_t pad_cols) {
-  after_previous();
+                                                                        int64_t ldy, int64_t pad_cols, int beside) {
+  after_previous(beside);
   const int lane = threadIdx.x & 31;
   const int64_t blocks = (pad_cols + 63) / 64;
   const int64_t chunks = (blocks + kCkChunk - 1) / kCkChunk;
@@ -224,6 +228,7 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_dequant_kernel(const in
       }
     }
   }
+  end_after_previous();
 }
 
 // dz = dy act'(z) and partial column sums of dz (and of a second matrix: a block's two bias gradients in one launch).  A CTA owns 128 columns (16 lanes x 8) and a slice of the rows; 16 rows per
@@ -263,8 +268,9 @@ template <typename T, bool KEEP8>
 __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(const T* __restrict__ dy, int64_t lddy, int64_t M, int64_t N, int act,
                                                               const T* __restrict__ keep, const int8_t* __restrict__ keep_q,
                                                               const float* __restrict__ keep_scale, int64_t keep_ld, T* __restrict__ dz,
-                                                              float* __restrict__ sums, const T* __restrict__ more, int64_t ld_more, int64_t n_more) {
-  after_previous();
+                                                              float* __restrict__ sums, const T* __restrict__ more, int64_t ld_more, int64_t n_more,
+                                                              int beside) {
+  after_previous(beside);
   __shared__ float red[kAgRows][kAgCols + 4];
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
   // CTAs behind those of dy take the columns of `more`, whose sums follow those of dy in a row of `sums`
@@ -321,6 +327,7 @@ __global__ void __launch_bounds__(kAgThreads, kAgCtasPerSm) act_grad_kernel(cons
       sums[blockIdx.y * width + (is_more ? behind : 0) + c] = s;
     }
   }
+  end_after_previous();
 }
 
 template <typename T>
@@ -409,10 +416,10 @@ static void launch_quant(const void* x, int64_t ldx, int64_t rows, int64_t cols,
 
 template <typename T, bool VEC>
 static void launch_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t lds, int64_t rows, int64_t cols, void* y, int64_t ldy,
-                           int64_t pad_cols, cudaStream_t st) {
+                           int64_t pad_cols, int beside, cudaStream_t st) {
   const int64_t chunks = ((pad_cols + 63) / 64 + kCkChunk - 1) / kCkChunk;
   const int grid = grid_for((rows * chunks + kCkThreads / 32 - 1) / (kCkThreads / 32), 8);
-  launch(checkpoint_dequant_kernel<T, VEC>, grid, kCkThreads, st, q, ldq, scale, lds, rows, cols, static_cast<T*>(y), ldy, pad_cols);
+  launch(checkpoint_dequant_kernel<T, VEC>, grid, kCkThreads, st, q, ldq, scale, lds, rows, cols, static_cast<T*>(y), ldy, pad_cols, beside);
 }
 
 // slices of the rows: as many as keep all CTAs resident at once, at least 64 rows each
@@ -465,7 +472,7 @@ extern "C" int tab_checkpoint_quant(const void* x, int dtype, int64_t ldx, int64
 }
 
 extern "C" int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float* scale, int64_t lds, int64_t rows, int64_t cols, void* y,
-                                      int dtype, int64_t ldy, int64_t pad_cols, tab_stream_t stream) {
+                                      int dtype, int64_t ldy, int64_t pad_cols, int beside_previous, tab_stream_t stream) {
   const char* op = "checkpoint_dequant";
   if (rows < 0 || cols < 0 || pad_cols < cols || rows > kMaxDim || pad_cols > kMaxDim)
     return fail(TAB_ERR_BAD_ARG, "%s: rows=%lld cols=%lld pad_cols=%lld", op, (long long)rows, (long long)cols, (long long)pad_cols);
@@ -483,7 +490,7 @@ extern "C" int tab_checkpoint_dequant(const int8_t* q, int64_t ldq, const float*
     rows = 1;
   }
   cudaStream_t st = as_stream(stream);
-#define TAB_CD(T) vec ? launch_dequant<T, true>(q, ldq, scale, lds, rows, cols, y, ldy, pad_cols, st) : launch_dequant<T, false>(q, ldq, scale, lds, rows, cols, y, ldy, pad_cols, st)
+#define TAB_CD(T) vec ? launch_dequant<T, true>(q, ldq, scale, lds, rows, cols, y, ldy, pad_cols, beside_previous ? 1 : 0, st) : launch_dequant<T, false>(q, ldq, scale, lds, rows, cols, y, ldy, pad_cols, beside_previous ? 1 : 0, st)
   if (dtype == TAB_BF16) TAB_CD(__nv_bfloat16);
   else if (dtype == TAB_F16) TAB_CD(__half);
   else TAB_CD(float);
@@ -514,7 +521,7 @@ extern "C" int tab_act_grad(const void* dy, int64_t lddy, int dtype, int64_t M, 
   cudaStream_t st = as_stream(stream);
 #define TAB_AG(T, K8) \
   launch(act_grad_kernel<T, K8>, grid, kAgThreads, st, static_cast<const T*>(dy), lddy, M, N, act, static_cast<const T*>(keep), keep_q, keep_scale, \
-         keep_ld, static_cast<T*>(dz), column_sums, nullptr, 0, 0)
+         keep_ld, static_cast<T*>(dz), column_sums, nullptr, 0, 0, 0)
   if (dtype == TAB_BF16) {
     if (keep_q) TAB_AG(__nv_bfloat16, true); else TAB_AG(__nv_bfloat16, false);
   } else {
@@ -536,7 +543,7 @@ extern "C" int tab_column_sums(const float* column_sums, int64_t splits, int64_t
 }
 
 extern "C" int tab_two_column_sums(const void* a, int64_t lda, int64_t Na, const void* b, int64_t ldb, int64_t Nb, int dtype, int64_t M, float* sums,
-                                   int64_t splits, void* out_a, void* out_b, tab_stream_t stream) {
+                                   int64_t splits, void* out_a, void* out_b, int beside_previous, tab_stream_t stream) {
   const char* op = "two_column_sums";
   if (M < 0 || Na <= 0 || Nb < 0 || M > kMaxDim || Na > (1LL << 24) || Nb > (1LL << 24) || splits < 1 || splits > 65535)
     return fail(TAB_ERR_BAD_ARG, "%s: M=%lld Na=%lld Nb=%lld splits=%lld", op, (long long)M, (long long)Na, (long long)Nb, (long long)splits);
@@ -550,7 +557,7 @@ extern "C" int tab_two_column_sums(const void* a, int64_t lda, int64_t Na, const
   cudaStream_t st = as_stream(stream);
 #define TAB_TS(T)                                                                                                                                  \
   launch(act_grad_kernel<T, false>, grid, kAgThreads, st, static_cast<const T*>(a), lda, M, Na, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, nullptr, \
-         sums, static_cast<const T*>(b), ldb, Nb);                                                                                                 \
+         sums, static_cast<const T*>(b), ldb, Nb, beside_previous ? 1 : 0);                                                                                                 \
   launch(column_sums_kernel<T>, grid2, 256, st, sums, splits, Na + Nb, static_cast<T*>(out_a), Na, static_cast<T*>(out_b))
   if (dtype == TAB_BF16) {
     TAB_TS(__nv_bfloat16);

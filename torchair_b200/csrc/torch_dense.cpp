@@ -277,11 +277,11 @@ void keep_x(const Call& c, const Tensor& x, Kept& kept) {
 }
 
 // int8 [m, k] with its scales (no gaps) -> 16 bits, rows of a multiple of 8 values, zero behind k
-Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale) {
+Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale, bool beside = false) {
   const int64_t pitch = up(q.size(1), 8);
   Tensor y = c.empty({q.size(0), pitch});
   ok(tab_checkpoint_dequant(static_cast<const int8_t*>(q.data_ptr()), q.size(1), static_cast<const float*>(scale.data_ptr()), scale.size(1), q.size(0),
-                            q.size(1), y.data_ptr(), c.dtype, pitch, pitch, c.stream),
+                            q.size(1), y.data_ptr(), c.dtype, pitch, pitch, beside, c.stream),
      "tab_checkpoint_dequant");
   return {y, pitch, true};
 }
@@ -410,8 +410,12 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
   kept.values = kept_values;
   kept.scale = kept_scale;
   Mat dz{Tensor(), 2 * inner8, true}, hidden{Tensor(), inner8, true};
-  if (want[0] || want[1] || want[2] || want[3]) {
-    const Mat w2 = matrix_of(c, inner == inner8 ? weight2 : padded_weight2(c, weight2, inner8));
+  const bool any = want[0] || want[1] || want[2] || want[3];
+  // Launches that run beside one another: everything that one of them touches stays allocated until all of them are launched, for memory
+  // that is freed may be handed out again at once.
+  Mat w2;
+  if (any) {
+    w2 = matrix_of(c, inner == inner8 ? weight2 : padded_weight2(c, weight2, inner8));
     dz.t = c.empty({m, 2 * inner8});
     hidden.t = c.empty({m, inner8});
     c.flush();
@@ -425,22 +429,9 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
       c.flush();
     }
   }
-  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}));
-  if (want[3] || want[4]) {                // in slices that do not depend on which of them are wanted, and so neither do their sums
-    const Mat &first = want[3] ? dz : dy, &second = want[3] && want[4] ? dy : Mat();
-    const int64_t n1 = want[3] ? 2 * inner8 : h8, n2 = want[3] && want[4] ? h8 : 0;
-    size_t splits = 0;
-    ok(tab_act_grad_splits(m, 2 * inner8 + h8, &splits), "tab_act_grad_splits");
-    const Tensor parts = c.empty({static_cast<int64_t>(splits), n1 + n2}, at::kFloat);
-    if (want[3]) db1 = c.empty({1, 2 * inner8});
-    if (want[4]) db2 = c.empty({1, h8});
-    c.flush();
-    ok(tab_two_column_sums(first.ptr(), first.ld, n1, n2 ? second.ptr() : nullptr, second.ld, n2, dtype, m, static_cast<float*>(parts.data_ptr()),
-                           static_cast<int64_t>(splits), want[3] ? db1.data_ptr() : db2.data_ptr(), n2 ? db2.data_ptr() : nullptr, c.stream),
-       "tab_two_column_sums");
-  }
-  // The products that are left depend on nothing but what is ordered before them: each may start in the SMs that the last turn of
-  // the one before leaves idle.  Everything they touch stays allocated until all of them are launched.
+  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), any);
+  // What is left depends on nothing but what is ordered before it: each launch may start in the SMs that the last turn of the one before
+  // leaves idle.
   bool beside = false;
   if (want[2]) {
     dw2 = weight_grad(c, hidden, dy, inner, h, weight2, beside);
@@ -451,7 +442,24 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h, 2 * inner8, dx, Tensor(), Tensor(), 0, Kept(), beside);
     beside = true;
   }
-  if (want[1]) dw1 = cut_halves(c, weight_grad(c, xm, dz, h, 2 * inner8, weight1, beside), inner);
+  if (want[1]) {
+    dw1 = weight_grad(c, xm, dz, h, 2 * inner8, weight1, beside);
+    beside = true;
+  }
+  if (want[3] || want[4]) {                // in slices that do not depend on which of them are wanted, and so neither do their sums
+    const Mat &first = want[3] ? dz : dy, &second = want[3] && want[4] ? dy : Mat();
+    const int64_t n1 = want[3] ? 2 * inner8 : h8, n2 = want[3] && want[4] ? h8 : 0;
+    size_t splits = 0;
+    ok(tab_act_grad_splits(m, 2 * inner8 + h8, &splits), "tab_act_grad_splits");
+    const Tensor parts = c.empty({static_cast<int64_t>(splits), n1 + n2}, at::kFloat);
+    if (want[3]) db1 = c.empty({1, 2 * inner8});
+    if (want[4]) db2 = c.empty({1, h8});
+    c.flush();
+    ok(tab_two_column_sums(first.ptr(), first.ld, n1, n2 ? second.ptr() : nullptr, second.ld, n2, dtype, m, static_cast<float*>(parts.data_ptr()),
+                           static_cast<int64_t>(splits), want[3] ? db1.data_ptr() : db2.data_ptr(), n2 ? db2.data_ptr() : nullptr, beside, c.stream),
+       "tab_two_column_sums");
+  }
+  if (want[1]) dw1 = cut_halves(c, dw1, inner);
   if (want[3]) db1 = cut_halves(c, db1, inner).reshape({2 * inner});
   if (want[4]) db2 = cut_row(c, db2, h);
   c.flush();
@@ -619,7 +627,7 @@ Tensor ck_dequant_cuda(const Tensor& q, const Tensor& scale, int64_t output_dtyp
     const int64_t cols = q.size(-1);
     const Tensor qc = q.contiguous(), sc = scale.contiguous();
     ok(tab_checkpoint_dequant(static_cast<const int8_t*>(qc.data_ptr()), cols, static_cast<const float*>(sc.data_ptr()), sc.size(-1), q.numel() / cols, cols,
-                              y.data_ptr(), c.dtype, cols, cols, c.stream),
+                              y.data_ptr(), c.dtype, cols, cols, 0, c.stream),
        "tab_checkpoint_dequant");
   }
   return y;
