@@ -52,14 +52,6 @@ __device__ __forceinline__ void sum_parts8(const float* src, int part_floats, in
   v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-template <typename T>
-__device__ __forceinline__ void add8(float (&v)[8], const T* src) {
-  float t[8];
-  Elem<T>::load8(src, t);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += t[i];
-}
-
 // Keeps 8 values of a row for the backward pass; the 8 lanes of an aligned group hold one 64-value block.  Every lane of the
 // warp calls it; `in` = these values exist, `live` = this lane's group of 64 has a place in the kept row.
 template <typename T>
@@ -168,6 +160,9 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     __syncwarp();
   } else if (warp == 1) {
     ptx::tmem_alloc<kTmemCols>(ptx::smem_u32(s_tmem));
+  } else if (threadIdx.x == 64) {
+    ptx::prefetch_tensormap(&tm_w);
+    ptx::prefetch_tensormap(&tm_x);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -178,6 +173,44 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     if (!p.beside) ptx::dependency_wait();
     ptx::launch_dependents();
   }
+
+  // What this thread will need in the epilogue: its columns are the same in every step (a step is an even number of groups), so the
+  // bias is fetched once, and the residual of the first step with it, while the products run.
+  constexpr bool ragged = EPI == kEpiLinearAny;
+  static_assert(kThreads / 8 % 2 == 0, "steps of an even number of groups");
+  const bool has_bias = p.bias != nullptr, has_res = epi_linear(EPI) && p.residual != nullptr;
+  const int n_out = ragged ? p.n_out : p.N;
+  const int64_t ld = n_out;
+  const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual);
+  const int g_begin = group_begin(rank), g_end = group_begin(rank + 1), g_first = g_begin + static_cast<int>(threadIdx.x >> 3);
+  const int col = ft * (EPI == kEpiGlu ? 64 : 128) + (kGroups == 2 ? (g_first & 1) * 64 : 0) + static_cast<int>(threadIdx.x & 7) * 8;
+  const bool col_in = col < p.N;
+  auto fetch8 = [&](const T* line, uint4& out) {           // 8 values from column `col` of a line
+    if constexpr (ragged) {
+      const unsigned short* from = reinterpret_cast<const unsigned short*>(line) + col;
+      uint32_t t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = col + i < n_out ? __ldcg(from + i) : 0u;
+      out = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+    } else {
+      out = __ldcg(reinterpret_cast<const uint4*>(line + col));
+    }
+  };
+  auto unpack_8 = [](const uint4& x, float (&v)[8]) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<T>(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  };
+  uint4 bias_v = make_uint4(0u, 0u, 0u, 0u), bias_up = bias_v, res_v = bias_v;
+  if (EPI != kEpiGluGrad && has_bias && col_in) {
+    fetch8(bias, bias_v);
+    if (EPI == kEpiGlu) fetch8(bias + p.N, bias_up);
+  }
+  if (has_res && col_in && g_first < g_end) fetch8(res + (row0 + g_first / kGroups) * ld, res_v);
 
   // Two producer warps (the second is one that has nothing to do before the epilogue) take the blocks in turn: one alone needs
   // some 400 cycles for a block's wait and copies, more than the bytes do.
@@ -268,7 +301,6 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   __syncthreads();
 
   // ---- the parts go to the CTAs that finish their rows ----
-  const int g_begin = group_begin(rank), g_end = group_begin(rank + 1);
   const int part_floats = split > 1 ? (g_end - g_begin) * kGroupFloats : 0;
   float* sums = part + g_begin * kGroupFloats;           // this CTA's groups in the first part
   if (split > 1) {
@@ -288,12 +320,8 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
 
   // ---- add up and finish: 8 lanes x 8 features to a group ----
-  const bool has_bias = p.bias != nullptr, has_res = p.residual != nullptr, keeps = p.keep != nullptr || p.keep_q != nullptr;
+  const bool keeps = p.keep != nullptr || p.keep_q != nullptr;
   const int act = p.act;
-  constexpr bool ragged = EPI == kEpiLinearAny;
-  const int n_out = ragged ? p.n_out : p.N;
-  const int64_t ld = n_out;
-  const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual);
   T* out = static_cast<T*>(p.out);
   const int lane8 = (threadIdx.x & 7) * 8;
 #pragma unroll 2
@@ -301,8 +329,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     const int g = g0 + static_cast<int>(threadIdx.x >> 3);
     const bool mine = g < g_end;
     const int64_t row = row0 + (mine ? g / kGroups : 0);
-    const int col = ft * (EPI == kEpiGlu ? 64 : 128) + (mine ? g % kGroups : 0) * 64 + lane8;
-    const bool in = mine && col < p.N;
+    const bool in = mine && col_in;
     float* src = sums + (mine ? g - g_begin : 0) * kGroupFloats + lane8;
     float v[8];
     if constexpr (EPI == kEpiGluGrad) {
@@ -320,24 +347,22 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     } else {
       float u[8], r[8];
       if (in) {
-        const int64_t at = row * ld + col;
-        if (epi_linear(EPI) && has_res) {
-          if (ragged) load8_any(res + row * ld, col, n_out, r); else Elem<T>::load8(res + at, r);
+        if (has_res) {
+          if (g0 > g_begin) fetch8(res + row * ld, res_v);
+          unpack_8(res_v, r);
         }
         sum_parts8(src, part_floats, split, v);
+        if constexpr (EPI == kEpiGlu) sum_parts8(src + 64, part_floats, split, u);
         if (has_bias) {
-          if (ragged) {
-            float b[8];
-            load8_any(bias, col, n_out, b);
+          float b[8];
+          unpack_8(bias_v, b);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += b[i];
-          } else {
-            add8(v, bias + col);
+          for (int i = 0; i < 8; ++i) v[i] += b[i];
+          if constexpr (EPI == kEpiGlu) {
+            unpack_8(bias_up, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] += b[i];
           }
-        }
-        if constexpr (EPI == kEpiGlu) {
-          sum_parts8(src + 64, part_floats, split, u);
-          if (has_bias) add8(u, bias + p.N + col);
         }
       }
       if (keeps) {
@@ -351,7 +376,7 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
         } else if (act != TAB_ACT_NONE) {
           with_act(act, [&](auto tag) { act_values<decltype(tag)::value>(v); });
         }
-        if (epi_linear(EPI) && has_res) {
+        if (has_res) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += r[i];
         }
