@@ -195,12 +195,13 @@ static NarrowPlan narrow_plan(int64_t M, int64_t N, int num_kb, int epi, bool x_
     best.nt = x_mn ? 64 : M <= 16 ? 16 : M <= 32 ? 32 : 64;       // (boxes of 64 rows where x is contiguous along its rows)
     best.row_tiles = 1;
     best.col_tiles = (int)col_tiles;
-    // CTAs per tile: as many as fill the SMs, two of them on some.  Measured over weights that come from HBM (us): one row, 56 tiles
-    // of K = 2048: 10.4 / 9.3 / 9.7 / 11.4 with 2 / 3 / 4 / 5 CTAs; 32 tiles of K = 7168: 15.6 / 14.8 / 14.4 / 14.2 with 3 / 4 / 5 / 6;
-    // with 64 rows the parts to exchange weigh more: 56 tiles 13.1 / 13.1 / 13.3 with 2 / 3 / 4.
-    int64_t split = (best.nt <= 32 ? 176 : 132) / col_tiles;
+    // CTAs per tile: up to 32 rows as many as put two on half of the SMs.  Measured in a row over weights that come from HBM (us): 8 rows,
+    // 56 tiles of K = 2048: 9.9 / 9.5 / 9.1 / 10.7 with 2 / 3 / 4 / 5 CTAs; 16 rows, 32 tiles of K = 4096: 11.1 / 10.7 / 10.4 / 10.0 / 9.9
+    // with 3 / 4 / 5 / 7 / 8.  With 64 rows the parts to exchange weigh more, 56 tiles of K = 2048: 11.7 / 12.9 / 12.2 / 14.3 with 2 / 3 /
+    // 4 / 5.  A part of fewer than 5 blocks does not pay: 32 rows, 32 tiles of K = 1408: 6.8 / 6.5 / 7.3 with 3 / 4 / 5.
+    int64_t split = (best.nt <= 32 ? 224 : 132) / col_tiles;
     if (split > kNwMaxSplit) split = kNwMaxSplit;
-    if (split > num_kb / 4) split = num_kb / 4;
+    if (split > num_kb / 5) split = num_kb / 5;
     best.split = split < 1 ? 1 : (int)split;
     best.cost = 0.0;                           // never slower than a 256-row tile: the same weights, less of everything else
     return best;
