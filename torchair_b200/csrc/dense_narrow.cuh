@@ -25,7 +25,7 @@ namespace tab {
 
 constexpr int kNwMaxTokens = 256;
 constexpr int kNwMaxStages = 12;
-constexpr int kNwCtrlBytes = 256;
+constexpr int kNwCtrlBytes = 512;                        // barriers, control words, from 256 on the bias of kEpiLinearAny
 constexpr int kNwMaxSplit = 8;
 
 // Up to 64 rows two CTAs may share an SM, each with a ring of about 110 KB: the one streams weights while the other is in its
@@ -175,7 +175,8 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   }
 
   // What this thread will need in the epilogue: its columns are the same in every step (a step is an even number of groups), so the
-  // bias is fetched once, and the residual of the first step with it, while the products run.
+  // bias is fetched once, and the residual of the first step with it, while the products run.  (Element by element the values would
+  // be waited for here, ahead of the products: kEpiLinearAny has one warp put the bias into shared memory.)
   constexpr bool ragged = EPI == kEpiLinearAny;
   static_assert(kThreads / 8 % 2 == 0, "steps of an even number of groups");
   const bool has_bias = p.bias != nullptr, has_res = epi_linear(EPI) && p.residual != nullptr;
@@ -185,17 +186,6 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
   const int g_begin = group_begin(rank), g_end = group_begin(rank + 1), g_first = g_begin + static_cast<int>(threadIdx.x >> 3);
   const int col = ft * (EPI == kEpiGlu ? 64 : 128) + (kGroups == 2 ? (g_first & 1) * 64 : 0) + static_cast<int>(threadIdx.x & 7) * 8;
   const bool col_in = col < p.N;
-  auto fetch8 = [&](const T* line, uint4& out) {           // 8 values from column `col` of a line
-    if constexpr (ragged) {
-      const unsigned short* from = reinterpret_cast<const unsigned short*>(line) + col;
-      uint32_t t[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = col + i < n_out ? __ldcg(from + i) : 0u;
-      out = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
-    } else {
-      out = __ldcg(reinterpret_cast<const uint4*>(line + col));
-    }
-  };
   auto unpack_8 = [](const uint4& x, float (&v)[8]) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -206,11 +196,22 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
     }
   };
   uint4 bias_v = make_uint4(0u, 0u, 0u, 0u), bias_up = bias_v, res_v = bias_v;
-  if (EPI != kEpiGluGrad && has_bias && col_in) {
-    fetch8(bias, bias_v);
-    if (EPI == kEpiGlu) fetch8(bias + p.N, bias_up);
+  T* s_bias = reinterpret_cast<T*>(ctrl + 256);
+  if constexpr (ragged) {
+    if (has_bias && warp == 3) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = ft * 128 + i * 32 + lane;
+        s_bias[i * 32 + lane] = c < n_out ? bias[c] : Elem<T>::from_f32(0.f);
+      }
+    }
+  } else if (col_in) {
+    if (EPI != kEpiGluGrad && has_bias) {
+      bias_v = __ldcg(reinterpret_cast<const uint4*>(bias + col));
+      if (EPI == kEpiGlu) bias_up = __ldcg(reinterpret_cast<const uint4*>(bias + p.N + col));
+    }
+    if (has_res && g_first < g_end) res_v = __ldcg(reinterpret_cast<const uint4*>(res + (row0 + g_first / kGroups) * ld + col));
   }
-  if (has_res && col_in && g_first < g_end) fetch8(res + (row0 + g_first / kGroups) * ld, res_v);
 
   // Two producer warps (the second is one that has nothing to do before the epilogue) take the blocks in turn: one alone needs
   // some 400 cycles for a block's wait and copies, more than the bytes do.
@@ -348,14 +349,18 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       float u[8], r[8];
       if (in) {
         if (has_res) {
-          if (g0 > g_begin) fetch8(res + row * ld, res_v);
-          unpack_8(res_v, r);
+          if constexpr (ragged) {
+            load8_any(res + row * ld, col, n_out, r);
+          } else {
+            if (g0 > g_begin) res_v = __ldcg(reinterpret_cast<const uint4*>(res + row * ld + col));
+            unpack_8(res_v, r);
+          }
         }
         sum_parts8(src, part_floats, split, v);
         if constexpr (EPI == kEpiGlu) sum_parts8(src + 64, part_floats, split, u);
         if (has_bias) {
           float b[8];
-          unpack_8(bias_v, b);
+          if constexpr (ragged) Elem<T>::load8(s_bias + (col - ft * 128), b); else unpack_8(bias_v, b);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] += b[i];
           if constexpr (EPI == kEpiGlu) {
@@ -385,12 +390,24 @@ dense_narrow_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_const
       }
     }
   }
-  if (ragged) {
+  if constexpr (ragged) {
+    // A warp to a group of 64 values, two values to a lane where they lie on a 4-byte boundary of the result.  These stores end in sectors
+    // that are written in part: 777 x 1003 -> 1501 takes 13.7 us with them, 9.5 without, 9.4 with whole rows of 1504.
     __syncthreads();
-    for (int e = threadIdx.x; e < (g_end - g_begin) * 64; e += kThreads) {
-      const int g = g_begin + (e >> 6), c = e & 63;
-      const int col = ft * 128 + (g % kGroups) * 64 + c;
-      if (col < n_out) out[(row0 + g / kGroups) * ld + col] = reinterpret_cast<const T*>(sums + (e & ~63) + (c & ~7))[c & 7];
+#pragma unroll 4
+    for (int g = g_begin + warp; g < g_end; g += kThreads / 32) {
+      const unsigned short* from = reinterpret_cast<const unsigned short*>(sums + (g - g_begin) * kGroupFloats);     // value c at (c / 8) * 16 + c % 8
+      const int col0 = ft * 128 + (g & 1) * 64;
+      unsigned short* to = reinterpret_cast<unsigned short*>(out) + (row0 + (g >> 1)) * ld + col0;
+      const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(to) >> 1) & 1u), n = n_out - col0;
+      auto value = [&](int c) { return static_cast<uint32_t>(from[(c & ~7) * 2 + (c & 7)]); };
+      const int c = 2 * lane + odd;
+      if (c + 1 < n && c + 1 < 64) {
+        *reinterpret_cast<uint32_t*>(to + c) = value(c) | value(c + 1) << 16;
+      } else if (c < n && c < 64) {
+        to[c] = static_cast<unsigned short>(value(c));
+      }
+      if (odd && lane == 0 && n > 0) to[0] = static_cast<unsigned short>(value(0));
     }
   }
   if (split > 1) {
