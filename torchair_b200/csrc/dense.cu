@@ -206,19 +206,22 @@ static NarrowPlan narrow_plan(int64_t M, int64_t N, int num_kb, int epi, bool x_
     best.cost = 0.0;                           // never slower than a 256-row tile: the same weights, less of everything else
     return best;
   }
-  // Estimates in SM cycles, from stamps inside the kernel: 58 bytes of operands a cycle reach an SM, a block takes at least 400; 3500 cycles until the first
-  // block and after the last, 30 per row of the tile for the epilogue; the exchange of parts 1500 and 64 per row.
+  // Estimates in SM cycles: 58 bytes of operands a cycle reach an SM, a block takes at least 400; 3500 cycles until the first block and
+  // after the last, 30 per row that a tile has for the epilogue; the exchange of parts 1500 and 32 per row.  At 19 shapes from 100 x 4096
+  // -> 4096 to 2048 x 3008 -> 2816 the combination chosen so took at most 9 % longer than the fastest of all (400 x 4096 -> 2048: 17.3 us
+  // with two CTAs to 128 rows, 19.3 with one to 64, 18.3 on CTA pairs).
   for (int nt = x_mn ? 64 : 32; nt <= kNwMaxTokens; nt *= 2) {
     const int64_t row_tiles = (M + nt - 1) / nt, tiles = row_tiles * col_tiles;
     if (tiles > 8 * 148) continue;
+    const double rows = static_cast<double>(std::min<int64_t>(nt, M));
     const int per_sm = nt <= 64 ? 2 : 1;
     for (int split = 1; split <= kNwMaxSplit; ++split) {
       if (split > 1 && (nt > 128 || split * 4 > num_kb || tiles * split > kClusterRoom[split])) continue;
       const int64_t ctas = tiles * split, room = static_cast<int64_t>(kClusterRoom[split]) * per_sm;
       const double turns = static_cast<double>((ctas + room - 1) / room);
       const double together = ctas > kClusterRoom[split] ? per_sm : 1;
-      const double cost = turns * ((num_kb + split - 1) / split * std::max(400.0, together * dense_narrow_stage_bytes(nt) / 58.0) + 3500.0 + 30.0 * nt * together +
-                                   (split > 1 ? 1500.0 + 64.0 * nt : 0.0));
+      const double cost = turns * ((num_kb + split - 1) / split * std::max(400.0, together * dense_narrow_stage_bytes(nt) / 58.0) + 3500.0 + 30.0 * rows * together +
+                                   (split > 1 ? 1500.0 + 32.0 * rows : 0.0));
       if (best.nt == 0 || cost < best.cost) best = NarrowPlan{nt, split, (int)row_tiles, (int)col_tiles, cost};
     }
   }
