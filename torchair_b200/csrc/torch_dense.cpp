@@ -78,14 +78,20 @@ struct Call {
 
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 
-// dst = src inside src's shape, zero elsewhere (2-D, 16-bit, any strides); done by the next flush
-void copy_2d(const Call& c, const Tensor& src, const Tensor& dst) {
+// Columns [dst_col, dst_col + dst_cols) of dst = columns [src_col, src_col + src_cols) of src inside its shape, zero elsewhere (2-D, 16-bit,
+// any strides); done by the next flush.
+void copy_cols(const Call& c, const Tensor& src, int64_t src_col, int64_t src_cols, const Tensor& dst, int64_t dst_col, int64_t dst_cols) {
   if (c.pending == static_cast<int>(c.copies.size())) c.flush();
-  c.copies[c.pending++] = tab_copy{src.data_ptr(), src.stride(0), src.stride(1), src.size(0), src.size(1),
-                                   dst.data_ptr(), dst.stride(0), dst.stride(1), dst.size(0), dst.size(1)};
+  const int64_t ss = src.stride(1), ds = dst.stride(1);
+  c.copies[c.pending++] = tab_copy{static_cast<const char*>(src.data_ptr()) + 2 * src_col * ss, src.stride(0), ss, src.size(0), src_cols,
+                                   static_cast<char*>(dst.data_ptr()) + 2 * dst_col * ds, dst.stride(0), ds, dst.size(0), dst_cols};
   c.held.push_back(src);
   c.held.push_back(dst);
 }
+void copy_2d(const Call& c, const Tensor& src, const Tensor& dst) { copy_cols(c, src, 0, src.size(1), dst, 0, dst.size(1)); }
+
+// t as [m, n]
+Tensor as_rows(const Tensor& t, int64_t m, int64_t n) { return t.dim() == 2 && t.size(0) == m && t.size(1) == n ? t : t.reshape({m, n}); }
 
 // A matrix in memory that the tensor maps take: contiguous along its columns (row-major) or along its rows, the other stride
 // a multiple of 8 elements.
@@ -143,8 +149,8 @@ Mat halves_of(const Call& c, const Tensor& t, int64_t half) {
   const bool cm = col_major(t);
   const int64_t pitch = cm ? up(rows, 8) : 2 * half;
   Tensor out = cm ? c.empty({2 * half, pitch}).t() : c.empty({rows, pitch});
-  copy_2d(c, t.narrow(1, 0, inner), out.narrow(1, 0, half));
-  copy_2d(c, t.narrow(1, inner, inner), out.narrow(1, half, half));
+  copy_cols(c, t, 0, inner, out, 0, half);
+  copy_cols(c, t, inner, inner, out, half, half);
   return {out, pitch, !cm};
 }
 
@@ -185,7 +191,7 @@ Tensor halves_vector(const Call& c, const OptTensor& t, int64_t half) {
 Tensor cut_row(const Call& c, const Tensor& t, int64_t n) {
   if (t.size(1) == n) return t.view({n});
   Tensor out = c.empty({1, n});
-  copy_2d(c, t.narrow(1, 0, n), out);
+  copy_cols(c, t, 0, n, out, 0, n);
   return out.view({n});
 }
 // [rows, 2 I8] -> [rows, 2 I], in the same order
@@ -193,8 +199,8 @@ Tensor cut_halves(const Call& c, const Tensor& t, int64_t inner) {
   const int64_t rows = t.size(0), half = t.size(1) / 2;
   if (half == inner) return t;
   Tensor out = col_major(t) ? c.empty({2 * inner, rows}).t() : c.empty({rows, 2 * inner});
-  copy_2d(c, t.narrow(1, 0, inner), out.narrow(1, 0, inner));
-  copy_2d(c, t.narrow(1, half, inner), out.narrow(1, inner, inner));
+  copy_cols(c, t, 0, inner, out, 0, inner);
+  copy_cols(c, t, half, inner, out, inner, inner);
   return out;
 }
 
@@ -326,10 +332,10 @@ Tensor ffn_forward(const Call& c, const FfnSizes& s, const Tensor& x, const Tens
   const int64_t inner8 = up(s.inner, 8);
   Tensor y = c.empty(x.sizes());
   if (s.m > 0) {
-    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.h}), up(s.h, 8));
+    const Mat xm = rows_of(c, as_rows(x, s.m, s.h), up(s.h, 8));
     const Mat w1 = halves_of(c, weight1, inner8), w2 = matrix_of(c, weight2);
     const Tensor b1 = halves_vector(c, bias1, inner8), b2 = vector_of(c, bias2);
-    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.h})) : Tensor();
+    const Tensor r = residual.has_value() ? dense_rows(c, as_rows(*residual, s.m, s.h)) : Tensor();
     size_t bytes = 0;
     ok(tab_gated_ffn_workspace_bytes(s.m, s.h, inner8, &bytes), "tab_gated_ffn_workspace_bytes");
     const Tensor ws = c.workspace(bytes);
@@ -355,7 +361,7 @@ Five ffn_keep_cuda(const Tensor& x, const Tensor& weight1, const Tensor& weight2
   const Call c(x, s.dtype);
   Kept kept;
   if (int8) {
-    keep_x(c, x.reshape({s.m, s.h}), kept);
+    keep_x(c, as_rows(x, s.m, s.h), kept);
     const int64_t width = 2 * up(s.inner, kBlock);
     kept.values = c.empty({s.m, width}, at::kChar);
     kept.scale = c.empty({s.m, width / kBlock}, at::kFloat);
@@ -402,10 +408,10 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
     return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
   }
   // column sums read whole pieces of 8: a gradient whose rows are not is copied for them with zeros behind h
-  const Mat dy = want[4] && h8 != h ? padded_rows(c, grad_.reshape({m, h}), h8) : rows_of(c, grad_.reshape({m, h}), h8);
+  const Mat dy = want[4] && h8 != h ? padded_rows(c, as_rows(grad_, m, h), h8) : rows_of(c, as_rows(grad_, m, h), h8);
   Mat w1, xm;
   if (want[0]) w1 = halves_of(c, weight1, inner8);
-  if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, h}), h8);
+  if (want[1] && !x8) xm = rows_of(c, as_rows(x_, m, h), h8);
   Kept kept;
   kept.values = kept_values;
   kept.scale = kept_scale;
@@ -423,13 +429,12 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
     if (want[0] && inner != inner8) {      // the product for dx runs over the columns behind I too: infinities leave NaN there
-      const Tensor nothing = dz.t.narrow(1, 0, 0);
-      copy_2d(c, nothing, dz.t.narrow(1, inner, inner8 - inner));
-      copy_2d(c, nothing, dz.t.narrow(1, inner8 + inner, inner8 - inner));
+      copy_cols(c, dz.t, 0, 0, dz.t, inner, inner8 - inner);
+      copy_cols(c, dz.t, 0, 0, dz.t, inner8 + inner, inner8 - inner);
       c.flush();
     }
   }
-  if (want[1] && x8) xm = dequantise(c, x_.view({m, h}), x_scale.view({m, -1}), any);
+  if (want[1] && x8) xm = dequantise(c, as_rows(x_, m, h), as_rows(x_scale, m, up(h, kBlock) / kBlock), any);
   // What is left depends on nothing but what is ordered before it: each launch may start in the SMs that the last turn of the one before
   // leaves idle.
   bool beside = false;
@@ -460,7 +465,7 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
        "tab_two_column_sums");
   }
   if (want[1]) dw1 = cut_halves(c, dw1, inner);
-  if (want[3]) db1 = cut_halves(c, db1, inner).reshape({2 * inner});
+  if (want[3]) db1 = cut_halves(c, db1, inner).view({2 * inner});
   if (want[4]) db2 = cut_row(c, db2, h);
   c.flush();
   return Five(result(dx), result(dw1), result(dw2), result(db1), result(db2));
@@ -497,10 +502,10 @@ Tensor linear_forward(const Call& c, const LinearSizes& s, at::IntArrayRef out_s
                       const OptTensor& residual, const Kept& kept) {
   Tensor y = c.empty(out_sizes);
   if (s.m > 0) {
-    const Mat xm = rows_of(c, x.dim() == 2 ? x : x.reshape({s.m, s.k}), up(s.k, 8));
+    const Mat xm = rows_of(c, as_rows(x, s.m, s.k), up(s.k, 8));
     const Mat w = matrix_of(c, weight);
     const Tensor b = vector_of(c, bias);
-    const Tensor r = residual.has_value() ? dense_rows(c, residual->dim() == 2 ? *residual : residual->reshape({s.m, s.n})) : Tensor();
+    const Tensor r = residual.has_value() ? dense_rows(c, as_rows(*residual, s.m, s.n)) : Tensor();
     matmul(c, xm.ptr(), xm.ld, 0, w.ptr(), w.ld, w.mn_by_cols(), s.m, s.n, s.k, y, b, r, s.act, kept);
   }
   return y;
@@ -519,7 +524,7 @@ Five linear_keep_cuda(const Tensor& x, const Tensor& weight, const OptTensor& bi
   const c10::cuda::CUDAGuard guard(x.device());
   const Call c(x, s.dtype);
   Kept kept;
-  if (int8) keep_x(c, x.reshape({s.m, s.k}), kept);
+  if (int8) keep_x(c, as_rows(x, s.m, s.k), kept);
   // without an activation the backward pass does not need its argument
   const int64_t width = s.act ? up(s.n, int8 ? kBlock : 8) : 0;
   Kept stored;
@@ -569,11 +574,11 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
     }
     Mat w, xm;
     if (want[0]) w = matrix_of(c, weight);
-    if (want[1] && !x8) xm = rows_of(c, x_.reshape({m, k}), up(k, 8));
+    if (want[1] && !x8) xm = rows_of(c, as_rows(x_, m, k), up(k, 8));
     // the elementwise kernel reads whole pieces of 8
-    const Mat dy = n8 != n && (act || want[2]) ? padded_rows(c, grad_.reshape({m, n}), n8) : rows_of(c, grad_.reshape({m, n}), n8);
+    const Mat dy = n8 != n && (act || want[2]) ? padded_rows(c, as_rows(grad_, m, n), n8) : rows_of(c, as_rows(grad_, m, n), n8);
     const Mat dz = act_grad(c, dy, n8, act, kept, want[0] || want[1], want[2], db);
-    if (want[1] && x8) xm = dequantise(c, x_.view({m, k}), x_scale.view({m, -1}));
+    if (want[1] && x8) xm = dequantise(c, as_rows(x_, m, k), as_rows(x_scale, m, up(k, kBlock) / kBlock));
     if (want[0]) {
       dx = c.empty(x_sizes);
       matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k, n, dx);
@@ -646,7 +651,7 @@ Tensor ck_weight_grad_cuda(const Tensor& q_, const Tensor& scale_, const Tensor&
   const Call c(grad_, dtype);
   if (m == 0) return at::zeros({k, n}, c.opt);
   const Tensor q = q_.contiguous().view({m, k}), scale = scale_.contiguous().view({m, -1});
-  const Mat x = dequantise(c, q, scale), dz = rows_of(c, grad_.reshape({m, n}), up(n, 8));
+  const Mat x = dequantise(c, q, scale), dz = rows_of(c, as_rows(grad_, m, n), up(n, 8));
   Tensor out = c.empty({k, n});
   matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out);
   return out;
