@@ -733,6 +733,49 @@ def test_first_cuda_call_of_a_thread(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [300, 2000])
+def test_two_threads_on_one_stream(dev, m):
+    """One host thread runs backward passes, another forward passes on the same stream: memory that either frees goes to the other while
+    launches of both are in flight, and every result has the bits of the same calls alone."""
+    import threading
+    g = gen(m + 18)
+    h = inner = 512                      # hidden rows, gradients and results of one size: they fit each other's memory
+    x, dy, nx = make(g, m, h), make(g, m, h), make(g, m, h)
+    w1, w2 = weight(g, h, 2 * inner, False, x.dtype), weight(g, inner, h, False, x.dtype)
+    _, kept, ks, xq, xs = npu.npu_gated_ffn_keep(x, w1, w2, checkpoint_int8=True)
+    _, lkept, lks, _, lxs = npu.npu_linear_act_keep(x, w1, activation="gelu")
+    dyl = make(g, m, 2 * inner)
+
+    def train():
+        return npu.npu_gated_ffn_backward(dy, xq, xs, w1, w2, kept, ks, "silu", [True] * 5) + \
+            npu.npu_linear_act_backward(dyl, x, lxs, w1, lkept, lks, "gelu", [True, True, False])[:2]
+
+    def infer():
+        return npu.npu_gated_ffn(nx, w1, w2), npu.npu_linear_act(nx, w1, activation="silu")
+
+    want = train(), infer()
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(2), []
+
+    def loop(call, want):
+        try:
+            start.wait()
+            for _ in range(40):
+                outs = [call() for _ in range(5)]
+                if not all(torch.equal(a, b) for out in outs for a, b in zip(out, want)):
+                    failed.append(call.__name__)
+        except BaseException as e:       # seen by the test, not only by the thread
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=loop, args=a) for a in ((train, want[0]), (infer, want[1]))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+@pytest.mark.gpu
 def test_training_step_in_a_graph(dev):
     ins = _step_inputs(300)
     want = [t.clone() for t in _train_step(*ins, True)]

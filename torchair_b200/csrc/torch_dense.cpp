@@ -71,9 +71,19 @@ struct Call {
     held.clear();
   }
   explicit Call(const Tensor& x, int dtype_) : dtype(dtype_), stream(c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), opt(x.options().requires_grad(false)) {}
-  Tensor empty(at::IntArrayRef sizes) const { return at::empty(sizes, opt); }
-  Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const { return at::empty(sizes, opt.dtype(t)); }
-  Tensor workspace(size_t bytes) const { return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, opt.dtype(at::kByte)); }
+  // Set while launches run beside one another.  Memory that another host thread freed meanwhile may still be in use by a launch of its own
+  // between two of these, and a launch that runs beside that one does not wait for it: what a group of such launches writes is allocated
+  // before the ordinary launch that opens the group, which waits for everything that was launched before the memory was handed out.
+  mutable bool group_open = false;
+  Tensor empty(at::IntArrayRef sizes) const { return empty(sizes, opt); }
+  Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const { return empty(sizes, opt.dtype(t)); }
+  Tensor workspace(size_t bytes) const { return empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, opt.dtype(at::kByte)); }
+
+ private:
+  Tensor empty(at::IntArrayRef sizes, const at::TensorOptions& o) const {
+    TORCH_INTERNAL_ASSERT(!group_open, "memory allocated between launches that run beside one another");
+    return at::empty(sizes, o);
+  }
 };
 
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
@@ -226,20 +236,21 @@ void matmul(const Call& c, const void* a, int64_t lda, int a_mn, const void* b, 
      "tab_dense_matmul");
 }
 
-// x^T dz [k, n] (both row-major), in the memory order of the weight `like`
-Tensor weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_t n, const Tensor& like, bool beside) {
-  const int64_t m = x.t.size(0);
-  if (col_major(like)) {
-    Tensor out = c.empty({n, k});
-    matmul(c, dz.ptr(), dz.ld, 1, x.ptr(), x.ld, 1, n, k, m, out, Tensor(), Tensor(), 0, Kept(), beside);
-    return out.t();
-  }
-  Tensor out = c.empty({k, n});
-  matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out, Tensor(), Tensor(), 0, Kept(), beside);
-  return out;
+// memory for the gradient [k, n] of a weight, in the memory order of the weight `like`
+Tensor weight_grad_memory(const Call& c, int64_t k, int64_t n, const Tensor& like) {
+  return col_major(like) ? c.empty({n, k}).t() : c.empty({k, n});
 }
 
-// the same without rows to sum over
+// x^T dz (both row-major) into out [k, n], which weight_grad_memory gave for `like`
+void weight_grad(const Call& c, const Mat& x, const Mat& dz, int64_t k, int64_t n, const Tensor& like, const Tensor& out, bool beside) {
+  const int64_t m = x.t.size(0);
+  if (col_major(like))
+    matmul(c, dz.ptr(), dz.ld, 1, x.ptr(), x.ld, 1, n, k, m, out, Tensor(), Tensor(), 0, Kept(), beside);
+  else
+    matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out, Tensor(), Tensor(), 0, Kept(), beside);
+}
+
+// a weight gradient without rows to sum over
 Tensor zero_grad(const Call& c, const Tensor& like) {
   return col_major(like) ? at::zeros({like.size(1), like.size(0)}, c.opt).t() : at::zeros({like.size(0), like.size(1)}, c.opt);
 }
@@ -282,14 +293,17 @@ void keep_x(const Call& c, const Tensor& x, Kept& kept) {
   quantise(c.stream, xr, x.size(0), x.size(1), xr.stride(0), kept.x_q, kept.x_scale);
 }
 
-// int8 [m, k] with its scales (no gaps) -> 16 bits, rows of a multiple of 8 values, zero behind k
-Mat dequantise(const Call& c, const Tensor& q, const Tensor& scale, bool beside = false) {
+// memory for int8 [m, k] in 16 bits: rows of a multiple of 8 values
+Mat dequantised_memory(const Call& c, const Tensor& q) {
   const int64_t pitch = up(q.size(1), 8);
-  Tensor y = c.empty({q.size(0), pitch});
+  return {c.empty({q.size(0), pitch}), pitch, true};
+}
+
+// int8 [m, k] with its scales (no gaps) -> 16 bits, zero behind k
+void dequantise(const Call& c, const Tensor& q, const Tensor& scale, const Mat& y, bool beside = false) {
   ok(tab_checkpoint_dequant(static_cast<const int8_t*>(q.data_ptr()), q.size(1), static_cast<const float*>(scale.data_ptr()), scale.size(1), q.size(0),
-                            q.size(1), y.data_ptr(), c.dtype, pitch, pitch, beside, c.stream),
+                            q.size(1), y.t.data_ptr(), c.dtype, y.ld, y.ld, beside, c.stream),
      "tab_checkpoint_dequant");
-  return {y, pitch, true};
 }
 
 using Five = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
@@ -417,14 +431,37 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
   kept.scale = kept_scale;
   Mat dz{Tensor(), 2 * inner8, true}, hidden{Tensor(), inner8, true};
   const bool any = want[0] || want[1] || want[2] || want[3];
-  // Launches that run beside one another: everything that one of them touches stays allocated until all of them are launched, for memory
-  // that is freed may be handed out again at once.
+  // Launches that run beside one another: everything that they touch is allocated before the first of them and stays so until all of them
+  // are launched (see Call::group_open).
   Mat w2;
   if (any) {
     w2 = matrix_of(c, inner == inner8 ? weight2 : padded_weight2(c, weight2, inner8));
     dz.t = c.empty({m, 2 * inner8});
     hidden.t = c.empty({m, inner8});
-    c.flush();
+  }
+  Tensor x_q, x_s;
+  if (want[1] && x8) {
+    x_q = as_rows(x_, m, h);
+    x_s = as_rows(x_scale, m, up(h, kBlock) / kBlock);
+    xm = dequantised_memory(c, x_q);
+  }
+  if (want[0]) dx = c.empty(grad_.sizes());
+  if (want[1]) dw1 = weight_grad_memory(c, h, 2 * inner8, weight1);
+  if (want[2]) dw2 = weight_grad_memory(c, inner, h, weight2);
+  if (want[3]) db1 = c.empty({1, 2 * inner8});
+  if (want[4]) db2 = c.empty({1, h8});
+  // both sums in slices that do not depend on which of them are wanted, and so neither do their values
+  const Mat &first = want[3] ? dz : dy, &second = want[3] && want[4] ? dy : Mat();
+  const int64_t n1 = want[3] ? 2 * inner8 : h8, n2 = want[3] && want[4] ? h8 : 0;
+  Tensor parts;
+  if (want[3] || want[4]) {
+    size_t splits = 0;
+    ok(tab_act_grad_splits(m, 2 * inner8 + h8, &splits), "tab_act_grad_splits");
+    parts = c.empty({static_cast<int64_t>(splits), n1 + n2}, at::kFloat);
+  }
+  c.flush();
+  c.group_open = true;
+  if (any) {
     ok(tab_gated_matmul_grad(dy.ptr(), dy.ld, w2.ptr(), w2.ld, w2.mn_by_rows(), dtype, m, inner8, h, act, kept.p16(), kept.p8(), kept.ps(), kept.ld(),
                              dz.t.data_ptr(), hidden.t.data_ptr(), c.stream),
        "tab_gated_matmul_grad");
@@ -434,36 +471,27 @@ Five ffn_backward_cuda(const Tensor& grad_, const Tensor& x_, const Tensor& x_sc
       c.flush();
     }
   }
-  if (want[1] && x8) xm = dequantise(c, as_rows(x_, m, h), as_rows(x_scale, m, up(h, kBlock) / kBlock), any);
+  if (want[1] && x8) dequantise(c, x_q, x_s, xm, any);
   // What is left depends on nothing but what is ordered before it: each launch may start in the SMs that the last turn of the one before
   // leaves idle.
   bool beside = false;
   if (want[2]) {
-    dw2 = weight_grad(c, hidden, dy, inner, h, weight2, beside);
+    weight_grad(c, hidden, dy, inner, h, weight2, dw2, beside);
     beside = true;
   }
   if (want[0]) {
-    dx = c.empty(grad_.sizes());
     matmul(c, dz.ptr(), dz.ld, 0, w1.ptr(), w1.ld, w1.mn_by_rows(), m, h, 2 * inner8, dx, Tensor(), Tensor(), 0, Kept(), beside);
     beside = true;
   }
   if (want[1]) {
-    dw1 = weight_grad(c, xm, dz, h, 2 * inner8, weight1, beside);
+    weight_grad(c, xm, dz, h, 2 * inner8, weight1, dw1, beside);
     beside = true;
   }
-  if (want[3] || want[4]) {                // in slices that do not depend on which of them are wanted, and so neither do their sums
-    const Mat &first = want[3] ? dz : dy, &second = want[3] && want[4] ? dy : Mat();
-    const int64_t n1 = want[3] ? 2 * inner8 : h8, n2 = want[3] && want[4] ? h8 : 0;
-    size_t splits = 0;
-    ok(tab_act_grad_splits(m, 2 * inner8 + h8, &splits), "tab_act_grad_splits");
-    const Tensor parts = c.empty({static_cast<int64_t>(splits), n1 + n2}, at::kFloat);
-    if (want[3]) db1 = c.empty({1, 2 * inner8});
-    if (want[4]) db2 = c.empty({1, h8});
-    c.flush();
+  if (parts.defined())
     ok(tab_two_column_sums(first.ptr(), first.ld, n1, n2 ? second.ptr() : nullptr, second.ld, n2, dtype, m, static_cast<float*>(parts.data_ptr()),
-                           static_cast<int64_t>(splits), want[3] ? db1.data_ptr() : db2.data_ptr(), n2 ? db2.data_ptr() : nullptr, beside, c.stream),
+                           parts.size(0), want[3] ? db1.data_ptr() : db2.data_ptr(), n2 ? db2.data_ptr() : nullptr, beside, c.stream),
        "tab_two_column_sums");
-  }
+  c.group_open = false;
   if (want[1]) dw1 = cut_halves(c, dw1, inner);
   if (want[3]) db1 = cut_halves(c, db1, inner).view({2 * inner});
   if (want[4]) db2 = cut_row(c, db2, h);
@@ -578,12 +606,18 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_cuda(const Tensor& grad_, con
     // the elementwise kernel reads whole pieces of 8
     const Mat dy = n8 != n && (act || want[2]) ? padded_rows(c, as_rows(grad_, m, n), n8) : rows_of(c, as_rows(grad_, m, n), n8);
     const Mat dz = act_grad(c, dy, n8, act, kept, want[0] || want[1], want[2], db);
-    if (want[1] && x8) xm = dequantise(c, as_rows(x_, m, k), as_rows(x_scale, m, up(k, kBlock) / kBlock));
-    if (want[0]) {
-      dx = c.empty(x_sizes);
-      matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k, n, dx);
+    if (want[1] && x8) {
+      const Tensor q = as_rows(x_, m, k);
+      xm = dequantised_memory(c, q);
+      dequantise(c, q, as_rows(x_scale, m, up(k, kBlock) / kBlock), xm);
     }
-    if (want[1]) dw = weight_grad(c, xm, dz, k, n, weight, want[0]);       // beside the one before: see npu_gated_ffn_backward
+    if (want[0]) dx = c.empty(x_sizes);
+    if (want[1]) dw = weight_grad_memory(c, k, n, weight);
+    c.flush();
+    c.group_open = true;
+    if (want[0]) matmul(c, dz.ptr(), dz.ld, 0, w.ptr(), w.ld, w.mn_by_rows(), m, k, n, dx);
+    if (want[1]) weight_grad(c, xm, dz, k, n, weight, dw, want[0]);        // beside the one before: see npu_gated_ffn_backward
+    c.group_open = false;
     if (want[2]) db = cut_row(c, db, n);
     c.flush();
   }
@@ -651,7 +685,8 @@ Tensor ck_weight_grad_cuda(const Tensor& q_, const Tensor& scale_, const Tensor&
   const Call c(grad_, dtype);
   if (m == 0) return at::zeros({k, n}, c.opt);
   const Tensor q = q_.contiguous().view({m, k}), scale = scale_.contiguous().view({m, -1});
-  const Mat x = dequantise(c, q, scale), dz = rows_of(c, as_rows(grad_, m, n), up(n, 8));
+  const Mat x = dequantised_memory(c, q), dz = rows_of(c, as_rows(grad_, m, n), up(n, 8));
+  dequantise(c, q, scale, x);
   Tensor out = c.empty({k, n});
   matmul(c, x.ptr(), x.ld, 1, dz.ptr(), dz.ld, 1, k, n, m, out);
   return out;
