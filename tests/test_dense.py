@@ -1050,3 +1050,32 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call(built_library):
     with pytest.raises(RuntimeError, match="workspace"):
         _lib.call("tab_gated_ffn", one, 64, one, 128, 1, one, 64, 1, 64, 15, 4, 64, 64, n, n, n, 4, n, n, n, 0, one, one, 16, n)
     assert _lib.workspace_bytes("tab_gated_ffn_workspace_bytes", 4, 64, 64) >= 4 * 64 * 2
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+def test_forward_mode_raises(which):
+    """A tangent is refused, whether or not something requires a gradient; it used to be dropped where nothing did."""
+    import torch.autograd.forward_ad as fw
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    fake = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    with FakeTensorMode(), fw.dual_level():
+        t = {"x": fake(4, 64), "weight": fake(64, 64), "bias": fake(64), "residual": fake(4, 64)}
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        for grad in (False, True):
+            v = fake(32, 64).requires_grad_(grad)
+            with pytest.raises(NotImplementedError, match="npu_linear_act: forward-mode"):
+                npu.npu_linear_act(t["x"], t["weight"].requires_grad_(grad) if which == "bias" else t["weight"], bias=t["bias"], residual=t["residual"])
+            with pytest.raises(NotImplementedError, match="npu_gated_ffn: forward-mode"):
+                npu.npu_gated_ffn(t["x"], t["weight"], v, bias1=t["bias"], residual=t["residual"])
+        for call in (lambda: npu.npu_checkpoint_quant(t["x"]), lambda: npu.npu_linear_act_keep(t["x"], t["weight"], bias=t["bias"], residual=t["residual"])):
+            if which == "x":
+                with pytest.raises(NotImplementedError, match="forward AD"):
+                    call()
+
+
+def test_jvp_raises():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = torch.empty(4, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(64, 32, dtype=torch.bfloat16, device="cuda")
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda v: npu.npu_linear_act(v, w), (x,), (torch.ones_like(x),))

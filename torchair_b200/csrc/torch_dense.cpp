@@ -7,6 +7,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -704,6 +705,18 @@ c10::TypedOperatorHandle<Sig> handle(const char* name) {
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
+// There is no forward-mode formula: a tangent raises instead of being dropped.
+void no_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), op, ": forward-mode differentiation is not implemented");
+}
+void no_tangent(const char* op, const OptTensor& t) {
+  if (t.has_value()) no_tangent(op, *t);
+}
+template <typename... Inputs>
+void no_tangents(const char* op, const Inputs&... inputs) {
+  (no_tangent(op, inputs), ...);
+}
+
 // Results of a backward pass that cannot be differentiated again: doing so raises, but only when it is done.
 void once_only(const char* name, const variable_list& inputs, variable_list& out) {
   if (!at::GradMode::is_enabled()) return;
@@ -767,6 +780,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 
 Tensor ffn_autograd(const Tensor& x, const Tensor& w1, const Tensor& w2, const OptTensor& b1, const OptTensor& b2, const OptTensor& r,
                     c10::string_view act, bool int8) {
+  no_tangents("npu_gated_ffn", x, w1, w2, b1, b2, r);
   if (at::GradMode::is_enabled() && (wants(x) || wants(w1) || wants(w2) || wants(b1) || wants(b2) || wants(r)))
     return GatedFfn::apply(x, w1, w2, b1, b2, r, std::string(act), int8);
   static const auto op = handle<FfnSig>("npu::npu_gated_ffn");
@@ -814,6 +828,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 };
 
 Tensor linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, c10::string_view act, bool int8) {
+  no_tangents("npu_linear_act", x, w, b, r);
   if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearAct::apply(x, w, b, r, std::string(act), int8);
   static const auto op = handle<LinearSig>("npu::npu_linear_act");
   at::AutoDispatchBelowADInplaceOrView below;
@@ -837,4 +852,8 @@ TORCH_LIBRARY_IMPL(npu, CUDA, m) {
 TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
   m.impl("npu_gated_ffn", TORCH_FN(ffn_autograd));
   m.impl("npu_linear_act", TORCH_FN(linear_autograd));
+  // not differentiable: a gradient or a tangent that is asked for raises
+  for (const char* op : {"npu_gated_ffn_keep", "npu_gated_ffn_backward", "npu_linear_act_keep", "npu_linear_act_backward", "npu_checkpoint_quant",
+                         "npu_checkpoint_dequant", "npu_checkpoint_weight_grad"})
+    m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

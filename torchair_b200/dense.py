@@ -10,7 +10,7 @@ The gate half of weight1 comes first (activate_left of npu_dequant_swiglu_quant)
 fp32, rounded once per result.  The first two are differentiable: the values before the activation are kept for the backward
 pass in the input's type, or, with checkpoint_int8, together with x in 8 bits.  The backward pass then differentiates at the
 kept values.  The *_keep and *_backward forms are what the gradients are made of; they and the checkpoint operators are not
-differentiable themselves.
+differentiable themselves: a gradient through them raises when it is asked for.  Forward-mode differentiation raises everywhere.
 
 As everywhere in this package the CUDA implementations launch on the current stream, the "Meta" ones (here) carry the shape
 rules, there is no CPU implementation, and argument combinations that are not built raise.  The CUDA and autograd sides are C++
