@@ -812,6 +812,41 @@ def test_only_the_wanted_gradients_and_no_second_order(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+@pytest.mark.parametrize("frozen", ["weights", "input", "nothing"])
+def test_a_second_differentiation_raises_and_loses_nothing(dev, frozen, int8):
+    """Gradients made with create_graph depend on what they were made from: a term that differentiates one again raises, whichever
+    inputs require gradients, instead of adding nothing to the other terms' gradients."""
+    g = gen(19)
+    t = {"x": make(g, 20, 64), "weight1": make(g, 64, 64, scale=0.1), "weight2": make(g, 32, 64, scale=0.1), "bias1": make(g, 64), "bias2": make(g, 64),
+         "residual": make(g, 20, 64)}
+    names = {"weights": ["x"], "input": ["bias1", "bias2"], "nothing": list(t)}[frozen]
+    leaves = {k: v.detach().requires_grad_(k in names) for k, v in t.items()}
+    wanted = [leaves[k] for k in names]
+
+    def ffn():
+        return npu.npu_gated_ffn(leaves["x"], leaves["weight1"], leaves["weight2"], bias1=leaves["bias1"], bias2=leaves["bias2"],
+                                 residual=leaves["residual"], checkpoint_int8=int8)
+
+    def linear():
+        return npu.npu_linear_act(leaves["x"], leaves["weight1"], bias=leaves["bias1"], residual=leaves["residual"], activation="silu",
+                                  checkpoint_int8=int8)
+
+    for call in (ffn, linear):
+        some = [p for k, p in zip(names, wanted) if call is ffn or k in ("x", "weight1", "bias1", "residual")]
+        y = call()
+        plain = torch.autograd.grad(y, some, torch.ones_like(y), retain_graph=True)
+        for i, p in enumerate(some):
+            grads = torch.autograd.grad(call().sum(), some, create_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(grads, plain))
+            if p is leaves["residual"]:
+                continue                                     # the incoming gradient itself
+            assert grads[i].requires_grad
+            with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+                ((p * 2).sum() + grads[i].float().pow(2).sum()).backward()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", [(700, 256, 200), (3001, 512, 352), (77, 100, 33), (5, 64, 48)], ids=str)
 @pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
 def test_each_gradient_alone_equals_all_at_once(dev, case, int8):

@@ -717,15 +717,14 @@ void no_tangents(const char* op, const Inputs&... inputs) {
   (no_tangent(op, inputs), ...);
 }
 
-// Results of a backward pass that cannot be differentiated again: doing so raises, but only when it is done.
-void once_only(const char* name, const variable_list& inputs, variable_list& out) {
-  if (!at::GradMode::is_enabled()) return;
-  bool any = false;
-  for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
-  if (!any) return;
+// Results of a backward pass that cannot be differentiated again: doing so raises, but only when it is done.  They depend on the incoming
+// gradient, the weights and (through the kept values) on every input, so all are marked whichever of these require gradients.
+void once_only(const char* name, variable_list& out) {
+  if (!at::GradMode::is_enabled()) return;       // without create_graph nothing is differentiated again
   variable_list some;
   for (const Tensor& t : out)
-    if (t.defined()) some.push_back(t.detach());
+    if (t.defined()) some.push_back(t.detach().set_requires_grad(true));       // (the node's results require gradients where its inputs do)
+  if (some.empty()) return;
   auto node = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " cannot be differentiated twice", static_cast<int64_t>(some.size()));
   variable_list marked = (*node)(std::move(some));
   size_t i = 0;
@@ -772,7 +771,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
       if (want[3]) out[3] = db1;
       if (want[4]) out[4] = db2;
     }
-    once_only("npu_gated_ffn", {grads[0], s[0], s[2], s[3]}, out);
+    once_only("npu_gated_ffn", out);
     if (want_r) out[5] = grads[0];
     return out;
   }
@@ -821,7 +820,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
       if (want[1]) out[1] = dw;
       if (want[2]) out[2] = db;
     }
-    once_only("npu_linear_act", {grads[0], s[0], s[2]}, out);
+    once_only("npu_linear_act", out);
     if (want_r) out[3] = grads[0];
     return out;
   }
