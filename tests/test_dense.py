@@ -948,6 +948,47 @@ def test_compiled_by_the_backend(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["max-autotune", "reduce-overhead"])
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+def test_training_compiled_by_the_backend(dev, mode, int8):
+    """What one forward pass keeps survives the next one, gradients survive the next backward pass, and weights that an optimiser changed
+    are seen: eager bits throughout."""
+    from torchair_b200 import backend
+
+    class Block(torch.nn.Module):
+        def __init__(self, *weights):
+            super().__init__()
+            self.w1, self.w2, self.w = (torch.nn.Parameter(t.detach().clone()) for t in weights)
+
+        def forward(self, x):
+            h = npu.npu_gated_ffn(x, self.w1, self.w2, residual=x, checkpoint_int8=int8)
+            return npu.npu_linear_act(h, self.w, activation="gelu", checkpoint_int8=int8)
+
+    ins = _step_inputs(50)
+    eager, model = Block(*ins[1:4]), Block(*ins[1:4])
+    config = torchair_b200.CompilerConfig()
+    config.mode = mode
+    compiled = torch.compile(model, backend=torchair_b200.get_npu_backend(compiler_config=config), dynamic=False)
+    xs = [make(gen(80 + i), *ins[0].shape) for i in range(2)]
+    before = backend.counters["captures"]
+    for step in range(4):
+        results = []
+        for f, module in ((eager, eager), (compiled, model)):
+            leaves = [x.clone().requires_grad_() for x in xs]
+            params = list(module.parameters())
+            ys = [f(x) for x in leaves]                                                   # both forward passes first
+            results.append([y.detach() for y in ys] + [t for x, y in zip(leaves, ys) for t in torch.autograd.grad(y, [x] + params, ins[4])])
+            with torch.no_grad():
+                for p, d in zip(params, results[-1][-3:]):
+                    p.sub_(d, alpha=2.0 ** -14)
+        for i, (want, got) in enumerate(zip(*results)):
+            assert torch.equal(got, want), (step, i)
+    assert backend.counters["captures"] - before <= 4, "an optimiser's steps do not capture anew each time"
+    with torch.no_grad():
+        assert torch.equal(compiled(xs[0]), eager(xs[0]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fused", [True, False])
 def test_moe_layer_with_a_shared_expert(dev, fused):
     """The layer's shared expert is npu_gated_ffn handed to the combine; without one nothing changes."""

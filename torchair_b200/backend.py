@@ -215,11 +215,17 @@ def _is_static_input(t) -> bool:
 
 
 class _CompiledFxGraph:
-    """Callable returned to AOT-autograd: eager FX replay, or CUDA-graph capture/replay keyed by input shapes."""
+    """Callable returned to AOT-autograd: eager FX replay, or CUDA-graph capture/replay keyed by input shapes.
 
-    def __init__(self, gm: torch.fx.GraphModule, config: CompilerConfig):
+    A captured graph hands out the same output buffers at every replay.  `training` (a forward graph whose results are kept for a
+    backward graph, or that backward graph): the outputs are copied out of them, for what one forward pass keeps has to outlive the next
+    one, and a gradient the next backward pass.
+    """
+
+    def __init__(self, gm: torch.fx.GraphModule, config: CompilerConfig, training: bool = False):
         from . import scope
         self.gm = gm
+        self.training = training
         # graphs with stream scopes are replayed node by node on CUDA streams; the others run their generated code
         self.run = scope.StreamedReplay(gm) if scope.uses_scopes(gm) else gm
         self.capture = config.mode.raw in ("reduce-overhead", "npugraph_ex") and not config.debug.run_eagerly.raw \
@@ -244,6 +250,14 @@ class _CompiledFxGraph:
                         for a, st in zip(args, static))
             entry = self.graphs.get(key)
             if entry is None:
+                if self.training and self._weights_changed(key, static):
+                    # an optimiser changes them between any two steps: a capture would serve one step
+                    logger.warning("weights of a differentiable graph were changed in place; running it eagerly")
+                    self.eager_forever = True
+                    torch.cuda.synchronize()       # no replay is in flight when the captures are given back
+                    self.graphs.clear()
+                    counters["eager_runs"] += 1
+                    return self.run(*args)
                 if len(self.graphs) >= self.limit:
                     # same policy as the reference when captures overflow: fall back to eager for good
                     # (python/torchair/_acl_concrete_graph/acl_graph.py:1001-1014)
@@ -257,7 +271,17 @@ class _CompiledFxGraph:
                     dst.copy_(src)
             graph.replay()
             counters["replays"] += 1
-            return static_out
+            if not self.training:
+                return static_out
+            mine = {id(a): b for a, b in zip(static_in, args)}       # an input that is handed on is the caller's own
+            return [mine[id(o)] if id(o) in mine else o.clone() if isinstance(o, torch.Tensor) else o for o in static_out]
+
+    def _weights_changed(self, key, static) -> bool:
+        """Whether a capture has one of these static inputs in an earlier version."""
+        if self.frozen:
+            return False
+        return any(st and old[:-1] == new[:-1] and old[-1] != new[-1]
+                   for known in self.graphs for old, new, st in zip(known, key, static))
 
     def _capture(self, key, args, static):
         static_in = [a if st or not self.clone_input else a.clone() for a, st in zip(args, static)]
@@ -280,7 +304,7 @@ def _npu_backend(gm: torch.fx.GraphModule, example_inputs: List[torch.Tensor], *
     from torch._functorch.aot_autograd import aot_module_simplified
     from . import ops  # noqa: F401  (registers torch.ops.npu.*)
 
-    def fw_compiler(fx_gm: torch.fx.GraphModule, inputs):
+    def compiler(fx_gm: torch.fx.GraphModule, inputs, training: bool):
         pre, post = config.post_grad_custom_pre_pass.raw, config.post_grad_custom_post_pass.raw
         if callable(pre):
             pre(fx_gm.graph)
@@ -294,9 +318,11 @@ def _npu_backend(gm: torch.fx.GraphModule, example_inputs: List[torch.Tensor], *
         ignored = config.ignored_settings()
         if ignored:
             logger.warning("options without effect on B200 were set and are ignored: %s", ignored)
-        return _CompiledFxGraph(fx_gm, config)
+        return _CompiledFxGraph(fx_gm, config, training)
 
-    return aot_module_simplified(gm, example_inputs, fw_compiler=fw_compiler, decompositions=decompositions)
+    differentiable = functools.partial(compiler, training=True)
+    return aot_module_simplified(gm, example_inputs, fw_compiler=differentiable, bw_compiler=differentiable,
+                                 inference_compiler=functools.partial(compiler, training=False), decompositions=decompositions)
 
 
 def get_compiler(compiler_config: Optional[CompilerConfig] = None):
