@@ -1013,6 +1013,36 @@ def test_moe_layer_with_a_shared_expert(dev, fused):
     assert torch.equal(plain.cpu(), O.moe_layer([x.cpu()], [ids.cpu()], [wt.cpu()], w, [])[0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("leaf", ["x", "shared_w1", "shared_w2"])
+def test_a_gradient_through_moe_layer_raises(dev, leaf):
+    """The routed half has no gradients, so a gradient of the shared expert through the layer is refused instead of lost; the forward
+    result with parameters as weights is the same."""
+    from oracle import moe_oracle as O
+    from torchair_b200.layer import moe_layer
+    cfg = O.CONFIGS["cfg0"]
+    w = O.make_weights(cfg, seed=3)
+    x, ids, wt = (t.to(dev) for t in O.make_tokens(cfg, seed=3))
+    g = gen(2)
+    t = {"x": x, "shared_w1": weight(g, x.shape[1], 512, True, x.dtype), "shared_w2": weight(g, 256, x.shape[1], True, x.dtype)}
+
+    modes = []
+
+    def call():
+        return moe_layer(t["x"], ids, wt, w.w1.to(dev), w.s1.to(dev), w.w2.to(dev), w.s2.to(dev), shared_w1=t["shared_w1"], shared_w2=t["shared_w2"],
+                         after_dispatch=lambda: modes.append(torch.is_grad_enabled()))
+
+    want = call()
+    t[leaf] = t[leaf].detach().requires_grad_()
+    got = call()
+    assert torch.equal(got.detach(), want)
+    with pytest.raises(NotImplementedError, match="no backward pass"):
+        (got.float().sum() + t[leaf].float().sum()).backward()
+    with torch.no_grad():
+        assert torch.equal(call(), want)
+    assert modes == [True, True, False], "the caller's own work runs in the caller's mode"
+
+
 # ---- refusals (CPU) ------------------------------------------------------------------------------------------------------
 def _meta(*shape, dtype=torch.bfloat16):
     return torch.empty(*shape, dtype=dtype, device="meta")

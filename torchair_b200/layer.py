@@ -12,6 +12,18 @@ import torch
 from . import dense, ops  # noqa: F401  (register torch.ops.npu.*)
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """Its result, differentiated, raises."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise NotImplementedError("moe_layer has no backward pass: train a shared expert through torch.ops.npu.npu_gated_ffn")
+
+
 def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "", ep_world_size: int = 1,
               ep_rank_id: int = 0, moe_expert_num: int = None, fused: bool = True, after_dispatch=None, shared_w1=None,
               shared_w2=None):
@@ -27,10 +39,20 @@ def moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, *, group_ep: str = "
     the expert GEMMs it disturbs the step less than next to the latency-bound exchange at the step's start.
 
     shared_w1 [H, 2 I_s], shared_w2 [I_s, H] (both or neither, of x's dtype): a shared expert in 16 bits.  Every token passes
-    through it (npu_gated_ffn) and the combine adds its row before the one rounding of the result.
+    through it (npu_gated_ffn) and the combine adds its row before the one rounding of the result.  The layer is for inference: its
+    routed experts and the combine have no gradients.  With a shared expert, a gradient of the result with respect to x or the shared
+    weights raises when it is asked for (under torch.compile torch's own rules for operators without one hold).
     """
     if (shared_w1 is None) != (shared_w2 is None):
         raise RuntimeError("moe_layer: a shared expert needs both shared_w1 and shared_w2")
+    if shared_w1 is not None and torch.is_grad_enabled() and not torch.compiler.is_compiling() and any(
+            t.requires_grad for t in (x, shared_w1, shared_w2)):
+        with torch.no_grad():
+            out = moe_layer(x, expert_ids, expert_scales, w1, s1, w2, s2, group_ep=group_ep, ep_world_size=ep_world_size,
+                            ep_rank_id=ep_rank_id, moe_expert_num=moe_expert_num, fused=fused,
+                            after_dispatch=after_dispatch and torch.enable_grad()(after_dispatch),
+                            shared_w1=shared_w1, shared_w2=shared_w2)
+        return _ForwardOnly.apply(out, x, shared_w1, shared_w2)
     npu = torch.ops.npu
     R = ep_world_size
     E = moe_expert_num if moe_expert_num is not None else w1.shape[0] * R
