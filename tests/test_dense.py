@@ -434,6 +434,25 @@ def test_checkpoint_weight_grad(dev, case, dtype):
     assert torch.equal(npu.npu_checkpoint_weight_grad(q.view(1, m, k), s.view(1, m, -1), dy.view(1, m, n)), npu.npu_checkpoint_weight_grad(q, s, dy))
 
 
+@pytest.mark.gpu
+def test_checkpoint_weight_grad_beyond_the_range_of_fp16(dev):
+    """The input goes into the product in the gradient's type: what does not fit becomes infinite or zero there, as a cast makes it, and
+    stays in its own rows of the result; bf16 has the range."""
+    g = gen(20)
+    size = torch.cat((torch.ones(64), torch.full((64,), 1e6), torch.full((2,), 1e-9))).to(dev)
+    x = (1 + torch.rand(48, 130, generator=g, device=dev)) * size
+    q, s = npu.npu_checkpoint_quant(x)
+    for dtype in DTYPES:
+        dy = make(g, 48, 72, dtype=dtype)
+        got = npu.npu_checkpoint_weight_grad(q, s, dy)
+        x64 = deq64(q, s).to(dtype).double()
+        ok = slice(0, 64) if dtype == torch.float16 else slice(0, 130)
+        want, e = mm(x64[:, ok].t(), dy.double())
+        check(got[ok], want, e, "in range")
+        if dtype == torch.float16:
+            assert not torch.isfinite(got[64:128]).any() and (got[128:] == 0).all()
+
+
 # ---- layouts, sizes, values ----------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_operands_of_other_strides(dev):

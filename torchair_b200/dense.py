@@ -4,6 +4,8 @@
     npu_linear_act(x, weight)              y = act(x weight + bias) + residual
     npu_checkpoint_quant / _dequant        activations kept in int8, one fp32 scale per row and 64 values
     npu_checkpoint_weight_grad             x^T grad of a linear layer whose x was kept so
+                                           (x = q scale is rounded to grad's type first: it has to lie in its range, beyond 65504
+                                           it is infinite in fp16 and below 2^-25 zero)
 
 Weights are [in, out] like the grouped operators' [E, K, N]; a transposed view of an [out, in] parameter is used as it is.
 The gate half of weight1 comes first (activate_left of npu_dequant_swiglu_quant).  bf16 and fp16; products and epilogues are
