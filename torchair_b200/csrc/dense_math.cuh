@@ -61,7 +61,9 @@ __device__ __forceinline__ uint64_t logistic2(uint64_t u) { return rcp_f32x2(add
 
 // Normal distribution function c = (1 + erf(z / sqrt 2)) / 2 and e = exp(-z^2 / 2), by Abramowitz and Stegun 7.1.26: with
 // x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x), erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2) within 1.5e-7.  The exponential serves
-// the derivative as well; erff takes about twice the instructions and a branch.
+// the derivative as well; erff takes about twice the instructions and a branch.  GELU is within 2.1e-7 of its value everywhere; relative
+// to the value that is 5e-5 at z = -3, 5e-4 at -4 (half an fp16 step there), 1.6e-3 at -5, 3.6e-3 at -6 (half a bf16 step) and 1e-2 at -8.
+// 1 + erff is closer down to about -4.5 and cancels below: 4e-2 off at -5, nothing left at -6.
 __device__ __forceinline__ void normal_cdf(uint64_t z, uint64_t& c, uint64_t& e) {
   const float2 f = from_f32x2(z);
   const uint64_t t = rcp_f32x2(fma_f32x2(f32x2(fabsf(f.x), fabsf(f.y)), splat(0.3275911f * kInvSqrt2), splat(1.f)));

@@ -9,7 +9,8 @@
 
 Weights are [in, out] like the grouped operators' [E, K, N]; a transposed view of an [out, in] parameter is used as it is.
 The gate half of weight1 comes first (activate_left of npu_dequant_swiglu_quant).  bf16 and fp16; products and epilogues are
-fp32, rounded once per result.  The first two are differentiable: the values before the activation are kept for the backward
+fp32.  A layer's result is rounded once; a block's hidden rows are rounded to 16 bits before the second product, as its operand, and so
+are the derivatives that the gradient products take.  The first two are differentiable: the values before the activation are kept for the backward
 pass in the input's type, or, with checkpoint_int8, together with x in 8 bits.  The backward pass then differentiates at the
 kept values.  The *_keep and *_backward forms are what the gradients are made of; they and the checkpoint operators are not
 differentiable themselves: a gradient through them raises when it is asked for.  Forward-mode differentiation raises everywhere.
