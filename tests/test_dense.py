@@ -1204,3 +1204,24 @@ def test_jvp_raises():
         x, w = torch.empty(4, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(64, 32, dtype=torch.bfloat16, device="cuda")
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda v: npu.npu_linear_act(v, w), (x,), (torch.ones_like(x),))
+
+
+def test_another_torch_rebuilds_the_library(tmp_path, monkeypatch):
+    """The PyTorch side is compiled again when the installed torch is not the one it was compiled against, and only then."""
+    import subprocess
+    from torchair_b200 import _build
+    lib, calls = tmp_path / "lib.so", []
+
+    def compiler(cmd, **kwargs):
+        calls.append(cmd)
+        lib.write_bytes(b"")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(_build, "TORCH_LIB_PATH", str(lib))
+    monkeypatch.setattr(_build, "TORCH_STAMP_PATH", str(lib) + ".torch", raising=False)
+    monkeypatch.setattr(_build.subprocess, "run", compiler)
+    for built_against, compiles in ((None, 1), (None, 1), ("another", 2), (None, 2)):
+        if built_against:
+            (tmp_path / "lib.so.torch").write_text(built_against)
+        _build.build_torch_library()
+        assert len(calls) == compiles

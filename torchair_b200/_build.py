@@ -11,6 +11,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libtorchair_b200.so")
 TORCH_SOURCE = os.path.join(CSRC, "torch_dense.cpp")
 TORCH_LIB_PATH = os.path.join(PKG_DIR, "libtorchair_b200_torch.so")
+TORCH_STAMP_PATH = TORCH_LIB_PATH + ".torch"      # the torch it was compiled against: its C++ interface changes with every version
 SOURCES = ["api.cu", "quant.cu", "routing.cu", "gmm_i8.cu", "gmm_finalize.cu", "ep_peer.cu", "dense.cu", "checkpoint.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
@@ -30,10 +31,24 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def torch_built_against() -> str:
+    """The torch that libtorchair_b200_torch.so was compiled against ("" where that is not known)."""
+    try:
+        with open(TORCH_STAMP_PATH) as f:
+            return f.read()
+    except FileNotFoundError:
+        return ""
+
+
+def torch_installed() -> str:
+    import torch
+    return f"{torch.__version__} cxx11abi={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
 def build_torch_library(force: bool = False) -> str:
     """Compiles the PyTorch side of the dense operators against the installed torch and links it to libtorchair_b200.so."""
     api = os.path.join(PKG_DIR, "..", "include", "tab_api.h")
-    if not force and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, api]):
+    if not force and torch_built_against() == torch_installed() and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, api]):
         return TORCH_LIB_PATH
     import torch
     from torch.utils.cpp_extension import include_paths
@@ -46,6 +61,8 @@ def build_torch_library(force: bool = False) -> str:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {TORCH_SOURCE}:\n{r.stdout}\n{r.stderr}")
+    with open(TORCH_STAMP_PATH, "w") as f:
+        f.write(torch_installed())
     return TORCH_LIB_PATH
 
 

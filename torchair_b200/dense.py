@@ -214,6 +214,12 @@ for _name, _meta in (
     _npu.impl(_name, _meta, "Meta")
 
 if os.path.exists(_lib.TORCH_LIB_PATH):
+    if os.path.exists(_lib.TORCH_LIB_PATH + ".torch"):       # written by _build.py
+        with open(_lib.TORCH_LIB_PATH + ".torch") as _f:
+            _built = _f.read()
+        if not _built.startswith(torch.__version__ + " "):
+            raise RuntimeError(f"{_lib.TORCH_LIB_PATH} was built against torch {_built}, installed is {torch.__version__}: build it "
+                               "again with `python torchair_b200/_build.py`")
     torch.ops.load_library(_lib.TORCH_LIB_PATH)
 else:
     def _missing(*args, **kwargs):
