@@ -481,6 +481,11 @@ TAB_API int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t ld
                           int64_t w2_rows, int dtype, int64_t M, int64_t H, int64_t I, const void* bias1, const void* bias2, const void* residual,
                           int act, void* keep, int8_t* keep_q, float* keep_scale, int64_t keep_ld, void* y, void* workspace,
                           size_t workspace_bytes, tab_stream_t stream);
+/* tab_dense_plan: which kernel a product of these takes, for profiles and tests; no device is needed.  gated 0: tab_dense_matmul, 1: the
+ *   first product of tab_gated_ffn (N = I), 2: tab_gated_matmul_grad (N = I); a_mn as above.  plan[0] = rows of a tile of the narrow kernel, 0: the pair
+ *   kernel with tiles of 256 rows; plan[1] = tiles; plan[2] = CTAs (pairs) that share the contraction of a tile, of the last plan[3] tiles
+ *   only on pairs. */
+TAB_API int tab_dense_plan(int gated, int64_t M, int64_t N, int64_t K, int a_mn, int64_t* plan);
 TAB_API int tab_dense_status(int* status_host, tab_stream_t stream);
 TAB_API int tab_dense_status_reset(tab_stream_t stream);
 

@@ -372,6 +372,92 @@ def test_gradients_against_differences(dev, act):
         assert (got - slope).abs() <= bound, f"{i}: {got} {slope} {bound}"
 
 
+# ---- the forms that the choice of kernel leads to ------------------------------------------------------------------------
+# together with the lists above, every kernel, tile height and kind of split that the three products of a block can take
+FFN_FORMS = [
+    (1024, 2048, 1024, False, "silu", False, True),
+    (2001, 1024, 1024, True, "gelu", True, False),
+    (701, 4096, 2048, False, "silu", True, False),
+    (1000, 4096, 1024, True, "gelu_tanh", True, True),
+    (3000, 4096, 2048, False, "silu", False, False),
+    (2000, 64, 264, True, "silu", True, False),
+    (3001, 4096, 8, False, "relu", True, True),
+    (4095, 64, 520, False, "silu", True, True),
+    (33, 64, 8, True, "none", True, False),
+    (2999, 4096, 136, True, "gelu_tanh", True, False),
+    (1023, 1024, 1001, False, "silu", True, False),
+]
+LINEAR_FORMS = [
+    (3001, 3000, 8, False, "gelu", True, True),
+    (4097, 2000, 520, False, "silu", True, False),
+    (4100, 520, 2000, True, "none", False, True),
+    # results whose rows are not whole 16-byte pieces
+    (3000, 4096, 5, False, "silu", True, True),
+    (9, 1000, 517, True, "gelu", True, True),
+    (17, 1500, 261, False, "relu", True, False),
+    (40, 2001, 263, True, "gelu_tanh", False, True),
+    (129, 4096, 7165, False, "silu", True, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", FFN_FORMS, ids=str)
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_gated_ffn_in_every_form(dev, case, dtype):
+    test_gated_ffn(dev, case, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+@pytest.mark.parametrize("case", FFN_FORMS, ids=str)
+def test_gated_ffn_gradients_in_every_form(dev, case, int8):
+    test_gated_ffn_gradients(dev, case, int8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True], ids=["keep16", "keep8"])
+@pytest.mark.parametrize("case", LINEAR_FORMS, ids=str)
+def test_linear_act_gradients_in_every_form(dev, case, int8):
+    test_linear_act(dev, case, DTYPES[int8])
+    test_linear_act_gradients(dev, case, int8)
+
+
+def _forms(gated, m, n, k, a_mn=0):
+    """The kernel forms of one product: (product, kernel, rows of a tile or share, ...)."""
+    import ctypes
+    plan = (ctypes.c_int64 * 4)()
+    _lib.call("tab_dense_plan", gated, m, n, k, a_mn, plan)
+    rows, tiles, share, rest = plan
+    name = ("linear", "linear mn")[a_mn] if gated == 0 else ("glu", "glu grad")[gated - 1]
+    if gated == 0 and n % 8:
+        name = "linear any"
+    if rows:
+        assert rows in (16, 32, 64, 128, 256) and tiles >= -(-m // rows) and 1 <= share <= 8 and share <= -(-k // 64)
+        return {(name, "narrow", rows, share > 1)}
+    assert rest <= tiles and share in (1, 2, 4) and (share > 1) == (rest > 0)
+    return ({(name, "pair", 1)} if rest < tiles else set()) | ({(name, "pair", share)} if rest else set())
+
+
+def test_every_form_that_the_choice_of_kernel_leads_to_is_tested(built_library):
+    """The plans over a grid of sizes, and those of the cases above: a change of the estimates that leads to a form without a case fails
+    here."""
+    tested = set()
+    for m, h, inner, *_ in FFN + FFN_FORMS:
+        i8 = -(-inner // 8) * 8
+        tested |= _forms(1, m, i8, h) | _forms(0, m, h, inner) | _forms(2, m, i8, h) | _forms(0, m, h, 2 * i8)
+        tested |= _forms(0, h, 2 * i8, m, 1) | _forms(0, inner, h, m, 1)
+    for m, k, n, transposed, *_ in LINEAR + LINEAR_FORMS:
+        tested |= _forms(0, m, n, k) | _forms(0, m, k, n) | (_forms(0, n, k, m, 1) if transposed else _forms(0, k, n, m, 1))
+    reached = set()
+    for m in (1, 16, 17, 32, 33, 64, 65, 80, 100, 128, 129, 160, 200, 256, 257, 300, 384, 400, 512, 600, 700, 1000, 1024, 1500, 2000, 2048, 4096):
+        for n in (5, 8, 64, 72, 128, 136, 200, 256, 261, 264, 517, 520, 640, 768, 1000, 1024, 1408, 2048, 2056, 2816, 4096, 7165, 7168, 8192):
+            for k in (8, 64, 128, 200, 256, 512, 768, 1024, 1536, 2048, 4096, 7168, 8192, 16384):
+                for gated, a_mn in ((0, 0), (0, 1), (1, 0), (2, 0)) if n % 8 == 0 else ((0, 0),):
+                    reached |= _forms(gated, m, n, k, a_mn)
+    assert reached <= tested, sorted(reached - tested)
+    assert len(reached) > 30
+
+
 # ---- 8-bit checkpoints ---------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES + [torch.float32], ids=str)

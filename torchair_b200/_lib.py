@@ -65,6 +65,7 @@ SIGNATURES = {
     "tab_gated_matmul_grad": [_P, _L, _P, _L, _I, _I, _L, _L, _L, _I, _P, _P, _P, _L, _P, _P, _P],
     "tab_gated_ffn_workspace_bytes": [_L, _L, _L, POINTER(c_size_t)],
     "tab_gated_ffn": [_P, _L, _P, _L, _I, _P, _L, _I, _L, _I, _L, _L, _L, _P, _P, _P, _I, _P, _P, _P, _L, _P, _P, c_size_t, _P],
+    "tab_dense_plan": [_I, _L, _L, _L, _I, POINTER(_L)],
     "tab_dense_status": [POINTER(c_int), _P],
     "tab_dense_status_reset": [_P],
     "tab_checkpoint_quant": [_P, _I, _L, _L, _L, _P, _L, _P, _L, _P],

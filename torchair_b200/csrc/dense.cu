@@ -132,15 +132,21 @@ static int pair_split(int64_t tiles, int num_kb) {
   return tiles <= 15 ? 4 : tiles <= 33 ? 2 : 1;
 }
 
+// Whole tiles for the turns that fill all pairs, clusters for the `rest` where that is shorter than another whole turn.
+static int pair_rest(int64_t tiles, int pairs, int num_kb, int64_t& rest) {
+  rest = tiles % pairs;
+  const int split = rest ? pair_split(rest, num_kb) : 1;
+  if (split == 1) rest = 0;
+  return split;
+}
+
 template <typename T, int EPI>
 static int launch_pair_t(const char* op, const CUtensorMap& ma, const CUtensorMap& mb, DenseParams& p, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0}, done_split{0};
   const int64_t tiles = static_cast<int64_t>(p.row_tiles) * p.col_tiles;
   const int pairs = dense_sms() / 2;
-  // whole tiles for the turns that fill all pairs, clusters for the rest where that is shorter than another whole turn
-  int64_t rest = tiles % pairs;
-  const int split = rest ? pair_split(rest, p.num_kb) : 1;
-  if (split == 1) rest = 0;
+  int64_t rest;
+  const int split = pair_rest(tiles, pairs, p.num_kb, rest);
   const int64_t whole = tiles - rest;
   int rc = TAB_OK;
   if (whole > 0) {
@@ -281,11 +287,15 @@ static_assert(narrow_fits(16, kNwMaxSplit, 5) && narrow_fits(32, kNwMaxSplit, 4)
               narrow_fits(128, kNwMaxSplit, 4) && narrow_fits(256, 1, 4), "shared memory of the narrow kernel");
 
 // Which kernel: the one with the lower estimate.
+static bool narrow_is_chosen(const NarrowPlan& plan, int64_t M, int64_t N, int num_kb, int epi) {
+  return plan.nt != 0 && plan.cost <= pair_cost(M, N, num_kb, epi, dense_sms() / 2);
+}
+
 template <int EPI>
 static int launch_dense(const char* op, int dtype, const DenseOperand& a, const DenseOperand& b, DenseParams& p, cudaStream_t st) {
   const int num_kb = (int)((a.depth + kDnBlockK - 1) / kDnBlockK);
   const NarrowPlan plan = narrow_plan(p.M, p.N, num_kb, EPI, a.mn != 0);
-  if (plan.nt != 0 && plan.cost <= pair_cost(p.M, p.N, num_kb, EPI, dense_sms() / 2)) return launch_narrow_epi<EPI>(op, dtype, a, b, p, plan, st);
+  if (narrow_is_chosen(plan, p.M, p.N, num_kb, EPI)) return launch_narrow_epi<EPI>(op, dtype, a, b, p, plan, st);
   return launch_pair_epi<EPI>(op, dtype, a, b, p, st);
 }
 
@@ -436,6 +446,30 @@ extern "C" int tab_gated_ffn(const void* x, int64_t ldx, const void* w1, int64_t
   // the hidden columns behind w2_rows meet no row of w2 and are not read: a row of infinities leaves NaN there
   const DenseOperand oh = {workspace, I, M, w2_rows, 0};
   return linear_matmul(op, oh, o2, dtype, M, H, bias2, residual, TAB_ACT_NONE, nullptr, nullptr, nullptr, 0, y, 1, 0, st);
+}
+
+extern "C" int tab_dense_plan(int gated, int64_t M, int64_t N, int64_t K, int a_mn, int64_t* plan) {
+  const char* op = "dense_plan";
+  int rc = check_dense(op, TAB_BF16, M, N, K, TAB_ACT_NONE);
+  if (rc != TAB_OK) return rc;
+  if (!plan || gated < 0 || gated > 2 || M == 0) return fail(TAB_ERR_BAD_ARG, "%s: gated=%d M=%lld", op, gated, (long long)M);
+  const int epi = gated == 0 ? kEpiLinear : gated == 1 ? kEpiGlu : kEpiGluGrad, num_kb = (int)((K + kDnBlockK - 1) / kDnBlockK);
+  const int64_t n8 = (N + 7) / 8 * 8;
+  const NarrowPlan narrow = narrow_plan(M, n8, num_kb, epi, a_mn != 0);
+  if (narrow_is_chosen(narrow, M, n8, num_kb, epi)) {
+    plan[0] = narrow.nt;
+    plan[1] = static_cast<int64_t>(narrow.row_tiles) * narrow.col_tiles;
+    plan[2] = narrow.split;
+    plan[3] = 0;
+  } else {
+    const int64_t cols = epi == kEpiGlu ? 128 : 256;
+    int64_t rest;
+    plan[0] = 0;
+    plan[1] = ((M + 255) / 256) * ((n8 + cols - 1) / cols);
+    plan[2] = pair_rest(plan[1], dense_sms() / 2, num_kb, rest);
+    plan[3] = rest;
+  }
+  return TAB_OK;
 }
 
 extern "C" int tab_dense_status_reset(tab_stream_t stream) {
