@@ -458,6 +458,20 @@ def test_every_form_that_the_choice_of_kernel_leads_to_is_tested(built_library):
     assert len(reached) > 30
 
 
+def test_few_rows_share_tiles_as_far_as_all_ctas_are_resident(built_library):
+    """The rule for up to 64 rows, at every number of tiles: the largest cluster of which the GPU holds enough at a time."""
+    import ctypes
+    room = {1: 148, 2: 148, 3: 135, 4: 132, 5: 130, 6: 132, 7: 105, 8: 120}        # CTAs in clusters of that size, one to an SM
+    plan = (ctypes.c_int64 * 4)()
+    for m, per_sm in ((1, 2), (8, 2), (32, 2), (33, 1), (64, 1)):
+        for k in (64, 640, 1408, 8192):
+            for tiles in range(1, 400):
+                for gated, features in ((0, 128), (1, 64), (2, 128)):
+                    _lib.call("tab_dense_plan", gated, m, tiles * features, k, 0, plan)
+                    fit = [s for s in room if s == 1 or tiles * s <= per_sm * room[s] and s * 5 <= -(-k // 64)]
+                    assert list(plan)[1:3] == [tiles, max(fit)], (m, k, tiles, gated)
+
+
 # ---- 8-bit checkpoints ---------------------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES + [torch.float32], ids=str)

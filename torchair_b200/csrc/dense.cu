@@ -201,14 +201,15 @@ static NarrowPlan narrow_plan(int64_t M, int64_t N, int num_kb, int epi, bool x_
     best.nt = x_mn ? 64 : M <= 16 ? 16 : M <= 32 ? 32 : 64;       // (boxes of 64 rows where x is contiguous along its rows)
     best.row_tiles = 1;
     best.col_tiles = (int)col_tiles;
-    // CTAs per tile: up to 32 rows as many as put two on half of the SMs.  Measured in a row over weights that come from HBM (us): 8 rows,
-    // 56 tiles of K = 2048: 9.9 / 9.5 / 9.1 / 10.7 with 2 / 3 / 4 / 5 CTAs; 16 rows, 32 tiles of K = 4096: 11.1 / 10.7 / 10.4 / 10.0 / 9.9
-    // with 3 / 4 / 5 / 7 / 8.  With 64 rows the parts to exchange weigh more, 56 tiles of K = 2048: 11.7 / 12.9 / 12.2 / 14.3 with 2 / 3 /
-    // 4 / 5.  A part of fewer than 5 blocks does not pay: 32 rows, 32 tiles of K = 1408: 6.8 / 6.5 / 7.3 with 3 / 4 / 5.
-    int64_t split = (best.nt <= 32 ? 224 : 132) / col_tiles;
-    if (split > kNwMaxSplit) split = kNwMaxSplit;
-    if (split > num_kb / 5) split = num_kb / 5;
-    best.split = split < 1 ? 1 : (int)split;
+    // CTAs per tile: the most with which all are resident at a time, two to an SM up to 32 rows, one with 64 (where the parts to exchange weigh
+    // more), and parts of at least 5 blocks.  Of all numbers up to 8 at 14 tile counts from 5 to 148 and K = 1408 .. 7168, weights from HBM,
+    // this one takes 2 % longer than the fastest on average.  8 rows, K = 4096, us with 1 .. 8 CTAs to one of 20 tiles: 16.3 11.4 9.7 9.1 8.8
+    // 8.8 8.5 8.2; of 48: 16.7 13.3 12.2 12.2 11.9, then a second turn: 17.6 17.1 16.6; of 110: 21.6 21.5, then 26.9 .. 33.9.  64 rows, 40 tiles:
+    // 18.5 14.6 12.8, then 15.0 and more.  Shorter parts: 8 rows, 40 tiles of K = 512: 4.3 with one CTA, 5.1 to 9.3 with more.
+    const int per_sm = best.nt <= 32 ? 2 : 1;
+    best.split = 1;
+    for (int split = 2; split <= kNwMaxSplit && split * 5 <= num_kb; ++split)
+      if (col_tiles * split <= per_sm * kClusterRoom[split]) best.split = split;
     best.cost = 0.0;                           // never slower than a 256-row tile: the same weights, less of everything else
     return best;
   }
