@@ -15,8 +15,10 @@
 // A launch of this kernel is over in 5 to 15 us, so its start counts: the producer sets up its barriers and asks for the first
 // weights before the CTA's threads have met and tensor memory is allocated.
 //
-// A launch marked `dependent` (the second projection of a feed-forward block) fills its ring with weights before it waits for
-// the kernel that writes x.
+// A launch marked `dependent` (the second projection of a feed-forward block) asks for weights before it waits for the kernel that writes
+// x, in those of its CTAs that find room beside that kernel's.  Those are few when the first projection has no more CTAs than SMs, for
+// each then takes all of its SM's shared memory: 37 rows, 4096 -> 1408: 132 of them leave 16 SMs to the second one's 128 CTAs; one row of
+// 7168 -> 2048: 192 half-SM places of 296 are taken, 104 of the second one's 224 CTAs find room.
 #pragma once
 
 #include "dense_common.cuh"
