@@ -1162,6 +1162,30 @@ def test_a_gradient_through_moe_layer_raises(dev, leaf):
     assert modes == [True, True, False], "the caller's own work runs in the caller's mode"
 
 
+@pytest.mark.gpu
+def test_moe_layer_with_a_shared_expert_compiled(dev):
+    """One graph, shared weights that require gradients included."""
+    from oracle import moe_oracle as O
+    from torchair_b200.layer import moe_layer
+    cfg = O.CONFIGS["cfg0"]
+    w = O.make_weights(cfg, seed=3)
+    x, ids, wt = (t.to(dev) for t in O.make_tokens(cfg, seed=3))
+    routed = [t.to(dev) for t in (w.w1, w.s1, w.w2, w.s2)]
+    g = gen(2)
+    shared = [weight(g, x.shape[1], 512, True, x.dtype).detach().requires_grad_(), weight(g, 256, x.shape[1], True, x.dtype).detach().requires_grad_()]
+
+    def fn(x, ids, wt, w1, s1, w2, s2, a, b):
+        return moe_layer(x, ids, wt, w1, s1, w2, s2, shared_w1=a, shared_w2=b)
+
+    config = torchair_b200.CompilerConfig()
+    config.mode = "reduce-overhead"
+    compiled = torch.compile(fn, backend=torchair_b200.get_npu_backend(compiler_config=config), fullgraph=True, dynamic=False)
+    with torch.no_grad():
+        want = fn(x, ids, wt, *routed, *shared)
+        for _ in range(3):
+            assert torch.equal(compiled(x, ids, wt, *routed, *shared), want)
+
+
 # ---- refusals (CPU) ------------------------------------------------------------------------------------------------------
 def _meta(*shape, dtype=torch.bfloat16):
     return torch.empty(*shape, dtype=dtype, device="meta")
